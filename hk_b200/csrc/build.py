@@ -44,6 +44,8 @@ LIBRARIES: Dict[str, str] = {
     "attention_flash": "attention_flash.cu",
     "attention_prefill_tc": "attention_prefill_tc.cu",
     "attention_latent": "attention_latent.cu",   # attention over a compressed cache whose rows are wider than a flash head
+    "attention_tree": "attention_tree.cu",       # attention of drafted token trees over the paged cache
+    "branches": "branches.cu",         # a cache's blocks copied, accepted rows moved up, the choice over beams and vocabulary
     "gemm_heads": "gemm_heads.cu",     # one small tensor-core product per head (a latent attention's up-projections)
     "recurrent": "recurrent.cu",       # scans of the recurrent mixers (delta rules, minGRU, matrix memory, retention)
     "delta_chunks": "delta_chunks.cu", # the same recurrences (but for minGRU) for prompt portions, in chunks of tokens

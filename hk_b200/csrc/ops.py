@@ -1511,4 +1511,144 @@ def zero_slot(table: torch.Tensor, slot: int, most_bytes: int) -> None:
     _check(build.load("elementwise").hk_zero_slot(_ptr(table), int(table.shape[0]), slot, most_bytes, _stream()), "zero_slot")
 
 
+# ---- several continuations of one request --------------------------------------------------
+
+
+TREE_TOKENS = 256       # drafted tokens of a request
+
+
+def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, n_heads: int, n_kv_heads: int, head_dim: int,
+                   page_tokens: int, window: int, scale: float, most_tokens: int, most_keys: int, all_keys: int = 0, sink: bool = False,
+                   sinks=None, softcap: float = 0.0) -> None:
+    """Attention of drafted token trees over the paged cache: out[t, h, :] = softmax_j(scale * q[t, h] . k[j]) v[j] over what the
+    token sees.  `requests` int32 [m, 4] = (slot, first row of q, drafted tokens, rows cached before them): a request's drafted
+    tokens are consecutive rows of q and out [n, H*hd], and their keys and values stand in the cache behind its own rows, in the same
+    order.  A token sees all cached rows and the drafted ones whose bits are set in its row of `ancestors` int32 [n, words] (bit j %
+    32 of word j / 32: drafted token j of its request; for a tree its ancestors and itself); with `window` w only those at positions
+    above its own less w, where a cached row's position is its place and a drafted token's is in `positions` int32 [n] (not below the
+    request's cached rows).  A token that sees nothing gives zeros; rows of no request keep what they hold.  sink, sinks, softcap
+    as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them;
+    all_keys: the rows of all requests together, where the caller knows it (0: as if all had the most)."""
+    _need(q, "q", dims=2)
+    _need(out, "out", q.dtype, 2)
+    _need(k_pages, "k_pages", q.dtype, 4)
+    _need(v_pages, "v_pages", q.dtype, 4)
+    _need(block_table, "block_table", torch.int32, 2)
+    _need(requests, "requests", torch.int32, 2)
+    _need(ancestors, "ancestors", torch.int32, 2)
+    _need(positions, "positions", torch.int32, 1)
+    n, H, G, hd = q.shape[0], n_heads, n_kv_heads, head_dim
+    if H < 1 or G < 1 or H % G != 0:
+        raise KernelError(f"tree_attention: {H} heads are not a multiple of {G} groups")
+    if tuple(q.shape) != (n, H * hd) or out.shape != q.shape:
+        raise KernelError("tree_attention: q and out must be [n, H*head_dim]")
+    if tuple(k_pages.shape[1:]) != (G, page_tokens, hd) or v_pages.shape != k_pages.shape:
+        raise KernelError("tree_attention: cache pages must be [pages, G, page_tokens, head_dim]")
+    if hd > 256:
+        raise KernelError(f"tree_attention: head_dim {hd} is above 256")
+    if requests.shape[1] != 4 or ancestors.shape[0] != n or positions.shape[0] != n:
+        raise KernelError("tree_attention: requests must be [m, 4], ancestors [n, words] and positions [n]")
+    if not 1 <= most_tokens <= TREE_TOKENS or most_tokens > 32 * ancestors.shape[1]:
+        raise KernelError(f"tree_attention: up to {most_tokens} drafted tokens a request: 1 to {TREE_TOKENS} are taken, with a bit each in ancestors")
+    if not 1 <= most_keys <= block_table.shape[1] * page_tokens or all_keys < 0:
+        raise KernelError(f"tree_attention: most_keys {most_keys} must be positive and inside the block table, all_keys not negative")
+    if not scale > 0 or not softcap >= 0:
+        raise KernelError("tree_attention: the scale must be positive, the soft cap positive or 0")
+    if sinks is not None:
+        _need(sinks, "sinks", torch.float32, 1)
+        if sinks.shape[0] != H or not sink:
+            raise KernelError("tree_attention: sinks must hold one score per query head (and sink be set)")
+    if not _one_device(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, sinks):
+        raise KernelError("tree_attention: all tensors must be on one device")
+    m = requests.shape[0]
+    if n == 0 or m == 0:
+        return
+    with _on(q):
+        _check(build.load("attention_tree").hk_tree_attention(
+            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _dt(q), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(requests),
+            m, most_tokens, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
+            scale, softcap, 1 if sink else 0, _ptr(sinks), 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
+
+
+def _one_device(first: torch.Tensor, *others) -> bool:
+    index = first.device.index
+    return all(t is None or t.device.index == index for t in others)
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """The device of `t` as the current one (a launch goes to the current device's stream)."""
+    return _here if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device.index)
+
+
+def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, table_stride: int, page_tokens: int, heads: int,
+                 row_bytes: int, num_pages: int) -> None:
+    """Moves the accepted rows of drafted trees up, side by side, in every layer's cache.  `table` int64 [arrays, 4] = (address of
+    pages [num_pages, heads, page_tokens, bytes a row], heads, bytes a row, address of an int32 block table [table_rows,
+    table_stride]) of tensors that the caller keeps; `paths` int32 [requests, 2 + width] = (slot, the tree's first row, its accepted
+    rows in ascending order, -1 behind the last): accepted row i moves to the tree's row i; a slot has one path.  heads, row_bytes:
+    the most of any array."""
+    _need(table, "table", torch.int64, 2)
+    _need(paths, "paths", torch.int32, 2)
+    if table.shape[1] != 4 or paths.shape[1] < 2:
+        raise KernelError("compact_rows: table must be [arrays, 4] and paths [requests, 2 + width]")
+    if min(table_rows, table_stride, page_tokens, heads, row_bytes, num_pages) < 1:
+        raise KernelError("compact_rows: the sizes must be positive")
+    if not _one_device(table, paths):
+        raise KernelError("compact_rows: table and paths must be on one device")
+    with _on(table):
+        _check(build.load("branches").hk_compact_rows(_ptr(table), table.shape[0], _ptr(paths), paths.shape[0], paths.shape[1] - 2, table_rows,
+                                                      table_stride, page_tokens, heads, row_bytes, num_pages, _stream()), "compact_rows")
+
+
+def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> None:
+    """Copies blocks (pages, or requests' slots of a state) inside every array of a cache, in one launch.  `table` int64 [arrays, 5] =
+    (address, blocks, pieces a block, bytes a piece, bytes a row) of tensors that the caller keeps; `moves` int32 [m, 3] = (from,
+    to, rows): of each piece (a key head's rows of a page; a state is one piece and one row) the first `rows` rows are copied.  In one call no block
+    is written twice, and none is both read and written.  most_bytes: the most that a block of any array has."""
+    _need(table, "table", torch.int64, 2)
+    _need(moves, "moves", torch.int32, 2)
+    if table.shape[1] != 5 or moves.shape[1] != 3:
+        raise KernelError("copy_blocks: table must be [arrays, 5] and moves [m, 3]")
+    if most_bytes < 1:
+        raise KernelError("copy_blocks: most_bytes must be positive")
+    if not _one_device(table, moves):
+        raise KernelError("copy_blocks: table and moves must be on one device")
+    with _on(table):
+        _check(build.load("branches").hk_copy_blocks(_ptr(table), table.shape[0], _ptr(moves), moves.shape[0], most_bytes, _stream()), "copy_blocks")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_beams: torch.Tensor,
+                out_tokens: torch.Tensor) -> None:
+    """The best continuations of beams: of all beams k of a prompt and tokens v the out_scores.shape[1] with the largest scores[b, k] +
+    log softmax(logits[b, k])[v], best first, of equal ones the lowest k * vocab + v first.  logits float32 [prompts * n_beams,
+    vocab], scores float32 [prompts * n_beams]; out_scores float32, out_beams (k) and out_tokens (v) int32 [prompts, choices].  A logit
+    that is not finite counts as -inf, and so do all continuations of a beam whose score is not finite (one that is not there yet, or no
+    longer).  Up to 256 beams and 256 choices."""
+    _need(logits, "logits", torch.float32, 2)
+    _need(scores, "scores", torch.float32, 1)
+    _need(out_scores, "out_scores", torch.float32, 2)
+    _need(out_beams, "out_beams", torch.int32, 2)
+    _need(out_tokens, "out_tokens", torch.int32, 2)
+    rows, vocab = logits.shape
+    prompts, choices = out_scores.shape
+    if n_beams < 1 or rows != prompts * n_beams or scores.shape[0] != rows:
+        raise KernelError(f"beam_select: {rows} rows of logits and {scores.shape[0]} scores for {prompts} prompts of {n_beams} beams")
+    if out_beams.shape != out_scores.shape or out_tokens.shape != out_scores.shape:
+        raise KernelError("beam_select: the three results must have one shape")
+    if prompts == 0:
+        return
+    if n_beams > 256 or not 1 <= choices <= min(256, n_beams * vocab) or n_beams * vocab >= 1 << 31:
+        raise KernelError(f"beam_select: {choices} choices of {n_beams} beams and {vocab} tokens; up to 256 beams and 256 choices are taken, no more than there are")
+    if not _one_device(logits, scores, out_scores, out_beams, out_tokens):
+        raise KernelError("beam_select: all tensors must be on one device")
+    lib = build.load("branches")
+    with _on(logits):
+        scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
+        _check(lib.hk_beam_select(_ptr(logits), _ptr(scores), prompts, n_beams, vocab, choices, _ptr(out_scores), _ptr(out_beams), _ptr(out_tokens),
+                                  _ptr(scratch), _stream()), "beam_select", launches=2)
+
+
 from . import attention_fast, gemm_fast  # noqa: E402  (they use this module; looked up once, not on each call)
