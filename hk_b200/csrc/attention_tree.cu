@@ -142,34 +142,29 @@ __device__ __forceinline__ long long warp_sum64(long long v) {
   return v;
 }
 
-// By a whole warp: the tiles of all requests, and of those before request `upto`.
+// By a whole warp: the tiles of all requests.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ void count_tiles(const TreeArgs& a, int upto, long long& before, long long& total) {
-  const int lane = threadIdx.x & 31;
-  long long b = 0, t = 0;
-  for (int r = lane; r < a.n_requests; r += 32) {
-    const long long n = tiles_of<ROWS, KEYS>(a, r);
-    t += n;
-    if (r < upto) b += n;
-  }
-  before = warp_sum64(b);
-  total = warp_sum64(t);
+__device__ __forceinline__ long long count_tiles(const TreeArgs& a) {
+  long long t = 0;
+  for (int r = threadIdx.x & 31; r < a.n_requests; r += 32) t += tiles_of<ROWS, KEYS>(a, r);
+  return warp_sum64(t);
 }
 
 // Where a CTA is in its share.
 struct Walk {
   int r, unit, tile;
   long long left;
+  long long from, total;   // the share's first tile among all; all tiles
 };
 
 // By a whole warp: the start of share `cta` of `ctas`.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Walk share_start(const TreeArgs& a, int cta, int ctas) {
   const int lane = threadIdx.x & 31;
-  long long none, total;
-  count_tiles<ROWS, KEYS>(a, 0, none, total);
-  const long long from = total * cta / ctas, to = total * (cta + 1) / ctas;
-  Walk w = {a.n_requests, 0, 0, to - from};
+  const long long total = count_tiles<ROWS, KEYS>(a);
+  ctas = (int)min((long long)ctas, total);               // no empty share between two of one unit
+  const long long from = cta < ctas ? total * cta / ctas : 0, to = cta < ctas ? total * (cta + 1) / ctas : 0;
+  Walk w = {a.n_requests, 0, 0, to - from, from, total};
   long long base = 0;
   if (to > from) {
     for (int r0 = 0; r0 < a.n_requests; r0 += 32) {
@@ -235,57 +230,78 @@ __device__ __forceinline__ bool next_segment(const TreeArgs& a, Walk& w, Segment
 // that it began (2 cta + 1).
 __device__ __forceinline__ size_t part_slot(int cta, bool begins) { return 2 * (size_t)cta + (begins ? 1 : 0); }
 
-// A warp a row (token, query head): the partial results of the shares that its unit is cut into, in order.
-constexpr int CW = 4;      // warps
-template <typename T, int ROWS, int KEYS>
+// The exponentials' domain: base 2 for bfloat16, natural in float32 (a score times log2(e) would be rounded once more).
+template <typename T>
+__device__ __forceinline__ float power(float x) {
+  return sizeof(T) == 4 ? expf(x) : exp2f(x);
+}
+
+// The partial results of a unit that lies in several shares, merged in order.  A block takes the border between two shares, if it is
+// the first inside its unit, and CR of the unit's rows, a warp a row.
+constexpr int CW = 4, CR = 16;      // warps, rows
+template <typename T, int HD, int ROWS, int KEYS>
 __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a, int ctas) {
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blockIdx.y, group = a.H / a.G;
-  const TreeReq q = load_request(a, r);
-  if (q.count == 0) return;
-  long long before, total;
-  count_tiles<ROWS, KEYS>(a, r, before, total);
+  constexpr int D = HD / 32;        // dims a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
+  const Walk w = share_start<ROWS, KEYS>(a, c, ctas);
+  if (w.left <= 0 || w.tile == 0) return;
+  ctas = (int)min((long long)ctas, w.total);
+  const long long start = w.from - w.tile;
+  if (w.total * (c - 1) / ctas > start) return;
+  const TreeReq q = load_request(a, w.r);
   int t_first, tiles, units;
   unit_shape<ROWS, KEYS>(a, q, t_first, tiles, units);
-  for (int i = blockIdx.x * CW + warp; i < q.count * a.H; i += gridDim.x * CW) {
-    const int token = i / a.H, head = i % a.H, g = head / group, row = token * group + head % group;
-    const long long start = before + (long long)(row / ROWS * a.G + g) * tiles;
-    const int c0 = (int)(((start + 1) * ctas - 1) / total), c1 = (int)(((start + tiles) * ctas - 1) / total);
-    if (c0 == c1) continue;                              // whole in one share: written there
-    float m = -CUDART_INF_F, l = 0.f, acc[8];            // up to 256 dims
+  const int parts = (int)(((start + tiles) * ctas - 1) / w.total) - c + 2;        // shares c - 1, c, ...
+  const int group = a.H / a.G, g = w.unit % a.G, row0 = w.unit / a.G * ROWS, rows = min(ROWS, q.count * group - row0);
+  for (int row = blockIdx.y * CR + warp; row < min(rows, (int)(blockIdx.y + 1) * CR); row += CW) {
+    auto place = [&](int p) { return part_slot(c - 1 + p, p == 0) * a.rows_cap + row; };
+    float m = -CUDART_INF_F;
+    for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(a.part_ml + 2 * place(p)));
+    m = warp_max(m);
+    const float safe = m == -CUDART_INF_F ? 0.f : m;
+    float l = 0.f, acc[D];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const size_t at = part_slot(c, c == c0) * a.rows_cap + row % ROWS;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at);
-      const float mn = fmaxf(m, ml.x), safe = mn == -CUDART_INF_F ? 0.f : mn;
-      const float f0 = exp2f(m - safe), f1 = exp2f(ml.x - safe);
-      l = l * f0 + ml.y * f1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = lane + 32 * e;
-        if (d < a.hd) acc[e] = acc[e] * f0 + __ldcg(a.part_o + at * a.hd + d) * f1;
+    for (int e = 0; e < D; ++e) acc[e] = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+      float f = 0.f;
+      if (p0 + lane < parts) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + place(p0 + lane));
+        f = power<T>(ml.x - safe);
+        l += ml.y * f;
       }
-      m = mn;
-    }
-    if (a.sink) l += exp2f((a.sinks ? a.sinks[head] * 1.4426950408889634f : 0.f) - m);
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-    T* out = reinterpret_cast<T*>(a.out) + ((size_t)(q.first + token) * a.H + head) * a.hd;
+#pragma unroll 4
+      for (int p = p0; p < min(parts, p0 + 32); ++p) {
+        const float* o = a.part_o + place(p) * HD + lane * D;
+        const float fp = __shfl_sync(0xffffffffu, f, p - p0);
+        float x[D];
+        if constexpr (D == 4) *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(o));
+        else *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(o));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = lane + 32 * e;
-      if (d < a.hd) out[d] = from_f32<T>(acc[e] * inv);
+        for (int e = 0; e < D; ++e) acc[e] = fmaf(x[e], fp, acc[e]);
+      }
     }
+    l = warp_sum(l);
+    const int token = (row0 + row) / group, head = g * group + (row0 + row) % group;
+    if (a.sink) {
+      const float score = (a.sinks ? a.sinks[head] : 0.f) * (sizeof(T) == 4 ? 1.0f : 1.4426950408889634f);
+      const float top = fmaxf(m, score), f = m == -CUDART_INF_F ? 0.f : power<T>(m - top);
+      l = l * f + power<T>(score - top);
+#pragma unroll
+      for (int e = 0; e < D; ++e) acc[e] *= f;
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    T* out = reinterpret_cast<T*>(a.out) + ((size_t)(q.first + token) * a.H + head) * HD + lane * D;
+#pragma unroll
+    for (int e = 0; e < D; ++e) out[e] = from_f32<T>(acc[e] * inv);
   }
 }
 
-template <typename T, int ROWS, int KEYS>
+template <typename T, int HD, int ROWS, int KEYS>
 int launch_combine(const TreeArgs& a, int ctas, cudaStream_t s) {
-  const long long rows = (long long)a.most_tokens * a.H;
-  const long long blocks = (rows + CW - 1) / CW;
-  return hk_launch_pdl(tree_combine_kernel<T, ROWS, KEYS>, dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)a.n_requests), dim3(CW * 32), 0, s,
-                       a, ctas);
+  if (ctas < 2) return 0;
+  return hk_launch_pdl(tree_combine_kernel<T, HD, ROWS, KEYS>, dim3((unsigned)(ctas - 1), (unsigned)((a.rows_cap + CR - 1) / CR)), dim3(CW * 32), 0, s, a,
+                       ctas);
 }
 
 // ---- any size: a block a (token, query head) -------------------------------------------------------------------------------
@@ -373,6 +389,858 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
   return hk_launch(tree_generic_kernel<T>, dim3((unsigned)blocks), dim3(GW * 32), 0, s, a);
 }
 
+// ---- bfloat16 on the tensor cores ---------------------------------------------------------------------------------------------
+// A tile has up to 256 rows.  Two groups of four softmax warps (a thread a row), one lane that issues the products and one warp that
+// loads K and V by TMA work on it side by side: with more than 128 rows each group has half of them and every key tile serves both;
+// with up to 128 rows both groups have the same rows and take the key tiles in turn, and their sums meet in tensor memory at the end.
+// Either way one group's exponentials run while the tensor core works for the other.  Tensor memory (512 columns): per group 128
+// columns of scores, which the probabilities overwrite (bfloat16, 64 columns), and HD of sums.  A group's next scores are issued
+// behind its product with V; products of one thread run in order, so they overwrite P only once it was read.
+//
+// Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits): they are at most 2^8 times a power of
+// two that is the row's reference maximum, an integer, so that moving it rounds nothing.
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 320;
+constexpr uint32_t WAIT_LIMIT = 1u << 17;   // tries of about 100 ns each: some 13 ms, far beyond any legitimate wait
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Waits for the phase of this parity, a bounded number of tries; false (and the flag set) if it did not come or another gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (i >= 4) __nanosleep(100);      // a waiting warp must not take issue slots from the working ones
+    if ((i & 255u) == 255u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+// The same for what is still on its way when the kernel gives up.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++i) __nanosleep(100);
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Shared-memory matrix descriptors, 128-byte swizzle, version 1 (sm_100); 8-row groups lie 1024 bytes apart.
+// K-major ([row][64 elements = 128 bytes]): leading offset unused.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// MN-major ([k row][64 elements of the MN dimension]): the next 64 MN elements `lbo` bytes further (leading).
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The same with the A operand in tensor memory (128 lanes = rows, 8 columns of two bf16 each per 16 k).
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {      // 2^x, one instruction; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// Barrier 1 among the 256 softmax threads; whether any of them says so.
+__device__ __forceinline__ bool softmax_any(bool said) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"(said ? 1u : 0u) : "memory");
+  return any != 0;
+}
+// byte offset of (row r, 16-byte chunk c along the row) in a [halves][128 rows][128 bytes] swizzled tile
+__device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+
+template <int HD>
+struct TcSmem {
+  static constexpr int STAGES = HD == 64 ? 4 : 2;      // of K, and of V
+  alignas(1024) uint8_t q[2][TC_ROWS * HD * 2];
+  alignas(1024) uint8_t k[STAGES][TC_KEYS * HD * 2];
+  alignas(1024) uint8_t v[STAGES][TC_KEYS * HD * 2];
+  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], drained;
+  float2 ml[2][TC_ROWS];      // a row's reference maximum and sum in either group
+  Walk start;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// The dims [c0, c0 + 32 D) of one row's sums over the keys of a segment that it sees, against the reference maximum m, by one warp in
+// 32 bits.  For a row whose sums came out NaN or Inf: the tensor core's product takes whole tiles of values, and a probability of zero
+// does not keep out a NaN or Inf among those that the row does not see.
+template <int D>
+__device__ __noinline__ void tree_row_again(const TreeArgs& a, const Segment& s, int row, int c0, float m, float cap_log2, float cap_in2, float (&acc)[D]) {
+  const int lane = threadIdx.x & 31, group = a.H / a.G, hd = a.hd;
+  const int token = (s.row0 + row) / group, head = s.g * group + (s.row0 + row) % group;
+  const TreeRow w = tree_row(a, s.q, token, true);
+  const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * hd;
+  const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
+  const float safe = m == -CUDART_INF_F ? 0.f : m, scale_log2 = a.scale * 1.4426950408889634f;
+#pragma unroll
+  for (int e = 0; e < D; ++e) acc[e] = 0.f;
+  for (int j0 = s.t0 * TC_KEYS; j0 < min((s.t0 + s.n) * TC_KEYS, s.q.context + s.q.count); j0 += 32) {
+    const uint32_t see = visible32(w, j0);
+    if (see == 0) continue;
+    float p = 0.f;
+    long long at = -1;
+    if ((see >> lane) & 1u) {
+      const int j = j0 + lane, page = bt[j / a.page_tokens];
+      if (page >= 0 && page < a.num_pages) {
+        at = (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * hd;
+        const bf16* k = reinterpret_cast<const bf16*>(a.k) + at;
+        float x = 0.f;
+        for (int d = 0; d < hd; ++d) x = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), x);
+        p = exp2f(log2_score(x, scale_log2, cap_log2, cap_in2) - safe);
+      }
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, at >= 0); left; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      const float f = __shfl_sync(0xffffffffu, p, i);
+      const bf16* v = reinterpret_cast<const bf16*>(a.v) + __shfl_sync(0xffffffffu, at, i) + c0 + lane * D;
+#pragma unroll
+      for (int e = 0; e < D; ++e) acc[e] = fmaf(f, __bfloat162float(v[e]), acc[e]);
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeArgs a, float cap_log2, float cap_in2) {
+  constexpr int STAGES = TcSmem<HD>::STAGES, CPR = HD / 8, KSTEPS = HD / 16, HALVES = HD / 64;
+  constexpr uint32_t TMEM_COLS = 512, SP_COL[2] = {0, 128}, O_COL[2] = {256, 256 + HD};
+  // fp32 accumulators, bf16 operands; N at bit 17 (>> 3), M at bit 24 (>> 4); bit 16: B is MN-major
+  constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC_KEYS >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+  constexpr uint32_t IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+
+  extern __shared__ uint8_t smem_raw[];
+  TcSmem<HD>& sm = *reinterpret_cast<TcSmem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  volatile int* abort_flag = &sm.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.G;
+
+  // The V stages start as zeros: rows of a tile that no box is copied to are multiplied by a probability of zero, which must not meet
+  // a NaN pattern.  K needs none: a score of such a key is masked before it is looked at.
+  {
+    uint4* z = reinterpret_cast<uint4*>(sm.v[0]);
+    constexpr int N16 = STAGES * TC_KEYS * HD * 2 / 16;
+    for (int i = threadIdx.x; i < N16; i += TC_THREADS) z[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (threadIdx.x == 32) {
+    mbar_init(&sm.q_full, 256);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.o_done[i], 1);
+    }
+    mbar_init(&sm.drained, 1);
+    sm.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  if (warp == 0) {
+    const Walk w = share_start<2 * TC_ROWS, TC_KEYS>(a, blockIdx.x, gridDim.x);
+    if (lane == 0) sm.start = w;
+  }
+  fence_async_proxy();            // the zeros above, before the writes of the async proxy
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  Walk w = sm.start;
+  Segment s;
+
+  if (warp == 9) {
+    // ================================================================= loads (a lane per box of a page's keys)
+    const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows;
+    const uint32_t box_bytes = (uint32_t)box_rows * 128u;
+    int n = 0;                    // tiles sent for so far
+    bool alive = true;
+    while (alive && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+      const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
+      const int end = s.q.context + s.q.count, begin = first_key(a, s.q);
+      // this lane's box of a tile: the row of the pages, seen as one matrix, or -1 where it holds no key of the request
+      auto box_row = [&](int t) -> int {
+        const int j = t * TC_KEYS + lane * box_rows;
+        if (lane >= boxes || j >= end || j + box_rows <= begin) return -1;
+        const int page = bt[j / a.page_tokens];
+        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + j % a.page_tokens : -1;
+      };
+      int next = box_row(s.t0);
+      for (int i = 0; i < s.n && alive; ++i, ++n) {
+        const int row = next, st = n % STAGES;
+        if (i + 1 < s.n) next = box_row(s.t0 + i + 1);          // on its way while the stage is waited for
+        const uint32_t parity = (uint32_t)(((n / STAGES) & 1) ^ 1);      // a fresh barrier lets the first fill through
+        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, row >= 0)) * box_bytes * HALVES;
+        for (int kv = 0; kv < 2 && alive; ++kv) {
+          uint64_t* full = kv == 0 ? &sm.k_full[st] : &sm.v_full[st];
+          int go = 1;
+          if (lane == 0) {
+            go = mbar_wait(kv == 0 ? &sm.k_empty[st] : &sm.v_empty[st], parity, abort_flag) ? 1 : 0;
+            if (go) {
+              if (bytes == 0) mbar_arrive(full);
+              else mbar_expect_tx(full, bytes);
+            }
+          }
+          alive = __shfl_sync(0xffffffffu, go, 0) != 0;
+          if (alive && row >= 0) {
+            const uint32_t base = smem_u32(kv == 0 ? sm.k[st] : sm.v[st]) + (uint32_t)(lane * box_rows) * 128u;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) tma_load_3d(base + (uint32_t)h * (TC_KEYS * 128), kv == 0 ? &map_k : &map_v, full, 0, row, h);
+          }
+        }
+      }
+    }
+    if (*abort_flag && lane == 0) {          // the copies that are still on their way
+      for (int i = max(0, n - STAGES); i <= n; ++i) {
+        if (i < n) mbar_drain(&sm.v_full[i % STAGES], (uint32_t)((i / STAGES) & 1));
+        if (i < n || !alive) mbar_drain(&sm.k_full[i % STAGES], (uint32_t)((i / STAGES) & 1));
+      }
+    }
+  } else if (warp == 8) {
+    // ================================================================= products (one lane)
+    if (elect_one()) {
+      bool ok = true;
+      int nk = 0, nv = 0, jobs_done[2] = {0, 0};
+      uint32_t seg = 0;
+      bool issued = false;
+      while (ok && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+        const bool two = s.rows > TC_ROWS;
+        const int jobs = two ? 2 * s.n : s.n;          // job j: group j & 1; tile j / 2 with two row tiles, else j
+        if (!mbar_wait(&sm.q_full, seg & 1u, abort_flag)) { ok = false; break; }
+        ++seg;
+        auto issue_s = [&](int j) -> bool {
+          const int x = j & 1, st = nk % STAGES;
+          if ((!two || x == 0) && !mbar_wait(&sm.k_full[st], (uint32_t)((nk / STAGES) & 1), abort_flag)) return false;
+          tc_fence_after();
+          const uint32_t qs = smem_u32(sm.q[two ? x : 0]), ks = smem_u32(sm.k[st]);
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; ++kk)
+            umma(tmem + SP_COL[x], desc_k_major(qs + (uint32_t)((kk >> 2) * (TC_ROWS * 128) + (kk & 3) * 32)),
+                 desc_k_major(ks + (uint32_t)((kk >> 2) * (TC_KEYS * 128) + (kk & 3) * 32)), IDESC_S, kk ? 1u : 0u);
+          issued = true;
+          umma_commit(&sm.s_full[x]);
+          if (!two || x == 1) {
+            umma_commit(&sm.k_empty[st]);
+            ++nk;
+          }
+          return true;
+        };
+        ok = issue_s(0) && (jobs < 2 || issue_s(1));
+        for (int j = 0; j < jobs && ok; ++j) {
+          const int x = j & 1, st = nv % STAGES;
+          if (!mbar_wait(&sm.p_full[x], (uint32_t)(jobs_done[x] & 1), abort_flag)) { ok = false; break; }
+          ++jobs_done[x];
+          if ((!two || x == 0) && !mbar_wait(&sm.v_full[st], (uint32_t)((nv / STAGES) & 1), abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t vs = smem_u32(sm.v[st]);
+#pragma unroll
+          for (int kk = 0; kk < TC_KEYS / 16; ++kk)
+            umma_ts(tmem + O_COL[x], tmem + SP_COL[x] + (uint32_t)(kk * 8), desc_mn_major(vs + (uint32_t)kk * 2048u, (uint32_t)(TC_KEYS * 128)), IDESC_O,
+                    (j > 1 || kk > 0) ? 1u : 0u);
+          if (!two || x == 1) {
+            umma_commit(&sm.v_empty[st]);
+            ++nv;
+          }
+          if (j + 2 < jobs) ok = issue_s(j + 2);       // behind this job's product with V: it overwrites the P that it reads
+          else umma_commit(&sm.o_done[x]);
+        }
+      }
+      if (!ok && issued) {                             // the products that are still under way
+        umma_commit(&sm.drained);
+        mbar_drain(&sm.drained, 0);
+      }
+    }
+  } else {
+    // ================================================================= softmax (two groups of 128 threads, a row each)
+    const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;      // r: row of the tile = lane of tensor memory
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float scale_log2 = a.scale * 1.4426950408889634f;
+    const float sl = cap_log2 > 0.f ? 1.0f : scale_log2;       // capped scores are in the exponent's domain already
+    uint32_t jobs_done = 0, o_done[2] = {0, 0};
+    bool ok = true;
+    while (ok && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+      const bool two = s.rows > TC_ROWS;
+      const int row = two ? x * TC_ROWS + r : r;
+      const bool valid = row < s.rows, busy = row - lane < s.rows;        // busy: any row of the warp is one
+      const int token = valid ? (s.row0 + row) / group : 0, head = s.g * group + (valid ? (s.row0 + row) % group : 0);
+      {   // Q: each thread its own row, or half of it where both groups have the same; rows past the unit are zeros
+        const bf16* src = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * HD;
+        const uint32_t qs = smem_u32(sm.q[two ? x : 0]);
+        const int c_from = two ? 0 : x * (CPR / 2), c_to = two ? CPR : c_from + CPR / 2;
+#pragma unroll 8
+        for (int c = c_from; c < c_to; ++c) cp_async16(qs + swz(r, c), src + c * 8, valid);
+        cp_async_commit();
+      }
+      const TreeRow tr = tree_row(a, s.q, token, valid);
+      cp_async_wait<0>();
+      fence_async_proxy();
+      mbar_arrive(&sm.q_full);
+      const int jobs = two ? s.n : (s.n + 1 - x) / 2;
+      float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
+      for (int n = 0; n < jobs; ++n, ++jobs_done) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) { ok = false; break; }
+        if (!busy) {
+          mbar_arrive(&sm.p_full[x]);
+          continue;
+        }
+        tc_fence_after();
+        // The row's 128 scores in four chunks of 32; the next chunk is on its way from tensor memory while one's exponentials run.  The
+        // reference maximum moves only when a chunk's maximum runs ahead of it by more than 8; what was summed under the old one (l, O,
+        // this tile's earlier chunks of P) is then multiplied by a power of two.  The scores are complete, and so is every product
+        // issued before them, the last with V among them: O may be touched.
+        const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS;
+        const bool whole = j0 >= tr.lo && j0 + TC_KEYS <= tr.context;
+        uint32_t sc[2][32];
+        tmem_ld32(lane_addr + SP_COL[x], sc[0]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < TC_KEYS / 32; ++c) {
+          uint32_t* su = sc[c & 1];
+          if (c + 1 < TC_KEYS / 32) tmem_ld32(lane_addr + SP_COL[x] + (uint32_t)(32 * (c + 1)), sc[(c + 1) & 1]);
+          if (cap_log2 > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) su[i] = __float_as_uint(log2_score(__uint_as_float(su[i]), 1.0f, cap_log2, cap_in2));
+          }
+          if (!whole) {
+            const uint32_t see = visible32(tr, j0 + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) su[i] = (see >> i) & 1u ? su[i] : 0xff800000u;      // -inf
+          }
+          float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(su[i + 2 * e]), __uint_as_float(su[i + 2 * e + 1])));
+          }
+          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl;
+          const bool move = cm > m + 8.0f;                  // also true for the first finite maximum (m = -inf)
+          if (__any_sync(0xffffffffu, move)) {
+            const float mn = move ? ceilf(cm) : m;
+            const float corr = move ? exp2f(m - mn) : 1.0f;      // m = -inf: 0; nothing was summed yet
+            l0 *= corr;
+            l1 *= corr;
+            if (n > 0) {
+#pragma unroll 1
+              for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t o[32];
+                tmem_ld32(lane_addr + O_COL[x] + (uint32_t)c0, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                tmem_st32(lane_addr + O_COL[x] + (uint32_t)c0, o);
+              }
+            }
+            if (c > 0) tmem_st_wait();       // this tile's earlier chunks of P are in tensor memory before they are read back
+#pragma unroll 1
+            for (int cp = 0; cp < c; ++cp) {
+              uint32_t pp[16];
+              tmem_ld16(lane_addr + SP_COL[x] + (uint32_t)(16 * cp), pp);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&pp[i]));
+                const __nv_bfloat162 v = __floats2bfloat162_rn(f.x * corr, f.y * corr);
+                pp[i] = *reinterpret_cast<const uint32_t*>(&v);
+              }
+              tmem_st16(lane_addr + SP_COL[x] + (uint32_t)(16 * cp), pp);
+            }
+            m = mn;
+          }
+          const float shift = m == -CUDART_INF_F ? 0.f : -m;
+          uint32_t pw[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = ex2(fmaf(__uint_as_float(su[2 * e]), sl, shift));
+            const float p1 = ex2(fmaf(__uint_as_float(su[2 * e + 1]), sl, shift));
+            l0 += p0;
+            l1 += p1;
+            const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
+            pw[e] = *reinterpret_cast<const uint32_t*>(&pk);
+          }
+          tmem_st16(lane_addr + SP_COL[x] + (uint32_t)(16 * c), pw);
+          if (c + 1 < TC_KEYS / 32) tmem_ld_wait();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[x]);
+      }
+      // the sums of both groups: each thread takes its own row's, or half of the dims of the row that it shares
+      const bool second = two || s.n > 1;              // the second group had a tile at all
+      for (int y = 0; y < 2 && ok; ++y) {
+        if (y == 1 && !second) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_done[y], o_done[y] & 1u, abort_flag))) ok = false;
+        else ++o_done[y];
+      }
+      float l = l0 + l1;
+      sm.ml[x][r] = make_float2(m, l);
+      tc_fence_before();
+      ok = !softmax_any(!ok);
+      if (!ok) break;
+      tc_fence_after();
+      float f[2] = {1.0f, 1.0f};
+      if (!two) {
+        const float2 u = sm.ml[0][r], v = sm.ml[1][r];
+        m = fmaxf(u.x, v.x);
+        const float safe = m == -CUDART_INF_F ? 0.f : m;
+        f[0] = exp2f(u.x - safe);
+        f[1] = exp2f(v.x - safe);
+        l = u.y * f[0] + v.y * f[1];
+      }
+      const int c_from = two ? 0 : x * (HD / 2), c_to = two ? HD : c_from + HD / 2;
+      const size_t part = part_slot(blockIdx.x, s.begins) * a.rows_cap + row;
+      float inv = 1.0f;
+      if (s.whole) {
+        float total = l;
+        if (a.sink) {
+          const float score = (a.sinks ? a.sinks[head] : 0.f) * 1.4426950408889634f, top = fmaxf(m, score);
+          inv = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
+          total = l * inv + exp2f(score - top);
+        }
+        inv = total > 0.f || total != total ? inv / total : 0.f;
+      } else if (valid && (two || x == 0)) {
+        *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
+      }
+      bf16* op = reinterpret_cast<bf16*>(a.out) + ((size_t)(s.q.first + token) * a.H + head) * HD;
+      float* po = a.part_o + part * HD;
+      float odd = 0.f;                                 // NaN where a sum is NaN or Inf
+      if (busy) {
+        for (int c0 = c_from; c0 < c_to; c0 += 32) {
+          uint32_t o[32], o2[32];
+          tmem_ld32(lane_addr + O_COL[two ? x : 0] + (uint32_t)c0, o);
+          if (!two && second) tmem_ld32(lane_addr + O_COL[1] + (uint32_t)c0, o2);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float y = __uint_as_float(o[i]) * f[0];
+            if (!two && second) y = fmaf(__uint_as_float(o2[i]), f[1], y);
+            odd = fmaf(y, 0.f, odd);
+            o[i] = __float_as_uint(y * inv);
+          }
+          if (valid && s.whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[i + 2 * e]), __uint_as_float(o[i + 2 * e + 1]));
+                pk[e] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+              *reinterpret_cast<uint4*>(op + c0 + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          } else if (valid) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(po + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+        for (unsigned again = __ballot_sync(0xffffffffu, valid && odd != 0.f); again; again &= again - 1) {
+          __syncwarp();
+          const int from = __ffs(again) - 1;
+          const float m_row = __shfl_sync(0xffffffffu, m, from), inv_row = __shfl_sync(0xffffffffu, inv, from);
+          const int at = row - lane + from;
+          bf16* op_row = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)op, from));
+          float* po_row = a.part_o + (part_slot(blockIdx.x, s.begins) * a.rows_cap + at) * HD;
+          for (int c0 = c_from; c0 < c_to; c0 += 64) {          // HD / 2 or HD: at least 32, 64 at a time
+            if (c_to - c0 >= 64) {
+              float acc[2];
+              tree_row_again<2>(a, s, at, c0, m_row, cap_log2, cap_in2, acc);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (s.whole) op_row[c0 + 2 * lane + e] = __float2bfloat16_rn(acc[e] * inv_row);
+                else po_row[c0 + 2 * lane + e] = acc[e];
+              }
+            } else {
+              float acc[1];
+              tree_row_again<1>(a, s, at, c0, m_row, cap_log2, cap_in2, acc);
+              if (s.whole) op_row[c0 + lane] = __float2bfloat16_rn(acc[0] * inv_row);
+              else po_row[c0 + lane] = acc[0];
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && sm.abort_flag) atomicExch(a.status, 4);
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// The cache pages of one layer, a bf16 matrix [rows, hd], seen as [64 columns, rows, hd / 64 halves]; a box takes 64 columns x
+// box_rows rows of one half and lands as [row][128 bytes] with the 128-byte swizzle.
+bool make_page_map(CUtensorMap* map, const void* ptr, unsigned long long rows, int hd, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {64u, (cuuint64_t)rows, (cuuint64_t)(hd / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)hd * 2, 128u};
+  cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, 1u};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD>
+int launch_tc(const TreeArgs& a, int ctas, cudaStream_t s) {
+  const int pt = a.page_tokens;
+  if (!((pt % 8 == 0 && TC_KEYS % pt == 0) || pt % TC_KEYS == 0) || a.status == nullptr) return HK_ERR_UNSUPPORTED;
+  if ((((uintptr_t)a.k | (uintptr_t)a.v) & 127) != 0) return HK_ERR_UNSUPPORTED;
+  const unsigned long long rows = (unsigned long long)a.num_pages * a.G * pt;
+  if (rows > 0x7fffffffull || a.rows_cap < (a.most_tokens * (a.H / a.G) < 2 * TC_ROWS ? a.most_tokens * (a.H / a.G) : 2 * TC_ROWS)) return HK_ERR_UNSUPPORTED;
+  CUtensorMap mk, mv;
+  const int box_rows = pt < TC_KEYS ? pt : TC_KEYS;
+  if (!make_page_map(&mk, a.k, rows, HD, box_rows) || !make_page_map(&mv, a.v, rows, HD, box_rows)) return HK_ERR_UNSUPPORTED;
+  const size_t smem = sizeof(TcSmem<HD>) + 1024;
+  if (int e = hk_allow_smem<tree_tc_kernel<HD>>(smem)) return e;
+  // a soft cap c in the base-2 domain: C = c log2(e), and 2 log2(e) scale / c, which takes a raw product to 2 z log2(e), z = score / c
+  const float cap_log2 = a.softcap > 0.f ? a.softcap * 1.4426950408889634f : 0.f, cap_in2 = a.softcap > 0.f ? 2.8853900817779268f * a.scale / a.softcap : 0.f;
+  if (int e = hk_launch_pdl(tree_tc_kernel<HD>, dim3((unsigned)ctas), dim3(TC_THREADS), smem, s, mk, mv, a, cap_log2, cap_in2)) return e;
+  return launch_combine<bf16, HD, 2 * TC_ROWS, TC_KEYS>(a, ctas, s);
+}
+
+// ---- float32 ------------------------------------------------------------------------------------------------------------------
+// A tile has 32 rows, keys come 64 at a time through shared memory, and scores and sums are register tiles of multiply-adds over
+// 16-byte loads (4 x 4 scores a thread along the head's dims, 4 rows x HD / 16 dims of sums).  The next tile's keys arrive while this
+// one's probabilities are made, the next values while the next scores are.
+constexpr int F32_ROWS = 32, F32_KEYS = 64, F32_THREADS = 128, F32_LDP = F32_KEYS + 4;
+
+template <int HD>
+struct F32Smem {
+  static constexpr int LD = HD + 4;
+  float q[F32_ROWS * LD], k[F32_KEYS * LD], v[F32_KEYS * LD], p[F32_ROWS * F32_LDP];
+  float corr[F32_ROWS], inv[F32_ROWS];
+  float2 ml[F32_ROWS];
+  uint32_t see[F32_ROWS][2];
+  Walk start;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs a) {
+  constexpr int LD = F32Smem<HD>::LD, C4 = HD / 4, B = HD / 64, RI = F32_ROWS / 8;
+  extern __shared__ __align__(16) uint8_t f32_raw[];
+  F32Smem<HD>& sm = *reinterpret_cast<F32Smem<HD>*>(f32_raw);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.H / a.G;
+  const float* qp = reinterpret_cast<const float*>(a.q);
+  pdl_wait();
+  if (tid < 32) {
+    const Walk w = share_start<F32_ROWS, F32_KEYS>(a, blockIdx.x, gridDim.x);
+    if (tid == 0) sm.start = w;
+  }
+  __syncthreads();
+  Walk w = sm.start;
+  Segment s;
+  while (next_segment<F32_ROWS, F32_KEYS>(a, w, s)) {
+    const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
+    const int end = s.q.context + s.q.count;
+    // a tile's keys or values, what does not exist as zeros
+    auto fetch = [&](const void* pages, float* dst, int tile) {
+#pragma unroll 4
+      for (int e = tid; e < F32_KEYS * C4; e += F32_THREADS) {
+        const int r = e / C4, d = e % C4 * 4, j = (s.t0 + tile) * F32_KEYS + r;
+        const int page = j < end ? bt[j / a.page_tokens] : -1;
+        const bool in = page >= 0 && page < a.num_pages;
+        const float* src = reinterpret_cast<const float*>(pages) + (in ? (((size_t)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * HD + d : 0);
+        cp_async16(smem_u32(dst + r * LD + d), src, in);
+      }
+      cp_async_commit();
+    };
+    fetch(a.k, sm.k, 0);
+    fetch(a.v, sm.v, 0);
+    for (int e = tid; e < F32_ROWS * C4; e += F32_THREADS) {
+      const int r = e / C4, d = e % C4 * 4, i = s.row0 + r;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < s.rows) x = *reinterpret_cast<const float4*>(qp + ((size_t)(s.q.first + i / group) * a.H + s.g * group + i % group) * HD + d);
+      *reinterpret_cast<float4*>(sm.q + r * LD + d) = make_float4(x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale);
+    }
+    const float cap = a.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
+    const TreeRow tr = tree_row(a, s.q, (s.row0 + (tid >> 1)) / group, tid < 2 * F32_ROWS && (tid >> 1) < s.rows);     // of row tid / 2
+    // the softmax's state of row tid / 4, alike in its four threads
+    const int sr = tid >> 2, sc = (tid & 3) * 16;
+    float m = -CUDART_INF_F, l = 0.f;
+    float4 acc[RI][B];
+#pragma unroll
+    for (int i = 0; i < RI; ++i)
+#pragma unroll
+      for (int b = 0; b < B; ++b) acc[i][b] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int t = 0; t < s.n; ++t) {
+      const int j0 = (s.t0 + t) * F32_KEYS;
+      bool part = false;
+      if (tid < 2 * F32_ROWS) {
+        const uint32_t see = visible32(tr, j0 + 32 * (tid & 1));
+        sm.see[tid >> 1][tid & 1] = see;
+        part = (tid >> 1) < s.rows && see != 0xffffffffu;
+      }
+      cp_async_wait<1>();          // the keys
+      part = __syncthreads_or(part);
+      float x[RI][4];
+#pragma unroll
+      for (int i = 0; i < RI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+#pragma unroll 2
+      for (int d = 0; d < HD; d += 4) {
+        float4 u[RI], v[4];
+#pragma unroll
+        for (int i = 0; i < RI; ++i) u[i] = *reinterpret_cast<const float4*>(sm.q + (ty + 8 * i) * LD + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * j) * LD + d);
+#pragma unroll
+        for (int i = 0; i < RI; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] = fmaf(u[i].w, v[j].w, fmaf(u[i].z, v[j].z, fmaf(u[i].y, v[j].y, fmaf(u[i].x, v[j].x, x[i][j]))));
+      }
+#pragma unroll
+      for (int i = 0; i < RI; ++i) {
+        const int r = ty + 8 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = tx + 16 * j;
+          float y = x[i][j];
+          if (cap > 0.f) y = cap * tanhf(y * inv_cap);
+          sm.p[r * F32_LDP + key] = (sm.see[r][key >> 5] >> (key & 31)) & 1u ? y : -CUDART_INF_F;
+        }
+      }
+      __syncthreads();
+      if (t + 1 < s.n) fetch(a.k, sm.k, t + 1);
+      else cp_async_commit();
+      {
+        float* row = sm.p + sr * F32_LDP + sc;
+        float4 y[4];
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = *reinterpret_cast<const float4*>(row + 4 * e);
+          top = fmaxf(top, fmaxf(fmaxf(y[e].x, y[e].y), fmaxf(y[e].z, y[e].w)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m, top), safe = mn == -CUDART_INF_F ? 0.f : mn;
+        const float corr = expf(m - safe);                          // m = -inf: 0
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = make_float4(expf(y[e].x - safe), expf(y[e].y - safe), expf(y[e].z - safe), expf(y[e].w - safe));
+          sum += (y[e].x + y[e].y) + (y[e].z + y[e].w);
+          *reinterpret_cast<float4*>(row + 4 * e) = y[e];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        l = fmaf(l, corr, sum);
+        m = mn;
+        if ((tid & 3) == 0) sm.corr[sr] = corr;
+      }
+      cp_async_wait<1>();          // the values
+      bool apart = false;          // NaN or Inf among values that some row does not see
+      if (part) {
+        float odd = 0.f;           // NaN if one of the pieces that this thread fetched holds any
+#pragma unroll 4
+        for (int e = tid; e < F32_KEYS * C4; e += F32_THREADS) {
+          const float4 y = *reinterpret_cast<const float4*>(sm.v + e / C4 * LD + e % C4 * 4);
+          odd = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, odd))));
+        }
+        apart = __syncthreads_or(odd != 0.f);
+      } else {
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < RI; ++i) {
+        const float c = sm.corr[ty + 8 * i];
+#pragma unroll
+        for (int b = 0; b < B; ++b) acc[i][b] = make_float4(acc[i][b].x * c, acc[i][b].y * c, acc[i][b].z * c, acc[i][b].w * c);
+      }
+      if (!apart) {
+#pragma unroll 2
+        for (int c = 0; c < F32_KEYS; c += 4) {
+          float4 p[RI];
+#pragma unroll
+          for (int i = 0; i < RI; ++i) p[i] = *reinterpret_cast<const float4*>(sm.p + (ty + 8 * i) * F32_LDP + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+              const float4 v = *reinterpret_cast<const float4*>(sm.v + (c + e) * LD + 64 * b + 4 * tx);
+#pragma unroll
+              for (int i = 0; i < RI; ++i) {
+                const float f = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+                acc[i][b] = make_float4(fmaf(f, v.x, acc[i][b].x), fmaf(f, v.y, acc[i][b].y), fmaf(f, v.z, acc[i][b].z), fmaf(f, v.w, acc[i][b].w));
+              }
+            }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < RI; ++i) {
+          const int r = ty + 8 * i;
+          for (int word = 0; word < 2; ++word)
+            for (uint32_t left = sm.see[r][word]; left; left &= left - 1) {
+              const int c = 32 * word + __ffs(left) - 1;
+              const float f = sm.p[r * F32_LDP + c];
+#pragma unroll
+              for (int b = 0; b < B; ++b) {
+                const float4 v = *reinterpret_cast<const float4*>(sm.v + c * LD + 64 * b + 4 * tx);
+                acc[i][b] = make_float4(fmaf(f, v.x, acc[i][b].x), fmaf(f, v.y, acc[i][b].y), fmaf(f, v.z, acc[i][b].z), fmaf(f, v.w, acc[i][b].w));
+              }
+            }
+        }
+      }
+      __syncthreads();
+      if (t + 1 < s.n) fetch(a.v, sm.v, t + 1);
+      else cp_async_commit();
+    }
+    cp_async_wait<0>();
+    if ((tid & 3) == 0) {
+      float inv = 1.0f, total = l;
+      if (s.whole) {
+        if (a.sink && sr < s.rows) {
+          const float score = a.sinks ? a.sinks[s.g * group + (s.row0 + sr) % group] : 0.f, top = fmaxf(m, score);
+          inv = m == -CUDART_INF_F ? 0.f : expf(m - top);
+          total = l * inv + expf(score - top);
+        }
+        inv = total > 0.f || total != total ? inv / total : 0.f;
+      }
+      sm.inv[sr] = inv;
+      sm.ml[sr] = make_float2(m, l);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      const int r = ty + 8 * i, at = s.row0 + r;
+      if (r >= s.rows) continue;
+      const float inv = sm.inv[r];
+      const size_t part = part_slot(blockIdx.x, s.begins) * a.rows_cap + r;
+      float* dst = s.whole ? reinterpret_cast<float*>(a.out) + ((size_t)(s.q.first + at / group) * a.H + s.g * group + at % group) * HD
+                           : a.part_o + part * HD;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        *reinterpret_cast<float4*>(dst + 64 * b + 4 * tx) = make_float4(acc[i][b].x * inv, acc[i][b].y * inv, acc[i][b].z * inv, acc[i][b].w * inv);
+      if (!s.whole && tx == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = sm.ml[r];
+    }
+    __syncthreads();
+  }
+}
+
+template <int HD>
+int launch_f32(const TreeArgs& a, int ctas, cudaStream_t s) {
+  if (a.rows_cap < (a.most_tokens * (a.H / a.G) < F32_ROWS ? a.most_tokens * (a.H / a.G) : F32_ROWS)) return HK_ERR_UNSUPPORTED;
+  if (int e = hk_allow_smem<tree_f32_kernel<HD>>(sizeof(F32Smem<HD>))) return e;
+  if (int e = hk_launch_pdl(tree_f32_kernel<HD>, dim3((unsigned)ctas), dim3(F32_THREADS), sizeof(F32Smem<HD>), s, a)) return e;
+  return launch_combine<float, HD, F32_ROWS, F32_KEYS>(a, ctas, s);
+}
+
 }  // namespace
 
 // q, out [n, H, hd]; k, v [num_pages, G, page_tokens, hd]; block_table int32 [table_rows, table_stride]; requests int32
@@ -380,7 +1248,10 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 // of a token's row: it sees the drafted token j of its request; positions int32 [n] (read with a window only): drafted tokens stand
 // at their request's `context` or behind it.  Only rows of q that belong to a request are computed.  scale on q . k, softcap c (0:
 // none), window w (0: none): a key at position x is seen from position p if x > p - w; sink, sinks: one more term of the
-// denominator.  most_tokens, n_requests: bounds of the grid.  `kernel` 0: any size up to heads of 256.
+// denominator.  most_tokens, n_requests: bounds of the grid.  `kernel` 0: any size up to heads of 256.  `kernel` 1: heads of 64 and
+// 128, in bfloat16 on the tensor cores (cache pages that are whole boxes of a 128-key tile: multiples of 8 that divide 128, and
+// multiples of 128), in float32 with multiply-adds; `ctas` shares, part_o float [2 ctas, rows_cap, hd] and part_ml [2 ctas, rows_cap,
+// 2] for what they leave, rows_cap at least the rows of a tile (256, in float32 32; or most_tokens * H / G where that is less); `status` is set to 4 if a bounded wait ran out.
 HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int* block_table, int table_rows,
                              int table_stride, const int* requests, int n_requests, int most_tokens, const void* ancestors, int words,
                              const int* positions, int n, long long num_pages, int page_tokens, int H, int G, int hd, int window,
@@ -406,5 +1277,9 @@ HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* 
   a.scale = scale; a.softcap = softcap;
   cudaStream_t s = (cudaStream_t)stream;
   if (kernel == 0) return dtype == HK_F32 ? launch_generic<float>(a, s) : launch_generic<bf16>(a, s);
-  return HK_ERR_UNSUPPORTED;
+  if (kernel != 1 || ctas < 1 || part_o == nullptr || part_ml == nullptr) return HK_ERR_UNSUPPORTED;
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)part_o) & 15) != 0 || (((uintptr_t)part_ml) & 7) != 0) return HK_ERR_UNSUPPORTED;
+  if (hd != 64 && hd != 128) return HK_ERR_UNSUPPORTED;
+  if (dtype == HK_F32) return hd == 128 ? launch_f32<128>(a, ctas, s) : launch_f32<64>(a, ctas, s);
+  return hd == 128 ? launch_tc<128>(a, ctas, s) : launch_tc<64>(a, ctas, s);
 }

@@ -1563,11 +1563,36 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
     m = requests.shape[0]
     if n == 0 or m == 0:
         return
+    lib = build.load("attention_tree")
+    group, kernel, ctas, cap, part_o, part_ml, status = H // G, 0, 0, 0, None, None, 0
+    choice = _forced["attention"]
     with _on(q):
-        _check(build.load("attention_tree").hk_tree_attention(
-            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _dt(q), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(requests),
-            m, most_tokens, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
-            scale, softcap, 1 if sink else 0, _ptr(sinks), 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
+        if hd in (64, 128) and choice != "generic":
+            wide = q.dtype == torch.float32
+            rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
+            # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), but no more shares than tiles
+            held = all_keys if all_keys > 0 else m * most_keys
+            if window > 0:
+                held = min(held, m * (window + most_tokens))
+            tiles = -(-most_tokens * group // rows) * G * (held // keys + m)
+            ctas = max(1, min(gemm_fast._sms(q.device) * (2 if wide else 1), tiles))
+            cap = min(rows, most_tokens * group)
+            part_o = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
+            part_ml = part_o.data_ptr() + 8 * ctas * cap * hd
+            kernel, status = 1, 0 if wide else _ptr(gemm_fast.status_flag(q.device))
+        args = (_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _dt(q), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(requests),
+                m, most_tokens, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
+                scale, softcap, 1 if sink else 0, _ptr(sinks))
+        if kernel:
+            code = lib.hk_tree_attention(*args, kernel, ctas, _ptr(part_o), part_ml, cap, status, _stream())
+            if code != _ERR_UNSUPPORTED:
+                return _check(code, "tree_attention", launches=2 if ctas > 1 else 1)
+        if choice not in (None, "generic"):
+            raise KernelError(f"tree_attention: the '{choice}' kernel refuses head_dim={hd} page_tokens={page_tokens}")
+        _check(lib.hk_tree_attention(*args, 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
+
+
+_TREE_ROWS_TC, _TREE_ROWS_F32 = 256, 32      # rows of a tile (TC_ROWS twice, F32_ROWS in csrc/attention_tree.cu)
 
 
 def _one_device(first: torch.Tensor, *others) -> bool:
