@@ -152,19 +152,35 @@ __device__ __forceinline__ long long count_tiles(const TreeArgs& a) {
 
 // Where a CTA is in its share.
 struct Walk {
-  int r, unit, tile;
-  long long left;
+  int r, unit, tile, left;
+};
+struct Share {
+  Walk w;
   long long from, total;   // the share's first tile among all; all tiles
 };
 
+// `total` tiles in `shares` equal parts (the first of them one tile larger where they do not come out even).
+__device__ __forceinline__ long long divide(long long x, long long by) {
+  return (unsigned long long)(x | by) >> 32 ? x / by : (long long)((uint32_t)x / (uint32_t)by);      // a 64-bit division takes several times as long
+}
+__device__ __forceinline__ long long share_from(long long total, int shares, long long share) {
+  const long long each = divide(total, shares);
+  return each * share + min(share, total - each * shares);
+}
+__device__ __forceinline__ int share_of(long long total, int shares, long long tile) {
+  const long long each = divide(total, shares), wide = total - each * shares, edge = wide * (each + 1);
+  return (int)(tile < edge ? divide(tile, each + 1) : wide + divide(tile - edge, each));
+}
+
 // By a whole warp: the start of share `cta` of `ctas`.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ Walk share_start(const TreeArgs& a, int cta, int ctas) {
+__device__ __forceinline__ Share share_start(const TreeArgs& a, int cta, int ctas) {
   const int lane = threadIdx.x & 31;
   const long long total = count_tiles<ROWS, KEYS>(a);
   ctas = (int)min((long long)ctas, total);               // no empty share between two of one unit
-  const long long from = cta < ctas ? total * cta / ctas : 0, to = cta < ctas ? total * (cta + 1) / ctas : 0;
-  Walk w = {a.n_requests, 0, 0, to - from, from, total};
+  const long long from = cta < ctas ? share_from(total, ctas, cta) : 0, to = cta < ctas ? share_from(total, ctas, cta + 1) : 0;
+  Share share = {{a.n_requests, 0, 0, (int)(to - from)}, from, total};
+  Walk& w = share.w;
   long long base = 0;
   if (to > from) {
     for (int r0 = 0; r0 < a.n_requests; r0 += 32) {
@@ -182,14 +198,14 @@ __device__ __forceinline__ Walk share_start(const TreeArgs& a, int cta, int ctas
         w.r = r0 + src;
         int t_first, tiles, units;
         unit_shape<ROWS, KEYS>(a, load_request(a, w.r), t_first, tiles, units);
-        w.unit = (int)((from - start) / tiles);
-        w.tile = (int)((from - start) % tiles);
+        w.unit = (int)divide(from - start, tiles);
+        w.tile = (int)(from - start - (long long)w.unit * tiles);
         break;
       }
       base += __shfl_sync(0xffffffffu, sum, 31);
     }
   }
-  return w;
+  return share;
 }
 
 // A unit, or the part of one that falls into a share.
@@ -214,7 +230,7 @@ __device__ __forceinline__ bool next_segment(const TreeArgs& a, Walk& w, Segment
   s.row0 = w.unit / a.G * ROWS;
   s.rows = min(ROWS, s.q.count * (a.H / a.G) - s.row0);
   s.t0 = t_first + w.tile;
-  s.n = (int)min((long long)(tiles - w.tile), w.left);
+  s.n = min(tiles - w.tile, w.left);
   s.whole = s.n == tiles;
   s.begins = w.tile == 0;
   w.left -= s.n;
@@ -236,72 +252,79 @@ __device__ __forceinline__ float power(float x) {
   return sizeof(T) == 4 ? expf(x) : exp2f(x);
 }
 
+// Partial sums lie [slot][dim / 4][row][4]: neighbouring rows, which neighbouring threads hold, side by side.
+__device__ __forceinline__ float* part_place(const TreeArgs& a, size_t slot, int row, int dim, int hd) {
+  return a.part_o + ((slot * (hd / 4) + dim / 4) * a.rows_cap + row) * 4;
+}
+
 // The partial results of a unit that lies in several shares, merged in order.  A block takes the border between two shares, if it is
-// the first inside its unit, and CR of the unit's rows, a warp a row.
-constexpr int CW = 4, CR = 16;      // warps, rows
+// the first inside its unit, 32 of the unit's rows and 32 dims: a thread a row and eight dims.  It starts beside the kernel that leaves
+// the parts (which lets it only behind its own wait, so what that one reads is there) and waits with its unit found.
+constexpr int CW = 4;
 template <typename T, int HD, int ROWS, int KEYS>
 __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a, int ctas) {
-  pdl_wait();
-  constexpr int D = HD / 32;        // dims a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
-  const Walk w = share_start<ROWS, KEYS>(a, c, ctas);
+  const Share share = share_start<ROWS, KEYS>(a, c, ctas);
+  const Walk w = share.w;
   if (w.left <= 0 || w.tile == 0) return;
-  ctas = (int)min((long long)ctas, w.total);
-  const long long start = w.from - w.tile;
-  if (w.total * (c - 1) / ctas > start) return;
+  ctas = (int)min((long long)ctas, share.total);
+  const long long start = share.from - w.tile;
+  if (share_from(share.total, ctas, c - 1) > start) return;
   const TreeReq q = load_request(a, w.r);
   int t_first, tiles, units;
   unit_shape<ROWS, KEYS>(a, q, t_first, tiles, units);
-  const int parts = (int)(((start + tiles) * ctas - 1) / w.total) - c + 2;        // shares c - 1, c, ...
+  const int parts = share_of(share.total, ctas, start + tiles - 1) - c + 2;        // shares c - 1, c, ...
   const int group = a.H / a.G, g = w.unit % a.G, row0 = w.unit / a.G * ROWS, rows = min(ROWS, q.count * group - row0);
-  for (int row = blockIdx.y * CR + warp; row < min(rows, (int)(blockIdx.y + 1) * CR); row += CW) {
-    auto place = [&](int p) { return part_slot(c - 1 + p, p == 0) * a.rows_cap + row; };
-    float m = -CUDART_INF_F;
-    for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(a.part_ml + 2 * place(p)));
-    m = warp_max(m);
-    const float safe = m == -CUDART_INF_F ? 0.f : m;
-    float l = 0.f, acc[D];
+  const int row = blockIdx.y * 32 + lane, dim = blockIdx.z * 32 + warp * 8;
+  if (row >= rows) return;
+  const int token = (row0 + row) / group, head = g * group + (row0 + row) % group;
+  pdl_wait();
+  auto slot = [&](int p) { return part_slot(c - 1 + p, p == 0); };
+  auto part = [&](int p) { return __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot(p) * a.rows_cap + row); };
+  float m = -CUDART_INF_F;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, part(p).x);
+  const float safe = m == -CUDART_INF_F ? 0.f : m;
+  float l = 0.f, acc[8];
 #pragma unroll
-    for (int e = 0; e < D; ++e) acc[e] = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
-      float f = 0.f;
-      if (p0 + lane < parts) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + place(p0 + lane));
-        f = power<T>(ml.x - safe);
-        l += ml.y * f;
-      }
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll 4
-      for (int p = p0; p < min(parts, p0 + 32); ++p) {
-        const float* o = a.part_o + place(p) * HD + lane * D;
-        const float fp = __shfl_sync(0xffffffffu, f, p - p0);
-        float x[D];
-        if constexpr (D == 4) *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(o));
-        else *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(o));
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = part(p);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot(p), row, dim, HD)));
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot(p), row, dim + 4, HD)));
+    const float f = power<T>(ml.x - safe);
+    l = fmaf(ml.y, f, l);
+    acc[0] = fmaf(x.x, f, acc[0]), acc[1] = fmaf(x.y, f, acc[1]), acc[2] = fmaf(x.z, f, acc[2]), acc[3] = fmaf(x.w, f, acc[3]);
+    acc[4] = fmaf(y.x, f, acc[4]), acc[5] = fmaf(y.y, f, acc[5]), acc[6] = fmaf(y.z, f, acc[6]), acc[7] = fmaf(y.w, f, acc[7]);
+  }
+  float factor = 1.0f;
+  if (a.sink) {
+    const float score = (a.sinks ? a.sinks[head] : 0.f) * (sizeof(T) == 4 ? 1.0f : 1.4426950408889634f), top = fmaxf(m, score);
+    factor = m == -CUDART_INF_F ? 0.f : power<T>(m - top);
+    l = l * factor + power<T>(score - top);
+  }
+  const float inv = l > 0.f || l != l ? factor / l : 0.f;
+  T* out = reinterpret_cast<T*>(a.out) + ((size_t)(q.first + token) * a.H + head) * HD + dim;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(out) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<float4*>(out + 4) = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+  } else {
+    uint32_t pk[4];
 #pragma unroll
-        for (int e = 0; e < D; ++e) acc[e] = fmaf(x[e], fp, acc[e]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const __nv_bfloat162 y = __floats2bfloat162_rn(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      pk[e] = *reinterpret_cast<const uint32_t*>(&y);
     }
-    l = warp_sum(l);
-    const int token = (row0 + row) / group, head = g * group + (row0 + row) % group;
-    if (a.sink) {
-      const float score = (a.sinks ? a.sinks[head] : 0.f) * (sizeof(T) == 4 ? 1.0f : 1.4426950408889634f);
-      const float top = fmaxf(m, score), f = m == -CUDART_INF_F ? 0.f : power<T>(m - top);
-      l = l * f + power<T>(score - top);
-#pragma unroll
-      for (int e = 0; e < D; ++e) acc[e] *= f;
-    }
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-    T* out = reinterpret_cast<T*>(a.out) + ((size_t)(q.first + token) * a.H + head) * HD + lane * D;
-#pragma unroll
-    for (int e = 0; e < D; ++e) out[e] = from_f32<T>(acc[e] * inv);
+    *reinterpret_cast<uint4*>(out) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
   }
 }
 
 template <typename T, int HD, int ROWS, int KEYS>
 int launch_combine(const TreeArgs& a, int ctas, cudaStream_t s) {
   if (ctas < 2) return 0;
-  return hk_launch_pdl(tree_combine_kernel<T, HD, ROWS, KEYS>, dim3((unsigned)(ctas - 1), (unsigned)((a.rows_cap + CR - 1) / CR)), dim3(CW * 32), 0, s, a,
-                       ctas);
+  return hk_launch_pdl(tree_combine_kernel<T, HD, ROWS, KEYS>, dim3((unsigned)(ctas - 1), (unsigned)((a.rows_cap + 31) / 32), HD / 32), dim3(CW * 32), 0, s,
+                       a, ctas);
 }
 
 // ---- any size: a block a (token, query head) -------------------------------------------------------------------------------
@@ -390,17 +413,19 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 }
 
 // ---- bfloat16 on the tensor cores ---------------------------------------------------------------------------------------------
-// A tile has up to 256 rows.  Two groups of four softmax warps (a thread a row), one lane that issues the products and one warp that
-// loads K and V by TMA work on it side by side: with more than 128 rows each group has half of them and every key tile serves both;
-// with up to 128 rows both groups have the same rows and take the key tiles in turn, and their sums meet in tensor memory at the end.
-// Either way one group's exponentials run while the tensor core works for the other.  Tensor memory (512 columns): per group 128
-// columns of scores, which the probabilities overwrite (bfloat16, 64 columns), and HD of sums.  A group's next scores are issued
-// behind its product with V; products of one thread run in order, so they overwrite P only once it was read.
+// A tile has up to 256 rows.  Two groups of eight softmax warps (two threads a row, half of a tile's keys each), one lane that issues
+// the products and one warp that loads K and V by TMA work on it side by side: with more than 128 rows each group has half of them and
+// every key tile serves both; with up to 128 rows both groups have the same rows and take the key tiles in turn, and their sums meet in
+// tensor memory at the end.  Either way one group's exponentials run while the tensor core works for the other.  Tensor memory (512
+// columns): per group 128 columns of scores, which the probabilities overwrite (bfloat16, each half 32 columns), and HD of sums.  A group's next
+// scores are issued behind its product with V; products of one thread run in order, so they overwrite P only once it was read.
 //
-// Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits): they are at most 2^8 times a power of
-// two that is the row's reference maximum, an integer, so that moving it rounds nothing.
-constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 320;
-constexpr uint32_t WAIT_LIMIT = 1u << 17;   // tries of about 100 ns each: some 13 ms, far beyond any legitimate wait
+// Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits).  They are taken against a reference, an
+// integer, that moves to a row's maximum only where that runs ahead by more than LAZY: bfloat16 and the sums in float32 have exponents to
+// spare, so nothing is lost meanwhile, and moving it multiplies by a power of two, which rounds nothing.
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 64;
+constexpr float LAZY = 24.0f;
+constexpr long long WAIT_CLOCKS = 1ll << 25;   // some 17 ms, far beyond any legitimate wait
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -421,19 +446,23 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
-// Waits for the phase of this parity, a bounded number of tries; false (and the flag set) if it did not come or another gave up.
+// Waits for the phase of this parity, a bounded time; false (and the flag set) if it did not come or another gave up.  (Without sleeps
+// between the tries: the tensor core's answers come in less than one.)
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (i >= 4) __nanosleep(100);      // a waiting warp must not take issue slots from the working ones
-    if ((i & 255u) == 255u && *abort_flag) return false;
+    if ((i & 63u) == 0u && (*abort_flag || clock64() - start > WAIT_CLOCKS)) break;
   }
   *abort_flag = 1;
   return false;
 }
 // The same for what is still on its way when the kernel gives up.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++i) __nanosleep(100);
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - start < WAIT_CLOCKS) {
+  }
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -524,13 +553,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// Barrier 1 among the 256 softmax threads; whether any of them says so.
+// Barrier 1 among the softmax threads; whether any of them says so.
 __device__ __forceinline__ bool softmax_any(bool said) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "bar.red.or.pred q, 1, 512, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(any) : "r"(said ? 1u : 0u) : "memory");
   return any != 0;
@@ -545,25 +574,24 @@ struct TcSmem {
   alignas(1024) uint8_t k[STAGES][TC_KEYS * HD * 2];
   alignas(1024) uint8_t v[STAGES][TC_KEYS * HD * 2];
   alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], drained;
-  float2 ml[2][TC_ROWS];      // a row's reference maximum and sum in either group
+  float top[2][2][TC_ROWS];   // [group][half of the keys][row]: a tile's largest score
+  float2 ml[2][2][TC_ROWS];   // the reference and the sum
   Walk start;
   uint32_t tmem_base;
   int abort_flag;
 };
 
-// The dims [c0, c0 + 32 D) of one row's sums over the keys of a segment that it sees, against the reference maximum m, by one warp in
-// 32 bits.  For a row whose sums came out NaN or Inf: the tensor core's product takes whole tiles of values, and a probability of zero
-// does not keep out a NaN or Inf among those that the row does not see.
-template <int D>
-__device__ __noinline__ void tree_row_again(const TreeArgs& a, const Segment& s, int row, int c0, float m, float cap_log2, float cap_in2, float (&acc)[D]) {
+// A dim a lane of one row's sums over the keys of a segment that it sees, against the reference maximum m, by one warp in 32 bits.  For
+// a row whose sums came out NaN or Inf: the tensor core's product takes whole tiles of values, and a probability of zero does not keep
+// out a NaN or Inf among those that the row does not see.
+__device__ __noinline__ float tree_row_again(const TreeArgs a, const Segment s, int row, int dim, float m, float cap_log2, float cap_in2) {
   const int lane = threadIdx.x & 31, group = a.H / a.G, hd = a.hd;
   const int token = (s.row0 + row) / group, head = s.g * group + (s.row0 + row) % group;
   const TreeRow w = tree_row(a, s.q, token, true);
   const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * hd;
   const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
   const float safe = m == -CUDART_INF_F ? 0.f : m, scale_log2 = a.scale * 1.4426950408889634f;
-#pragma unroll
-  for (int e = 0; e < D; ++e) acc[e] = 0.f;
+  float acc = 0.f;
   for (int j0 = s.t0 * TC_KEYS; j0 < min((s.t0 + s.n) * TC_KEYS, s.q.context + s.q.count); j0 += 32) {
     const uint32_t see = visible32(w, j0);
     if (see == 0) continue;
@@ -582,17 +610,17 @@ __device__ __noinline__ void tree_row_again(const TreeArgs& a, const Segment& s,
     for (uint32_t left = __ballot_sync(0xffffffffu, at >= 0); left; left &= left - 1) {
       const int i = __ffs(left) - 1;
       const float f = __shfl_sync(0xffffffffu, p, i);
-      const bf16* v = reinterpret_cast<const bf16*>(a.v) + __shfl_sync(0xffffffffu, at, i) + c0 + lane * D;
-#pragma unroll
-      for (int e = 0; e < D; ++e) acc[e] = fmaf(f, __bfloat162float(v[e]), acc[e]);
+      acc = fmaf(f, __bfloat162float(reinterpret_cast<const bf16*>(a.v)[__shfl_sync(0xffffffffu, at, i) + dim]), acc);
     }
   }
+  return acc;
 }
 
 template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeArgs a, float cap_log2, float cap_in2) {
   constexpr int STAGES = TcSmem<HD>::STAGES, CPR = HD / 8, KSTEPS = HD / 16, HALVES = HD / 64;
+  constexpr int MMA_WARP = TC_SOFTMAX / 32, LOAD_WARP = MMA_WARP + 1;
   constexpr uint32_t TMEM_COLS = 512, SP_COL[2] = {0, 128}, O_COL[2] = {256, 256 + HD};
   // fp32 accumulators, bf16 operands; N at bit 17 (>> 3), M at bit 24 (>> 4); bit 16: B is MN-major
   constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC_KEYS >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
@@ -603,15 +631,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.G;
 
-  // The V stages start as zeros: rows of a tile that no box is copied to are multiplied by a probability of zero, which must not meet
-  // a NaN pattern.  K needs none: a score of such a key is masked before it is looked at.
-  {
-    uint4* z = reinterpret_cast<uint4*>(sm.v[0]);
-    constexpr int N16 = STAGES * TC_KEYS * HD * 2 / 16;
-    for (int i = threadIdx.x; i < N16; i += TC_THREADS) z[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
   if (threadIdx.x == 32) {
-    mbar_init(&sm.q_full, 256);
+    mbar_init(&sm.q_full, TC_SOFTMAX);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.v_full[i], 1);
@@ -620,23 +641,23 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.p_full[i], TC_SOFTMAX / 2);
       mbar_init(&sm.o_done[i], 1);
     }
     mbar_init(&sm.drained, 1);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
+  pdl_launch_dependents();
   if (warp == 0) {
-    const Walk w = share_start<2 * TC_ROWS, TC_KEYS>(a, blockIdx.x, gridDim.x);
-    if (lane == 0) sm.start = w;
+    const Share share = share_start<2 * TC_ROWS, TC_KEYS>(a, blockIdx.x, gridDim.x);
+    if (lane == 0) sm.start = share.w;
   }
-  fence_async_proxy();            // the zeros above, before the writes of the async proxy
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -644,40 +665,36 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   Walk w = sm.start;
   Segment s;
 
-  if (warp == 9) {
+  if (warp == LOAD_WARP) {
     // ================================================================= loads (a lane per box of a page's keys)
     const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows;
-    const uint32_t box_bytes = (uint32_t)box_rows * 128u;
     int n = 0;                    // tiles sent for so far
     bool alive = true;
     while (alive && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
       const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
       const int end = s.q.context + s.q.count, begin = first_key(a, s.q);
-      // this lane's box of a tile: the row of the pages, seen as one matrix, or -1 where it holds no key of the request
+      // This lane's box of a tile: its first row of the pages, seen as one matrix.  A box that holds no key of the request is the one
+      // of its nearest key, so that nothing but cache rows ever lies in a stage: an old NaN pattern there would not be kept out of the
+      // sums by a probability of zero.
       auto box_row = [&](int t) -> int {
-        const int j = t * TC_KEYS + lane * box_rows;
-        if (lane >= boxes || j >= end || j + box_rows <= begin) return -1;
+        const int j = min(max(t * TC_KEYS + min(lane, boxes - 1) * box_rows, begin / box_rows * box_rows), (end - 1) / box_rows * box_rows);
         const int page = bt[j / a.page_tokens];
-        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + j % a.page_tokens : -1;
+        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + j % a.page_tokens : 0;
       };
       int next = box_row(s.t0);
       for (int i = 0; i < s.n && alive; ++i, ++n) {
         const int row = next, st = n % STAGES;
         if (i + 1 < s.n) next = box_row(s.t0 + i + 1);          // on its way while the stage is waited for
         const uint32_t parity = (uint32_t)(((n / STAGES) & 1) ^ 1);      // a fresh barrier lets the first fill through
-        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, row >= 0)) * box_bytes * HALVES;
         for (int kv = 0; kv < 2 && alive; ++kv) {
           uint64_t* full = kv == 0 ? &sm.k_full[st] : &sm.v_full[st];
           int go = 1;
           if (lane == 0) {
             go = mbar_wait(kv == 0 ? &sm.k_empty[st] : &sm.v_empty[st], parity, abort_flag) ? 1 : 0;
-            if (go) {
-              if (bytes == 0) mbar_arrive(full);
-              else mbar_expect_tx(full, bytes);
-            }
+            if (go) mbar_expect_tx(full, TC_KEYS * HD * 2);
           }
           alive = __shfl_sync(0xffffffffu, go, 0) != 0;
-          if (alive && row >= 0) {
+          if (alive && lane < boxes) {
             const uint32_t base = smem_u32(kv == 0 ? sm.k[st] : sm.v[st]) + (uint32_t)(lane * box_rows) * 128u;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) tma_load_3d(base + (uint32_t)h * (TC_KEYS * 128), kv == 0 ? &map_k : &map_v, full, 0, row, h);
@@ -691,7 +708,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (i < n || !alive) mbar_drain(&sm.k_full[i % STAGES], (uint32_t)((i / STAGES) & 1));
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == MMA_WARP) {
     // ================================================================= products (one lane)
     if (elect_one()) {
       bool ok = true;
@@ -730,7 +747,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           const uint32_t vs = smem_u32(sm.v[st]);
 #pragma unroll
           for (int kk = 0; kk < TC_KEYS / 16; ++kk)
-            umma_ts(tmem + O_COL[x], tmem + SP_COL[x] + (uint32_t)(kk * 8), desc_mn_major(vs + (uint32_t)kk * 2048u, (uint32_t)(TC_KEYS * 128)), IDESC_O,
+            umma_ts(tmem + O_COL[x], tmem + SP_COL[x] + (uint32_t)((kk >> 2) * (TC_KEYS / 2) + (kk & 3) * 8), desc_mn_major(vs + (uint32_t)kk * 2048u, (uint32_t)(TC_KEYS * 128)), IDESC_O,
                     (j > 1 || kk > 0) ? 1u : 0u);
           if (!two || x == 1) {
             umma_commit(&sm.v_empty[st]);
@@ -746,102 +763,118 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       }
     }
   } else {
-    // ================================================================= softmax (two groups of 128 threads, a row each)
-    const int x = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;      // r: row of the tile = lane of tensor memory
+    // ================================================================= softmax (two groups of 256 threads, two a row)
+    // Warps w and w + 4 of a group read the same lanes of tensor memory (32 * (w & 3) ..): the first the lower half of a tile's keys, the
+    // second the upper.  A row's two threads meet through shared memory for its maximum and its sum.
+    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;      // r: row of the tile = lane of tensor memory
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    constexpr int HK = TC_KEYS / 2, EC = 16;        // keys a thread; dims of the sums that a thread finishes at once
     const float scale_log2 = a.scale * 1.4426950408889634f;
     const float sl = cap_log2 > 0.f ? 1.0f : scale_log2;       // capped scores are in the exponent's domain already
+    const uint32_t sp = lane_addr + (x ? SP_COL[1] : SP_COL[0]), oc = lane_addr + (x ? O_COL[1] : O_COL[0]);
     uint32_t jobs_done = 0, o_done[2] = {0, 0};
     bool ok = true;
-    while (ok && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+    // Q: the threads of a row share it out; rows past the unit are zeros
+    auto send_q = [&](const Segment& u) {
+      const bool two = u.rows > TC_ROWS;
+      const int row = two ? x * TC_ROWS + r : r, i = u.row0 + (row < u.rows ? row : 0);
+      const bf16* src = reinterpret_cast<const bf16*>(a.q) + ((size_t)(u.q.first + i / group) * a.H + u.g * group + i % group) * HD;
+      const uint32_t qs = smem_u32(sm.q[two ? x : 0]);
+      const int c_from = two ? half * (CPR / 2) : (2 * x + half) * (CPR / 4), c_to = c_from + (two ? CPR / 2 : CPR / 4);
+#pragma unroll 4
+      for (int c = c_from; c < c_to; ++c) cp_async16(qs + swz(r, c), src + c * 8, row < u.rows);
+      cp_async_commit();
+    };
+    Segment ahead;
+    bool more = next_segment<2 * TC_ROWS, TC_KEYS>(a, w, ahead);
+    if (more) send_q(ahead);
+    while (ok && more) {
+      s = ahead;
       const bool two = s.rows > TC_ROWS;
       const int row = two ? x * TC_ROWS + r : r;
       const bool valid = row < s.rows, busy = row - lane < s.rows;        // busy: any row of the warp is one
-      const int token = valid ? (s.row0 + row) / group : 0, head = s.g * group + (valid ? (s.row0 + row) % group : 0);
-      {   // Q: each thread its own row, or half of it where both groups have the same; rows past the unit are zeros
-        const bf16* src = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * HD;
-        const uint32_t qs = smem_u32(sm.q[two ? x : 0]);
-        const int c_from = two ? 0 : x * (CPR / 2), c_to = two ? CPR : c_from + CPR / 2;
-#pragma unroll 8
-        for (int c = c_from; c < c_to; ++c) cp_async16(qs + swz(r, c), src + c * 8, valid);
-        cp_async_commit();
-      }
-      const TreeRow tr = tree_row(a, s.q, token, valid);
+      const int token = valid ? (s.row0 + row) / group : 0;
+      const int lo = valid ? tree_row(a, s.q, token, true).lo : 0x7fffffff;
       cp_async_wait<0>();
       fence_async_proxy();
       mbar_arrive(&sm.q_full);
       const int jobs = two ? s.n : (s.n + 1 - x) / 2;
       float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
       for (int n = 0; n < jobs; ++n, ++jobs_done) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) { ok = false; break; }
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) ok = false;
         if (!busy) {
-          mbar_arrive(&sm.p_full[x]);
+          if (ok) mbar_arrive(&sm.p_full[x]);
           continue;
         }
-        tc_fence_after();
-        // The row's 128 scores in four chunks of 32; the next chunk is on its way from tensor memory while one's exponentials run.  The
-        // reference maximum moves only when a chunk's maximum runs ahead of it by more than 8; what was summed under the old one (l, O,
-        // this tile's earlier chunks of P) is then multiplied by a power of two.  The scores are complete, and so is every product
-        // issued before them, the last with V among them: O may be touched.
-        const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS;
-        const bool whole = j0 >= tr.lo && j0 + TC_KEYS <= tr.context;
-        uint32_t sc[2][32];
-        tmem_ld32(lane_addr + SP_COL[x], sc[0]);
-        tmem_ld_wait();
+        const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
+        const bool part = j0 < lo || j0 + HK > s.q.context;
+        uint32_t see[2] = {0xffffffffu, 0xffffffffu}, su[32];
+        if (ok) {
+          // the largest score that counts; the scores are read from tensor memory once more below: a thread holds 32 of them, not 64
+          tc_fence_after();
+          float top = -CUDART_INF_F;
+          if (part) {
+            const TreeRow tr = tree_row(a, s.q, token, valid);
+            see[0] = visible32(tr, j0);
+            see[1] = visible32(tr, j0 + 32);
+          }
 #pragma unroll
-        for (int c = 0; c < TC_KEYS / 32; ++c) {
-          uint32_t* su = sc[c & 1];
-          if (c + 1 < TC_KEYS / 32) tmem_ld32(lane_addr + SP_COL[x] + (uint32_t)(32 * (c + 1)), sc[(c + 1) & 1]);
+          for (int c = 0; c < 2; ++c) {
+            tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
+            tmem_ld_wait();
+            if (part) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) su[i] = (see[c] >> i) & 1u ? su[i] : 0xff800000u;      // -inf
+            }
+            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(su[i + 2 * e]), __uint_as_float(su[i + 2 * e + 1])));
+            }
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          }
+          // (a cap climbs with the score: the largest stays the largest; a masked one stays out of it)
+          sm.top[x][half][r] = cap_log2 > 0.f && (see[0] | see[1]) ? log2_score(top, 1.0f, cap_log2, cap_in2) : top * sl;
+        }
+        // the row's other thread; who gave up comes here all the same, or the other would wait for good
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * x + quarter) : "memory");
+        if (!ok) continue;
+        const float cm = fmaxf(sm.top[x][0][r], sm.top[x][1][r]);
+        // The scores are complete, and so is every product issued before them, the last with V among them: O may be touched.
+        const bool move = cm > m + LAZY;                  // also true for the first finite maximum (m = -inf)
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = move ? ceilf(cm) : m;
+          const float corr = move ? exp2f(m - mn) : 1.0f;      // m = -inf: 0; nothing was summed yet
+          l0 *= corr;
+          l1 *= corr;
+          if (n > 0) {
+#pragma unroll 1
+            for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(oc + (uint32_t)c0, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st16(oc + (uint32_t)c0, o);
+            }
+          }
+          m = mn;
+        }
+        const float shift = m == -CUDART_INF_F ? 0.f : -m;
+        // a half's P lies in the columns of its own scores that are read already
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
+          tmem_ld_wait();
           if (cap_log2 > 0.f) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) su[i] = __float_as_uint(log2_score(__uint_as_float(su[i]), 1.0f, cap_log2, cap_in2));
           }
-          if (!whole) {
-            const uint32_t see = visible32(tr, j0 + 32 * c);
+          if (part) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) su[i] = (see >> i) & 1u ? su[i] : 0xff800000u;      // -inf
+            for (int i = 0; i < 32; ++i) su[i] = (see[c] >> i) & 1u ? su[i] : 0xff800000u;
           }
-          float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(su[i + 2 * e]), __uint_as_float(su[i + 2 * e + 1])));
-          }
-          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl;
-          const bool move = cm > m + 8.0f;                  // also true for the first finite maximum (m = -inf)
-          if (__any_sync(0xffffffffu, move)) {
-            const float mn = move ? ceilf(cm) : m;
-            const float corr = move ? exp2f(m - mn) : 1.0f;      // m = -inf: 0; nothing was summed yet
-            l0 *= corr;
-            l1 *= corr;
-            if (n > 0) {
-#pragma unroll 1
-              for (int c0 = 0; c0 < HD; c0 += 32) {
-                uint32_t o[32];
-                tmem_ld32(lane_addr + O_COL[x] + (uint32_t)c0, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                tmem_st32(lane_addr + O_COL[x] + (uint32_t)c0, o);
-              }
-            }
-            if (c > 0) tmem_st_wait();       // this tile's earlier chunks of P are in tensor memory before they are read back
-#pragma unroll 1
-            for (int cp = 0; cp < c; ++cp) {
-              uint32_t pp[16];
-              tmem_ld16(lane_addr + SP_COL[x] + (uint32_t)(16 * cp), pp);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&pp[i]));
-                const __nv_bfloat162 v = __floats2bfloat162_rn(f.x * corr, f.y * corr);
-                pp[i] = *reinterpret_cast<const uint32_t*>(&v);
-              }
-              tmem_st16(lane_addr + SP_COL[x] + (uint32_t)(16 * cp), pp);
-            }
-            m = mn;
-          }
-          const float shift = m == -CUDART_INF_F ? 0.f : -m;
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -852,60 +885,62 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
             pw[e] = *reinterpret_cast<const uint32_t*>(&pk);
           }
-          tmem_st16(lane_addr + SP_COL[x] + (uint32_t)(16 * c), pw);
-          if (c + 1 < TC_KEYS / 32) tmem_ld_wait();
+          tmem_st16(sp + (uint32_t)(half * HK + 16 * c), pw);
         }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_full[x]);
       }
-      // the sums of both groups: each thread takes its own row's, or half of the dims of the row that it shares
+      // the sums of both groups: a row's two threads (four where the groups share their rows) take a part of its dims each
       const bool second = two || s.n > 1;              // the second group had a tile at all
       for (int y = 0; y < 2 && ok; ++y) {
         if (y == 1 && !second) break;
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_done[y], o_done[y] & 1u, abort_flag))) ok = false;
         else ++o_done[y];
       }
-      float l = l0 + l1;
-      sm.ml[x][r] = make_float2(m, l);
+      sm.ml[x][half][r] = make_float2(m, l0 + l1);
       tc_fence_before();
       ok = !softmax_any(!ok);
       if (!ok) break;
       tc_fence_after();
-      float f[2] = {1.0f, 1.0f};
-      if (!two) {
-        const float2 u = sm.ml[0][r], v = sm.ml[1][r];
-        m = fmaxf(u.x, v.x);
-        const float safe = m == -CUDART_INF_F ? 0.f : m;
-        f[0] = exp2f(u.x - safe);
-        f[1] = exp2f(v.x - safe);
-        l = u.y * f[0] + v.y * f[1];
-      }
-      const int c_from = two ? 0 : x * (HD / 2), c_to = two ? HD : c_from + HD / 2;
-      const size_t part = part_slot(blockIdx.x, s.begins) * a.rows_cap + row;
-      float inv = 1.0f;
-      if (s.whole) {
-        float total = l;
-        if (a.sink) {
-          const float score = (a.sinks ? a.sinks[head] : 0.f) * 1.4426950408889634f, top = fmaxf(m, score);
-          inv = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
-          total = l * inv + exp2f(score - top);
-        }
-        inv = total > 0.f || total != total ? inv / total : 0.f;
-      } else if (valid && (two || x == 0)) {
-        *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
-      }
-      bf16* op = reinterpret_cast<bf16*>(a.out) + ((size_t)(s.q.first + token) * a.H + head) * HD;
-      float* po = a.part_o + part * HD;
-      float odd = 0.f;                                 // NaN where a sum is NaN or Inf
+      more = next_segment<2 * TC_ROWS, TC_KEYS>(a, w, ahead);
+      if (more) send_q(ahead);                         // both groups' scores are through: Q is free
       if (busy) {
-        for (int c0 = c_from; c0 < c_to; c0 += 32) {
-          uint32_t o[32], o2[32];
-          tmem_ld32(lane_addr + O_COL[two ? x : 0] + (uint32_t)c0, o);
-          if (!two && second) tmem_ld32(lane_addr + O_COL[1] + (uint32_t)c0, o2);
+        float f[2] = {1.0f, 1.0f}, l;
+        if (two) {
+          l = sm.ml[x][0][r].y + sm.ml[x][1][r].y;
+        } else {
+          const float2 u = sm.ml[0][0][r], v = sm.ml[1][0][r];
+          m = fmaxf(u.x, v.x);
+          const float safe = m == -CUDART_INF_F ? 0.f : m;
+          f[0] = exp2f(u.x - safe);
+          f[1] = exp2f(v.x - safe);
+          l = (u.y + sm.ml[0][1][r].y) * f[0] + (v.y + sm.ml[1][1][r].y) * f[1];
+        }
+        const int head = s.g * group + (s.row0 + (valid ? row : 0)) % group;
+        const size_t slot = part_slot(blockIdx.x, s.begins);
+        float inv = 1.0f;
+        if (s.whole) {
+          float total = l;
+          if (a.sink) {
+            const float score = (a.sinks ? a.sinks[head] : 0.f) * 1.4426950408889634f, top = fmaxf(m, score);
+            inv = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
+            total = l * inv + exp2f(score - top);
+          }
+          inv = total > 0.f || total != total ? inv / total : 0.f;
+        } else if (valid && half == 0 && (two || x == 0)) {
+          *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + row) = make_float2(m, l);
+        }
+        bf16* op = reinterpret_cast<bf16*>(a.out) + ((size_t)(s.q.first + token) * a.H + head) * HD;
+        float odd = 0.f;                               // NaN where a sum is NaN or Inf
+        const int c_from = two ? half * (HD / 2) : (2 * x + half) * (HD / 4), c_to = c_from + (two ? HD / 2 : HD / 4);
+        for (int c0 = c_from; c0 < c_to; c0 += EC) {
+          uint32_t o[EC], o2[EC];
+          tmem_ld16((two ? oc : lane_addr + O_COL[0]) + (uint32_t)c0, o);
+          if (!two && second) tmem_ld16(lane_addr + O_COL[1] + (uint32_t)c0, o2);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < EC; ++i) {
             float y = __uint_as_float(o[i]) * f[0];
             if (!two && second) y = fmaf(__uint_as_float(o2[i]), f[1], y);
             odd = fmaf(y, 0.f, odd);
@@ -913,7 +948,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           }
           if (valid && s.whole) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
+            for (int i = 0; i < EC; i += 8) {
               uint32_t pk[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -924,30 +959,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
           } else if (valid) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(po + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < EC; i += 4)
+              *reinterpret_cast<uint4*>(part_place(a, slot, row, c0 + i, HD)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
         for (unsigned again = __ballot_sync(0xffffffffu, valid && odd != 0.f); again; again &= again - 1) {
           __syncwarp();
-          const int from = __ffs(again) - 1;
+          const int from = __ffs(again) - 1, at = row - lane + from;
           const float m_row = __shfl_sync(0xffffffffu, m, from), inv_row = __shfl_sync(0xffffffffu, inv, from);
-          const int at = row - lane + from;
           bf16* op_row = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)op, from));
-          float* po_row = a.part_o + (part_slot(blockIdx.x, s.begins) * a.rows_cap + at) * HD;
-          for (int c0 = c_from; c0 < c_to; c0 += 64) {          // HD / 2 or HD: at least 32, 64 at a time
-            if (c_to - c0 >= 64) {
-              float acc[2];
-              tree_row_again<2>(a, s, at, c0, m_row, cap_log2, cap_in2, acc);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (s.whole) op_row[c0 + 2 * lane + e] = __float2bfloat16_rn(acc[e] * inv_row);
-                else po_row[c0 + 2 * lane + e] = acc[e];
-              }
-            } else {
-              float acc[1];
-              tree_row_again<1>(a, s, at, c0, m_row, cap_log2, cap_in2, acc);
-              if (s.whole) op_row[c0 + lane] = __float2bfloat16_rn(acc[0] * inv_row);
-              else po_row[c0 + lane] = acc[0];
+          for (int c0 = c_from; c0 < c_to; c0 += 32) {
+            const int dim = c0 + lane;
+            const float y = tree_row_again(a, s, at, min(dim, HD - 1), m_row, cap_log2, cap_in2);
+            if (dim < c_to) {
+              if (s.whole) op_row[dim] = __float2bfloat16_rn(y * inv_row);
+              else part_place(a, slot, at, dim, HD)[dim & 3] = y;
             }
           }
         }
@@ -959,7 +985,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && sm.abort_flag) atomicExch(a.status, 4);
-  if (warp == 8) {
+  if (warp == MMA_WARP) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
@@ -1037,9 +1063,10 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.H / a.G;
   const float* qp = reinterpret_cast<const float*>(a.q);
   pdl_wait();
+  pdl_launch_dependents();
   if (tid < 32) {
-    const Walk w = share_start<F32_ROWS, F32_KEYS>(a, blockIdx.x, gridDim.x);
-    if (tid == 0) sm.start = w;
+    const Share share = share_start<F32_ROWS, F32_KEYS>(a, blockIdx.x, gridDim.x);
+    if (tid == 0) sm.start = share.w;
   }
   __syncthreads();
   Walk w = sm.start;
@@ -1221,13 +1248,13 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
       const int r = ty + 8 * i, at = s.row0 + r;
       if (r >= s.rows) continue;
       const float inv = sm.inv[r];
-      const size_t part = part_slot(blockIdx.x, s.begins) * a.rows_cap + r;
-      float* dst = s.whole ? reinterpret_cast<float*>(a.out) + ((size_t)(s.q.first + at / group) * a.H + s.g * group + at % group) * HD
-                           : a.part_o + part * HD;
+      const size_t slot = part_slot(blockIdx.x, s.begins);
+      float* out = reinterpret_cast<float*>(a.out) + ((size_t)(s.q.first + at / group) * a.H + s.g * group + at % group) * HD;
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        *reinterpret_cast<float4*>(dst + 64 * b + 4 * tx) = make_float4(acc[i][b].x * inv, acc[i][b].y * inv, acc[i][b].z * inv, acc[i][b].w * inv);
-      if (!s.whole && tx == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = sm.ml[r];
+        *reinterpret_cast<float4*>(s.whole ? out + 64 * b + 4 * tx : part_place(a, slot, r, 64 * b + 4 * tx, HD)) =
+            make_float4(acc[i][b].x * inv, acc[i][b].y * inv, acc[i][b].z * inv, acc[i][b].w * inv);
+      if (!s.whole && tx == 0) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + r) = sm.ml[r];
     }
     __syncthreads();
   }
@@ -1250,8 +1277,8 @@ int launch_f32(const TreeArgs& a, int ctas, cudaStream_t s) {
 // none), window w (0: none): a key at position x is seen from position p if x > p - w; sink, sinks: one more term of the
 // denominator.  most_tokens, n_requests: bounds of the grid.  `kernel` 0: any size up to heads of 256.  `kernel` 1: heads of 64 and
 // 128, in bfloat16 on the tensor cores (cache pages that are whole boxes of a 128-key tile: multiples of 8 that divide 128, and
-// multiples of 128), in float32 with multiply-adds; `ctas` shares, part_o float [2 ctas, rows_cap, hd] and part_ml [2 ctas, rows_cap,
-// 2] for what they leave, rows_cap at least the rows of a tile (256, in float32 32; or most_tokens * H / G where that is less); `status` is set to 4 if a bounded wait ran out.
+// multiples of 128), in float32 with multiply-adds; `ctas` shares, part_o float [2 ctas, hd / 4, rows_cap, 4] and part_ml [2 ctas,
+// rows_cap, 2] for what they leave, rows_cap at least the rows of a tile (256, in float32 32; or most_tokens * H / G where that is less); `status` is set to 4 if a bounded wait ran out.
 HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int* block_table, int table_rows,
                              int table_stride, const int* requests, int n_requests, int most_tokens, const void* ancestors, int words,
                              const int* positions, int n, long long num_pages, int page_tokens, int H, int G, int hd, int window,
