@@ -421,10 +421,12 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 // scores are issued behind its product with V; products of one thread run in order, so they overwrite P only once it was read.
 //
 // Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits).  They are taken against a reference, an
-// integer, that moves to a row's maximum only where that runs ahead by more than LAZY: bfloat16 and the sums in float32 have exponents to
-// spare, so nothing is lost meanwhile, and moving it multiplies by a power of two, which rounds nothing.
+// integer near the largest score of the first tile in which a row sees anything: bfloat16 and the sums in float32 have exponents to
+// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference for
+// the next one, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
+// threads need not meet over it.  Where one tile jumps by more than 2^60 the row's sum is set to NaN, and the row is taken again (below).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 64;
-constexpr float LAZY = 24.0f;
+constexpr float MUCH = 16777216.0f, TOO_MUCH = 1152921504606846976.0f;      // 2^24, 2^60
 constexpr long long WAIT_CLOCKS = 1ll << 25;   // some 17 ms, far beyond any legitimate wait
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -513,17 +515,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -573,40 +564,70 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][TC_ROWS * HD * 2];
   alignas(1024) uint8_t k[STAGES][TC_KEYS * HD * 2];
   alignas(1024) uint8_t v[STAGES][TC_KEYS * HD * 2];
-  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], drained;
-  float top[2][2][TC_ROWS];   // [group][half of the keys][row]: a tile's largest score
+  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], drained, pair[2][4];
+  float first[2][2][TC_ROWS], asked[2][2][2][TC_ROWS];   // [group][half of the keys][row]: a first tile's largest score; [parity of the
+                                                         // tile]..: the reference asked for
   float2 ml[2][2][TC_ROWS];   // the reference and the sum
   Walk start;
   uint32_t tmem_base;
   int abort_flag;
 };
 
-// A dim a lane of one row's sums over the keys of a segment that it sees, against the reference maximum m, by one warp in 32 bits.  For
-// a row whose sums came out NaN or Inf: the tensor core's product takes whole tiles of values, and a probability of zero does not keep
-// out a NaN or Inf among those that the row does not see.
-__device__ __noinline__ float tree_row_again(const TreeArgs a, const Segment s, int row, int dim, float m, float cap_log2, float cap_in2) {
-  const int lane = threadIdx.x & 31, group = a.H / a.G, hd = a.hd;
-  const int token = (s.row0 + row) / group, head = s.g * group + (s.row0 + row) % group;
-  const TreeRow w = tree_row(a, s.q, token, true);
-  const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * hd;
-  const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
-  const float safe = m == -CUDART_INF_F ? 0.f : m, scale_log2 = a.scale * 1.4426950408889634f;
-  float acc = 0.f;
-  for (int j0 = s.t0 * TC_KEYS; j0 < min((s.t0 + s.n) * TC_KEYS, s.q.context + s.q.count); j0 += 32) {
-    const uint32_t see = visible32(w, j0);
-    if (see == 0) continue;
-    float p = 0.f;
-    long long at = -1;
-    if ((see >> lane) & 1u) {
-      const int j = j0 + lane, page = bt[j / a.page_tokens];
-      if (page >= 0 && page < a.num_pages) {
-        at = (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * hd;
-        const bf16* k = reinterpret_cast<const bf16*>(a.k) + at;
-        float x = 0.f;
-        for (int d = 0; d < hd; ++d) x = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), x);
-        p = exp2f(log2_score(x, scale_log2, cap_log2, cap_in2) - safe);
-      }
-    }
+// One row once more, by one warp in 32 bits over the keys of a segment that it sees.  For a row whose sums came out NaN or Inf: the
+// tensor core's product takes whole tiles of values, and a probability of zero does not keep out a NaN or Inf among those that the row
+// does not see; or one tile's scores ran too far ahead of the reference.
+struct RowKeys {
+  const bf16* q;
+  const int* bt;
+  TreeRow w;
+  float scale_log2;
+  int j, end;
+};
+__device__ __forceinline__ RowKeys row_keys(const TreeArgs& a, const Segment& s, int row) {
+  const int group = a.H / a.G, token = (s.row0 + row) / group, head = s.g * group + (s.row0 + row) % group;
+  RowKeys k;
+  k.w = tree_row(a, s.q, token, true);
+  k.q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * a.hd;
+  k.bt = a.block_table + (size_t)s.q.slot * a.table_stride;
+  k.scale_log2 = a.scale * 1.4426950408889634f;
+  k.j = s.t0 * TC_KEYS;
+  k.end = min((s.t0 + s.n) * TC_KEYS, s.q.context + s.q.count);
+  return k;
+}
+// This lane's key of the next 32: its score and the place of its row in the pages, or -1 where the row does not see it.
+__device__ __forceinline__ long long next_key(const TreeArgs& a, const Segment& s, RowKeys& k, float cap_log2, float cap_in2, float& score) {
+  const uint32_t see = visible32(k.w, k.j);
+  const int j = k.j + (int)(threadIdx.x & 31);
+  k.j += 32;
+  if (!((see >> (threadIdx.x & 31)) & 1u)) return -1;
+  const int page = k.bt[j / a.page_tokens];
+  if (page < 0 || page >= a.num_pages) return -1;
+  const long long at = (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * a.hd;
+  const bf16* key = reinterpret_cast<const bf16*>(a.k) + at;
+  float x = 0.f;
+  for (int d = 0; d < a.hd; ++d) x = fmaf(__bfloat162float(k.q[d]), __bfloat162float(key[d]), x);
+  score = log2_score(x, k.scale_log2, cap_log2, cap_in2);
+  return at;
+}
+// The row's largest score m and the sum l of exp2(score - m).
+__device__ __noinline__ void tree_row_top(const TreeArgs& a, const Segment& s, int row, float cap_log2, float cap_in2, float& m, float& l) {
+  float score, top = -CUDART_INF_F, sum = 0.f;
+  for (RowKeys k = row_keys(a, s, row); k.j < k.end;)
+    if (next_key(a, s, k, cap_log2, cap_in2, score) >= 0) top = fmaxf(top, score);
+  top = warp_max(top);
+  const float safe = top == -CUDART_INF_F ? 0.f : top;
+  for (RowKeys k = row_keys(a, s, row); k.j < k.end;)
+    if (next_key(a, s, k, cap_log2, cap_in2, score) >= 0) sum += exp2f(score - safe);
+  m = top;
+  l = warp_sum(sum);
+}
+// A dim a lane of the row's sums against the reference m.
+__device__ __noinline__ float tree_row_again(const TreeArgs& a, const Segment& s, int row, int dim, float m, float cap_log2, float cap_in2) {
+  const float safe = m == -CUDART_INF_F ? 0.f : m;
+  float acc = 0.f, score = 0.f;
+  for (RowKeys k = row_keys(a, s, row); k.j < k.end;) {
+    const long long at = next_key(a, s, k, cap_log2, cap_in2, score);
+    const float p = exp2f(score - safe);
     for (uint32_t left = __ballot_sync(0xffffffffu, at >= 0); left; left &= left - 1) {
       const int i = __ffs(left) - 1;
       const float f = __shfl_sync(0xffffffffu, p, i);
@@ -618,7 +639,7 @@ __device__ __noinline__ float tree_row_again(const TreeArgs a, const Segment s, 
 
 template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1)
-tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeArgs a, float cap_log2, float cap_in2) {
+tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeArgs a, float cap_log2, float cap_in2) {
   constexpr int STAGES = TcSmem<HD>::STAGES, CPR = HD / 8, KSTEPS = HD / 16, HALVES = HD / 64;
   constexpr int MMA_WARP = TC_SOFTMAX / 32, LOAD_WARP = MMA_WARP + 1;
   constexpr uint32_t TMEM_COLS = 512, SP_COL[2] = {0, 128}, O_COL[2] = {256, 256 + HD};
@@ -632,7 +653,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.G;
 
   if (threadIdx.x == 32) {
-    mbar_init(&sm.q_full, TC_SOFTMAX);
+    mbar_init(&sm.q_full, TC_SOFTMAX / 32);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.v_full[i], 1);
@@ -641,8 +662,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], TC_SOFTMAX / 2);
+      mbar_init(&sm.p_full[i], TC_SOFTMAX / 64);
       mbar_init(&sm.o_done[i], 1);
+      for (int j = 0; j < 4; ++j) mbar_init(&sm.pair[i][j], 2);
     }
     mbar_init(&sm.drained, 1);
     sm.abort_flag = 0;
@@ -666,25 +688,35 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   Segment s;
 
   if (warp == LOAD_WARP) {
-    // ================================================================= loads (a lane per box of a page's keys)
+    // ================================================================= loads (a lane per box of a page's keys and half of the head)
     const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows;
+    const int box = lane & (boxes - 1), h = lane / boxes;      // boxes: a power of two up to 16
     int n = 0;                    // tiles sent for so far
     bool alive = true;
     while (alive && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
       const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
-      const int end = s.q.context + s.q.count, begin = first_key(a, s.q);
-      // This lane's box of a tile: its first row of the pages, seen as one matrix.  A box that holds no key of the request is the one
-      // of its nearest key, so that nothing but cache rows ever lies in a stage: an old NaN pattern there would not be kept out of the
-      // sums by a probability of zero.
-      auto box_row = [&](int t) -> int {
-        const int j = min(max(t * TC_KEYS + min(lane, boxes - 1) * box_rows, begin / box_rows * box_rows), (end - 1) / box_rows * box_rows);
-        const int page = bt[j / a.page_tokens];
-        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + j % a.page_tokens : 0;
+      const int first = first_key(a, s.q) / box_rows, last = (s.q.context + s.q.count - 1) / box_rows;
+      // Box b of the request: its page, and from that its first row of the pages, seen as one matrix.  A box that holds no key of the
+      // request is the one of its nearest key, so that nothing but cache rows ever lies in a stage: an old NaN pattern there would not
+      // be kept out of the sums by a probability of zero.
+      auto key_of = [&](int b) { return min(max(b, first), last) * box_rows; };
+      auto row_of = [&](int b, int page) {
+        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + key_of(b) % a.page_tokens : 0;
       };
-      int next = box_row(s.t0);
+      // 32 boxes at a time, a lane each; the next 32 are on their way meanwhile
+      int at = s.t0 * boxes + lane;
+      int row = row_of(at, bt[key_of(at) / a.page_tokens]);
+      int page = bt[key_of(at + 32) / a.page_tokens];
+      int sent = 0;
       for (int i = 0; i < s.n && alive; ++i, ++n) {
-        const int row = next, st = n % STAGES;
-        if (i + 1 < s.n) next = box_row(s.t0 + i + 1);          // on its way while the stage is waited for
+        if (sent == 32) {
+          at += 32;
+          row = row_of(at, page);
+          page = bt[key_of(at + 32) / a.page_tokens];
+          sent = 0;
+        }
+        const int mine = __shfl_sync(0xffffffffu, row, sent + box), st = n % STAGES;
+        sent += boxes;
         const uint32_t parity = (uint32_t)(((n / STAGES) & 1) ^ 1);      // a fresh barrier lets the first fill through
         for (int kv = 0; kv < 2 && alive; ++kv) {
           uint64_t* full = kv == 0 ? &sm.k_full[st] : &sm.v_full[st];
@@ -694,11 +726,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (go) mbar_expect_tx(full, TC_KEYS * HD * 2);
           }
           alive = __shfl_sync(0xffffffffu, go, 0) != 0;
-          if (alive && lane < boxes) {
-            const uint32_t base = smem_u32(kv == 0 ? sm.k[st] : sm.v[st]) + (uint32_t)(lane * box_rows) * 128u;
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) tma_load_3d(base + (uint32_t)h * (TC_KEYS * 128), kv == 0 ? &map_k : &map_v, full, 0, row, h);
-          }
+          if (alive && h < HALVES)
+            tma_load_3d(smem_u32(kv == 0 ? sm.k[st] : sm.v[st]) + (uint32_t)(box * box_rows + h * TC_KEYS) * 128u, kv == 0 ? &map_k : &map_v, full, 0, mine, h);
         }
       }
     }
@@ -772,7 +801,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const float scale_log2 = a.scale * 1.4426950408889634f;
     const float sl = cap_log2 > 0.f ? 1.0f : scale_log2;       // capped scores are in the exponent's domain already
     const uint32_t sp = lane_addr + (x ? SP_COL[1] : SP_COL[0]), oc = lane_addr + (x ? O_COL[1] : O_COL[0]);
-    uint32_t jobs_done = 0, o_done[2] = {0, 0};
+    uint32_t jobs_done = 0, met = 0, o_done[2] = {0, 0};
     bool ok = true;
     // Q: the threads of a row share it out; rows past the unit are zeros
     auto send_q = [&](const Segment& u) {
@@ -794,61 +823,65 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       const int row = two ? x * TC_ROWS + r : r;
       const bool valid = row < s.rows, busy = row - lane < s.rows;        // busy: any row of the warp is one
       const int token = valid ? (s.row0 + row) / group : 0;
-      const int lo = valid ? tree_row(a, s.q, token, true).lo : 0x7fffffff;
+      const int lo = valid ? tree_row(a, s.q, token, true).lo : 0;
       cp_async_wait<0>();
       fence_async_proxy();
-      mbar_arrive(&sm.q_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
       const int jobs = two ? s.n : (s.n + 1 - x) / 2;
       float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
       for (int n = 0; n < jobs; ++n, ++jobs_done) {
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) ok = false;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) { ok = false; break; }
         if (!busy) {
-          if (ok) mbar_arrive(&sm.p_full[x]);
+          if (lane == 0) mbar_arrive(&sm.p_full[x]);
           continue;
         }
         const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
         const bool part = j0 < lo || j0 + HK > s.q.context;
         uint32_t see[2] = {0xffffffffu, 0xffffffffu}, su[32];
-        if (ok) {
-          // the largest score that counts; the scores are read from tensor memory once more below: a thread holds 32 of them, not 64
-          tc_fence_after();
-          float top = -CUDART_INF_F;
-          if (part) {
-            const TreeRow tr = tree_row(a, s.q, token, valid);
-            see[0] = visible32(tr, j0);
-            see[1] = visible32(tr, j0 + 32);
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
-            tmem_ld_wait();
-            if (part) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) su[i] = (see[c] >> i) & 1u ? su[i] : 0xff800000u;      // -inf
-            }
-            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(su[i + 2 * e]), __uint_as_float(su[i + 2 * e + 1])));
-            }
-            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-          }
-          // (a cap climbs with the score: the largest stays the largest; a masked one stays out of it)
-          sm.top[x][half][r] = cap_log2 > 0.f && (see[0] | see[1]) ? log2_score(top, 1.0f, cap_log2, cap_in2) : top * sl;
+        if (part) {
+          const TreeRow tr = tree_row(a, s.q, token, valid);
+          see[0] = visible32(tr, j0);
+          see[1] = visible32(tr, j0 + 32);
         }
-        // the row's other thread; who gave up comes here all the same, or the other would wait for good
-        asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * x + quarter) : "memory");
-        if (!ok) continue;
-        const float cm = fmaxf(sm.top[x][0][r], sm.top[x][1][r]);
-        // The scores are complete, and so is every product issued before them, the last with V among them: O may be touched.
-        const bool move = cm > m + LAZY;                  // also true for the first finite maximum (m = -inf)
-        if (__any_sync(0xffffffffu, move)) {
-          const float mn = move ? ceilf(cm) : m;
-          const float corr = move ? exp2f(m - mn) : 1.0f;      // m = -inf: 0; nothing was summed yet
-          l0 *= corr;
-          l1 *= corr;
-          if (n > 0) {
+        tc_fence_after();
+        // 32 of the thread's scores, capped and in the exponent's domain but for the factor sl, -inf where they do not count
+        auto load = [&](int c) {
+          tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
+          tmem_ld_wait();
+          if (cap_log2 > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) su[i] = __float_as_uint(log2_score(__uint_as_float(su[i]), 1.0f, cap_log2, cap_in2));
+          }
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) su[i] = ((c ? see[1] : see[0]) >> i) & 1u ? su[i] : 0xff800000u;
+          }
+        };
+        // The scores are complete, and so is every product issued before them, the last with V among them: O may be touched.  m is alike
+        // in a row's two threads, and so are both branches.
+        if (__any_sync(0xffffffffu, valid && m == -CUDART_INF_F)) {
+          float top = -CUDART_INF_F;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            load(c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(su[i]));
+          }
+          sm.first[x][half][r] = top * sl;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.pair[x][quarter]);
+          if (!__all_sync(0xffffffffu, mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag))) { ok = false; break; }
+          ++met;
+          if (m == -CUDART_INF_F) m = ceilf(fmaxf(sm.first[x][0][r], sm.first[x][1][r]));
+        } else {
+          // what the two asked for behind the last tile (which all have announced: the wait is over already, and orders the reads)
+          if (!__all_sync(0xffffffffu, mbar_wait(&sm.p_full[x], (jobs_done - 1) & 1u, abort_flag))) { ok = false; break; }
+          const float asked = fmaxf(sm.asked[(n - 1) & 1][x][0][r], sm.asked[(n - 1) & 1][x][1][r]);
+          if (__any_sync(0xffffffffu, asked > m)) {
+            const float corr = asked > m ? exp2f(m - asked) : 1.0f;
+            l0 *= corr;
+            l1 *= corr;
 #pragma unroll 1
             for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 16) {
               uint32_t o[16];
@@ -858,23 +891,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
               tmem_st16(oc + (uint32_t)c0, o);
             }
+            m = fmaxf(m, asked);
           }
-          m = mn;
         }
-        const float shift = m == -CUDART_INF_F ? 0.f : -m;
+        const float shift = m == -CUDART_INF_F ? 0.f : -m, l_before = l0 + l1;
         // a half's P lies in the columns of its own scores that are read already
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
-          tmem_ld_wait();
-          if (cap_log2 > 0.f) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) su[i] = __float_as_uint(log2_score(__uint_as_float(su[i]), 1.0f, cap_log2, cap_in2));
-          }
-          if (part) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) su[i] = (see[c] >> i) & 1u ? su[i] : 0xff800000u;
-          }
+          load(c);
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -887,9 +911,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           }
           tmem_st16(sp + (uint32_t)(half * HK + 16 * c), pw);
         }
+        const float more_l = l0 + l1 - l_before;
+        float ask = m;
+        if (!(more_l <= MUCH)) {
+          ask = m + ceilf(log2f(more_l));
+          if (!(more_l <= TOO_MUCH)) {
+            l0 = CUDART_NAN_F;
+            ask = m;
+          }
+        }
+        sm.asked[n & 1][x][half][r] = ask;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&sm.p_full[x]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[x]);
       }
       // the sums of both groups: a row's two threads (four where the groups share their rows) take a part of its dims each
       const bool second = two || s.n > 1;              // the second group had a tile at all
@@ -919,18 +954,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         }
         const int head = s.g * group + (s.row0 + (valid ? row : 0)) % group;
         const size_t slot = part_slot(blockIdx.x, s.begins);
-        float inv = 1.0f;
-        if (s.whole) {
-          float total = l;
+        // one over a row's denominator, the sink's term in it
+        auto finish = [&](float top, float sum, int of_head) {
+          float f = 1.0f;
           if (a.sink) {
-            const float score = (a.sinks ? a.sinks[head] : 0.f) * 1.4426950408889634f, top = fmaxf(m, score);
-            inv = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
-            total = l * inv + exp2f(score - top);
+            const float score = (a.sinks ? a.sinks[of_head] : 0.f) * 1.4426950408889634f, high = fmaxf(top, score);
+            f = top == -CUDART_INF_F ? 0.f : exp2f(top - high);
+            sum = sum * f + exp2f(score - high);
           }
-          inv = total > 0.f || total != total ? inv / total : 0.f;
-        } else if (valid && half == 0 && (two || x == 0)) {
-          *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + row) = make_float2(m, l);
-        }
+          return sum > 0.f || sum != sum ? f / sum : 0.f;
+        };
+        float inv = 1.0f;
+        if (s.whole) inv = finish(m, l, head);
+        else if (valid && half == 0 && (two || x == 0)) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + row) = make_float2(m, l);
         bf16* op = reinterpret_cast<bf16*>(a.out) + ((size_t)(s.q.first + token) * a.H + head) * HD;
         float odd = 0.f;                               // NaN where a sum is NaN or Inf
         const int c_from = two ? half * (HD / 2) : (2 * x + half) * (HD / 4), c_to = c_from + (two ? HD / 2 : HD / 4);
@@ -963,14 +999,22 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
               *reinterpret_cast<uint4*>(part_place(a, slot, row, c0 + i, HD)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
+        if (!(l <= CUDART_MAX_NORMAL_F)) odd = CUDART_NAN_F;         // alike in all threads of a row
         for (unsigned again = __ballot_sync(0xffffffffu, valid && odd != 0.f); again; again &= again - 1) {
+          const Segment unit = s;
           __syncwarp();
           const int from = __ffs(again) - 1, at = row - lane + from;
-          const float m_row = __shfl_sync(0xffffffffu, m, from), inv_row = __shfl_sync(0xffffffffu, inv, from);
+          float m_row = __shfl_sync(0xffffffffu, m, from), l_row = __shfl_sync(0xffffffffu, l, from), inv_row = __shfl_sync(0xffffffffu, inv, from);
           bf16* op_row = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)op, from));
+          const int head_row = __shfl_sync(0xffffffffu, head, from);
+          if (!(l_row <= CUDART_MAX_NORMAL_F)) {        // the reference and the sum as well
+            tree_row_top(a, unit, at, cap_log2, cap_in2, m_row, l_row);
+            if (s.whole) inv_row = finish(m_row, l_row, head_row);
+            else if (lane == 0 && half == 0 && (two || x == 0)) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + at) = make_float2(m_row, l_row);
+          }
           for (int c0 = c_from; c0 < c_to; c0 += 32) {
             const int dim = c0 + lane;
-            const float y = tree_row_again(a, s, at, min(dim, HD - 1), m_row, cap_log2, cap_in2);
+            const float y = tree_row_again(a, unit, at, min(dim, HD - 1), m_row, cap_log2, cap_in2);
             if (dim < c_to) {
               if (s.whole) op_row[dim] = __float2bfloat16_rn(y * inv_row);
               else part_place(a, slot, at, dim, HD)[dim & 3] = y;
