@@ -413,19 +413,21 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 }
 
 // ---- bfloat16 on the tensor cores ---------------------------------------------------------------------------------------------
-// A tile has up to 256 rows.  Two groups of eight softmax warps (two threads a row, half of a tile's keys each), one lane that issues
-// the products and one warp that loads K and V by TMA work on it side by side: with more than 128 rows each group has half of them and
-// every key tile serves both; with up to 128 rows both groups have the same rows and take the key tiles in turn, and their sums meet in
-// tensor memory at the end.  Either way one group's exponentials run while the tensor core works for the other.  Tensor memory (512
-// columns): per group 128 columns of scores, which the probabilities overwrite (bfloat16, each half 32 columns), and HD of sums.  A group's next
-// scores are issued behind its product with V; products of one thread run in order, so they overwrite P only once it was read.
+// A tile has up to 256 rows.  Two groups of eight softmax warps, a lane for each that issues its products and two warps that
+// load K and V by TMA work on it side by side: with more than 128 rows each group has half of them and every key tile serves both; with up to 128 rows
+// both groups have the same rows and take the key tiles in turn, and their sums meet in tensor memory at the end.  A group's first four
+// warps take the first 64 keys of a tile, a thread a row, and the others the last 64: so there are four streams of scores -> probabilities
+// -> product with V, and while the tensor core works for one the exponentials of the others run.  Tensor memory (512 columns): per stream
+// 64 columns of scores, which the probabilities overwrite (bfloat16, 32 columns), per group HD of sums.  A stream's next scores are issued
+// behind its product with V; products of one thread run in order, so they overwrite P only once it was read.  (One lane for both groups was
+// what the kernel waited for: a product takes it some 40 clocks to issue, and a tile of 256 rows is 48 of them.)
 //
 // Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits).  They are taken against a reference, an
 // integer near the largest score of the first tile in which a row sees anything: bfloat16 and the sums in float32 have exponents to
-// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference for
-// the next one, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
+// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference two
+// tiles later, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
 // threads need not meet over it.  Where one tile jumps by more than 2^60 the row's sum is set to NaN, and the row is taken again (below).
-constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 64;
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 128;
 constexpr float MUCH = 16777216.0f, TOO_MUCH = 1152921504606846976.0f;      // 2^24, 2^60
 constexpr long long WAIT_CLOCKS = 1ll << 25;   // some 17 ms, far beyond any legitimate wait
 
@@ -564,9 +566,9 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][TC_ROWS * HD * 2];
   alignas(1024) uint8_t k[STAGES][TC_KEYS * HD * 2];
   alignas(1024) uint8_t v[STAGES][TC_KEYS * HD * 2];
-  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], drained, pair[2][4];
-  float first[2][2][TC_ROWS], asked[2][2][2][TC_ROWS];   // [group][half of the keys][row]: a first tile's largest score; [parity of the
-                                                         // tile]..: the reference asked for
+  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2][2], p_full[2][2], o_done[2], drained[2], pair[2][4];
+  float first[2][2][2][TC_ROWS], asked[4][2][2][TC_ROWS];   // [tile % 2][group][half of the keys][row]: a first tile's largest score;
+                                                            // [tile % 4]..: the reference asked for
   float2 ml[2][2][TC_ROWS];   // the reference and the sum
   Walk start;
   uint32_t tmem_base;
@@ -641,10 +643,10 @@ template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeArgs a, float cap_log2, float cap_in2) {
   constexpr int STAGES = TcSmem<HD>::STAGES, CPR = HD / 8, KSTEPS = HD / 16, HALVES = HD / 64;
-  constexpr int MMA_WARP = TC_SOFTMAX / 32, LOAD_WARP = MMA_WARP + 1;
+  constexpr int MMA_WARP = TC_SOFTMAX / 32, LOAD_WARP = MMA_WARP + 2;
   constexpr uint32_t TMEM_COLS = 512, SP_COL[2] = {0, 128}, O_COL[2] = {256, 256 + HD};
   // fp32 accumulators, bf16 operands; N at bit 17 (>> 3), M at bit 24 (>> 4); bit 16: B is MN-major
-  constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC_KEYS >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+  constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TC_KEYS >> 4) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
   constexpr uint32_t IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
 
   extern __shared__ uint8_t smem_raw[];
@@ -657,16 +659,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.v_full[i], 1);
-      mbar_init(&sm.k_empty[i], 1);
-      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.k_empty[i], 2);
+      mbar_init(&sm.v_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], TC_SOFTMAX / 64);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sm.s_full[i][j], 2);
+        mbar_init(&sm.p_full[i][j], TC_SOFTMAX / 128);
+      }
       mbar_init(&sm.o_done[i], 1);
+      mbar_init(&sm.drained[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&sm.pair[i][j], 2);
     }
-    mbar_init(&sm.drained, 1);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -687,10 +691,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   Walk w = sm.start;
   Segment s;
 
-  if (warp == LOAD_WARP) {
+  if (warp >= LOAD_WARP) {
     // ================================================================= loads (a lane per box of a page's keys and half of the head)
     const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows;
     const int box = lane & (boxes - 1), h = lane / boxes;      // boxes: a power of two up to 16
+    // A warp for K and one for V: a stream's next scores want K tiles before the V tiles are free that one warp would have to send for first.
+    const bool is_v = warp != LOAD_WARP;
+    uint64_t *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
+    const uint32_t stages = smem_u32(is_v ? sm.v[0] : sm.k[0]) + (uint32_t)(box * box_rows + h * TC_KEYS) * 128u;
+    const CUtensorMap* map = is_v ? &map_v : &map_k;
     int n = 0;                    // tiles sent for so far
     bool alive = true;
     while (alive && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
@@ -718,83 +727,88 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int mine = __shfl_sync(0xffffffffu, row, sent + box), st = n % STAGES;
         sent += boxes;
         const uint32_t parity = (uint32_t)(((n / STAGES) & 1) ^ 1);      // a fresh barrier lets the first fill through
-        for (int kv = 0; kv < 2 && alive; ++kv) {
-          uint64_t* full = kv == 0 ? &sm.k_full[st] : &sm.v_full[st];
-          int go = 1;
-          if (lane == 0) {
-            go = mbar_wait(kv == 0 ? &sm.k_empty[st] : &sm.v_empty[st], parity, abort_flag) ? 1 : 0;
-            if (go) mbar_expect_tx(full, TC_KEYS * HD * 2);
-          }
-          alive = __shfl_sync(0xffffffffu, go, 0) != 0;
-          if (alive && h < HALVES)
-            tma_load_3d(smem_u32(kv == 0 ? sm.k[st] : sm.v[st]) + (uint32_t)(box * box_rows + h * TC_KEYS) * 128u, kv == 0 ? &map_k : &map_v, full, 0, mine, h);
+        int go = 1;
+        if (lane == 0) {
+          go = mbar_wait(&empty[st], parity, abort_flag) ? 1 : 0;
+          if (go) mbar_expect_tx(&full[st], TC_KEYS * HD * 2);
         }
+        alive = __shfl_sync(0xffffffffu, go, 0) != 0;
+        if (alive && h < HALVES) tma_load_3d(stages + (uint32_t)(st * TC_KEYS * HD * 2), map, &full[st], 0, mine, h);
       }
     }
     if (*abort_flag && lane == 0) {          // the copies that are still on their way
-      for (int i = max(0, n - STAGES); i <= n; ++i) {
-        if (i < n) mbar_drain(&sm.v_full[i % STAGES], (uint32_t)((i / STAGES) & 1));
-        if (i < n || !alive) mbar_drain(&sm.k_full[i % STAGES], (uint32_t)((i / STAGES) & 1));
-      }
+      for (int i = max(0, n - STAGES); i < n; ++i) mbar_drain(&full[i % STAGES], (uint32_t)((i / STAGES) & 1));
     }
-  } else if (warp == MMA_WARP) {
-    // ================================================================= products (one lane)
+  } else if (warp >= MMA_WARP) {
+    // ================================================================= products (one lane a group)
+    const uint32_t x = __shfl_sync(0xffffffffu, (uint32_t)(warp - MMA_WARP), 0);
     if (elect_one()) {
-      bool ok = true;
-      int nk = 0, nv = 0, jobs_done[2] = {0, 0};
-      uint32_t seg = 0;
-      bool issued = false;
+      bool ok = true, issued = false;
+      uint32_t tiles_done = 0, steps = 0, seg = 0;
+      const uint32_t sp = tmem + x * SP_COL[1], oc = tmem + O_COL[0] + x * HD;
+      const uint64_t dq0 = desc_k_major(smem_u32(sm.q[0])), dk0 = desc_k_major(smem_u32(sm.k[0])), dv0 = desc_mn_major(smem_u32(sm.v[0]), TC_KEYS * 128);
+      constexpr uint32_t STAGE16 = TC_KEYS * HD * 2 >> 4, HALF16 = TC_KEYS / 2 * 128 >> 4;      // descriptors count in 16 bytes
       while (ok && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
         const bool two = s.rows > TC_ROWS;
-        const int jobs = two ? 2 * s.n : s.n;          // job j: group j & 1; tile j / 2 with two row tiles, else j
+        const int jobs = two ? s.n : (s.n + 1 - (int)x) / 2;
         if (!mbar_wait(&sm.q_full, seg & 1u, abort_flag)) { ok = false; break; }
         ++seg;
-        auto issue_s = [&](int j) -> bool {
-          const int x = j & 1, st = nk % STAGES;
-          if ((!two || x == 0) && !mbar_wait(&sm.k_full[st], (uint32_t)((nk / STAGES) & 1), abort_flag)) return false;
+        const uint64_t dq = dq0 + (two && x ? TC_ROWS * HD * 2 >> 4 : 0);
+        // Step t of the group: tile t of the unit with two row tiles, else tile 2 t + x.  A tile is free when both groups are through with
+        // it, or where only one takes it, when that one is.
+        auto issue_s = [&](int h, uint32_t n) -> bool {
+          const uint32_t st = n % STAGES;
+          if (h == 0 && !mbar_wait(&sm.k_full[st], (n / STAGES) & 1u, abort_flag)) return false;
           tc_fence_after();
-          const uint32_t qs = smem_u32(sm.q[two ? x : 0]), ks = smem_u32(sm.k[st]);
+          const uint64_t dk = dk0 + st * STAGE16 + (uint32_t)h * HALF16;
 #pragma unroll
           for (int kk = 0; kk < KSTEPS; ++kk)
-            umma(tmem + SP_COL[x], desc_k_major(qs + (uint32_t)((kk >> 2) * (TC_ROWS * 128) + (kk & 3) * 32)),
-                 desc_k_major(ks + (uint32_t)((kk >> 2) * (TC_KEYS * 128) + (kk & 3) * 32)), IDESC_S, kk ? 1u : 0u);
+            umma(sp + (uint32_t)(h * (TC_KEYS / 2)), dq + ((kk >> 2) * (TC_ROWS * 128 >> 4) + (kk & 3) * 2), dk + ((kk >> 2) * (TC_KEYS * 128 >> 4) + (kk & 3) * 2),
+                 IDESC_S, kk ? 1u : 0u);
           issued = true;
-          umma_commit(&sm.s_full[x]);
-          if (!two || x == 1) {
+          umma_commit(&sm.s_full[x][h]);
+          mbar_arrive(&sm.s_full[x][h]);          // what this thread has seen of the softmax threads' announcements, in order with the scores
+          if (h == 1) {
             umma_commit(&sm.k_empty[st]);
-            ++nk;
+            if (!two) mbar_arrive(&sm.k_empty[st]);
           }
           return true;
         };
-        ok = issue_s(0) && (jobs < 2 || issue_s(1));
-        for (int j = 0; j < jobs && ok; ++j) {
-          const int x = j & 1, st = nv % STAGES;
-          if (!mbar_wait(&sm.p_full[x], (uint32_t)(jobs_done[x] & 1), abort_flag)) { ok = false; break; }
-          ++jobs_done[x];
-          if ((!two || x == 0) && !mbar_wait(&sm.v_full[st], (uint32_t)((nv / STAGES) & 1), abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t vs = smem_u32(sm.v[st]);
+        uint32_t n = tiles_done + (two ? 0 : x);
+        if (jobs > 0) ok = issue_s(0, n) && issue_s(1, n);
+        for (int t = 0; t < jobs && ok; ++t) {
+          const uint32_t st = n % STAGES, next = n + (two ? 1 : 2);
+          const uint64_t dv = dv0 + st * STAGE16;
 #pragma unroll
-          for (int kk = 0; kk < TC_KEYS / 16; ++kk)
-            umma_ts(tmem + O_COL[x], tmem + SP_COL[x] + (uint32_t)((kk >> 2) * (TC_KEYS / 2) + (kk & 3) * 8), desc_mn_major(vs + (uint32_t)kk * 2048u, (uint32_t)(TC_KEYS * 128)), IDESC_O,
-                    (j > 1 || kk > 0) ? 1u : 0u);
-          if (!two || x == 1) {
-            umma_commit(&sm.v_empty[st]);
-            ++nv;
+          for (int h = 0; h < 2; ++h) {
+            if (!ok) break;
+            if (!mbar_wait(&sm.p_full[x][h], (steps + t) & 1u, abort_flag) ||
+                (h == 0 && !mbar_wait(&sm.v_full[st], (n / STAGES) & 1u, abort_flag))) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TC_KEYS / 32; ++kk)
+              umma_ts(oc, sp + (uint32_t)(h * (TC_KEYS / 2) + kk * 8), dv + (uint32_t)h * HALF16 + kk * (2048 >> 4), IDESC_O, (t > 0 || h > 0 || kk > 0) ? 1u : 0u);
+            if (h == 1) {
+              umma_commit(&sm.v_empty[st]);
+              if (!two) mbar_arrive(&sm.v_empty[st]);
+            }
+            if (t + 1 < jobs) ok = issue_s(h, next);       // behind this stream's product with V: it overwrites the P that it reads
+            else if (h == 1) umma_commit(&sm.o_done[x]);
           }
-          if (j + 2 < jobs) ok = issue_s(j + 2);       // behind this job's product with V: it overwrites the P that it reads
-          else umma_commit(&sm.o_done[x]);
+          n = next;
         }
+        tiles_done += s.n;
+        steps += jobs;
       }
       if (!ok && issued) {                             // the products that are still under way
-        umma_commit(&sm.drained);
-        mbar_drain(&sm.drained, 0);
+        umma_commit(&sm.drained[x]);
+        mbar_drain(&sm.drained[x], 0);
       }
     }
   } else {
     // ================================================================= softmax (two groups of 256 threads, two a row)
     // Warps w and w + 4 of a group read the same lanes of tensor memory (32 * (w & 3) ..): the first the lower half of a tile's keys, the
-    // second the upper.  A row's two threads meet through shared memory for its maximum and its sum.
+    // second the upper.
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;      // r: row of the tile = lane of tensor memory
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     constexpr int HK = TC_KEYS / 2, EC = 16;        // keys a thread; dims of the sums that a thread finishes at once
@@ -831,9 +845,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       const int jobs = two ? s.n : (s.n + 1 - x) / 2;
       float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
       for (int n = 0; n < jobs; ++n, ++jobs_done) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x], jobs_done & 1u, abort_flag))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x][half], jobs_done & 1u, abort_flag))) { ok = false; break; }
         if (!busy) {
-          if (lane == 0) mbar_arrive(&sm.p_full[x]);
+          if (lane == 0) mbar_arrive(&sm.p_full[x][half]);
           continue;
         }
         const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
@@ -858,8 +872,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             for (int i = 0; i < 32; ++i) su[i] = ((c ? see[1] : see[0]) >> i) & 1u ? su[i] : 0xff800000u;
           }
         };
-        // The scores are complete, and so is every product issued before them, the last with V among them: O may be touched.  m is alike
-        // in a row's two threads, and so are both branches.
+        // m is alike in a row's two threads, and so are the branches that they take
         if (__any_sync(0xffffffffu, valid && m == -CUDART_INF_F)) {
           float top = -CUDART_INF_F;
 #pragma unroll 1
@@ -868,17 +881,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(su[i]));
           }
-          sm.first[x][half][r] = top * sl;
+          sm.first[n & 1][x][half][r] = top * sl;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.pair[x][quarter]);
           if (!__all_sync(0xffffffffu, mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag))) { ok = false; break; }
           ++met;
-          if (m == -CUDART_INF_F) m = ceilf(fmaxf(sm.first[x][0][r], sm.first[x][1][r]));
-        } else {
-          // what the two asked for behind the last tile (which all have announced: the wait is over already, and orders the reads)
-          if (!__all_sync(0xffffffffu, mbar_wait(&sm.p_full[x], (jobs_done - 1) & 1u, abort_flag))) { ok = false; break; }
-          const float asked = fmaxf(sm.asked[(n - 1) & 1][x][0][r], sm.asked[(n - 1) & 1][x][1][r]);
+          if (m == -CUDART_INF_F) m = ceilf(fmaxf(sm.first[n & 1][x][0][r], sm.first[n & 1][x][1][r]));
+        } else if (n >= 2) {
+          // what the two asked for two tiles ago: the tensor core's thread had seen both announce it before it issued these scores
+          const float asked = fmaxf(sm.asked[(n - 2) & 3][x][0][r], sm.asked[(n - 2) & 3][x][1][r]);
           if (__any_sync(0xffffffffu, asked > m)) {
+            // O may be touched: this half's product with V of the last tile is complete, since these scores are, and the other half's is
+            // once its scores are; the next ones wait for the two warps, which meet when both have done their part of the dims
+            bool fine = mbar_wait(&sm.s_full[x][half ^ 1], jobs_done & 1u, abort_flag);
+            tc_fence_after();
             const float corr = asked > m ? exp2f(m - asked) : 1.0f;
             l0 *= corr;
             l1 *= corr;
@@ -892,6 +908,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
               tmem_st16(oc + (uint32_t)c0, o);
             }
             m = fmaxf(m, asked);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.pair[x][quarter]);
+            fine = mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag) && fine;
+            tc_fence_after();
+            if (!__all_sync(0xffffffffu, fine)) { ok = false; break; }
+            ++met;
           }
         }
         const float shift = m == -CUDART_INF_F ? 0.f : -m, l_before = l0 + l1;
@@ -920,11 +944,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             ask = m;
           }
         }
-        sm.asked[n & 1][x][half][r] = ask;
+        sm.asked[n & 3][x][half][r] = ask;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[x]);
+        if (lane == 0) mbar_arrive(&sm.p_full[x][half]);
       }
       // the sums of both groups: a row's two threads (four where the groups share their rows) take a part of its dims each
       const bool second = two || s.n > 1;              // the second group had a tile at all

@@ -7,6 +7,15 @@ from ref_branches import TreeCase
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    if torch.cuda.is_available():
+        from hk_b200.csrc import gemm_fast
+        gemm_fast.check_status(torch.device("cuda", 0))
+
+
 SHAPES = [
     # contexts, drafted tokens, heads, key heads, dim, page
     ([0], [1], 4, 2, 64, 16),
@@ -19,6 +28,9 @@ SHAPES = [
     ([300], [256], 4, 1, 64, 128),
     ([513, 5, 90], [130, 1, 40], 10, 2, 128, 256),
     ([2100], [3], 5, 1, 128, 8),
+    ([30000], [16], 8, 2, 128, 16),
+    ([9000, 70, 12000], [64, 100, 17], 32, 8, 128, 16),
+    ([15000], [64], 8, 2, 64, 64),
     ([40], [20], 6, 2, 80, 16),
     ([33, 65], [9, 18], 4, 2, 16, 5),
     ([61], [10], 2, 1, 256, 16),
