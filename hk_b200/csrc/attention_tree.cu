@@ -9,12 +9,13 @@
 // what the tensor cores do in that time for T H / G up to about 250 rows.
 //
 // Work is cut on the device.  A unit is (request, tile of rows, key head) with its key tiles; all units' tiles, side by side, are
-// dealt to the CTAs of one wave in equal contiguous shares.  So whatever the lengths are, every CTA reads as much as the others,
-// and only a unit that a border falls into leaves partial results (at most two a CTA), which `tree_combine_kernel` merges in order.
+// dealt to the CTAs of one wave in equal contiguous shares (a unit counts LEAD tiles more: what starting one costs).  So whatever the
+// lengths are, every CTA works as long as the others, and only a unit that a border falls into leaves partial results (at most two a
+// CTA), which `tree_combine_kernel` merges in order.
 // Nothing depends on the host but bounds on the sizes: a launch can be captured and replayed over other contexts.
 //
-// What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays is skipped,
-// and a page outside the pool is not read.
+// What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays or the bounds is
+// skipped, and a page outside the pool is not read.
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -39,9 +40,14 @@ struct TreeArgs {
   float *part_o, *part_ml;
   int* status;
   long long num_pages;
-  int n, n_requests, most_tokens, words, table_rows, table_stride, page_tokens, H, G, hd, window, sink, rows_cap;
+  int n, n_requests, most_tokens, most_keys, words, table_rows, table_stride, page_tokens, H, G, hd, window, sink, rows_cap, group;
+  uint32_t group_inverse;  // 2^32 / group, rounded up (a group of 1: 0)
   float scale, softcap;    // scale on q . k; softcap c (0: none)
 };
+
+// Row `i` of a request (token * group + head of the group, at most 256 tokens): its token.  A division by a variable takes a hundred and
+// more clocks, of which the start of a short kernel has none to spare; i < 2^16 and group < 2^16 make this exact for their product below 2^32.
+__device__ __forceinline__ int token_of(const TreeArgs& a, int i) { return a.group == 1 ? i : (int)__umulhi((uint32_t)i, a.group_inverse); }
 
 // A request as the kernels take it: with nothing to do (count 0) where its numbers lie outside the arrays.
 __device__ __forceinline__ TreeReq load_request(const TreeArgs& a, int r) {
@@ -49,7 +55,7 @@ __device__ __forceinline__ TreeReq load_request(const TreeArgs& a, int r) {
   TreeReq q = {x.x, x.y, x.z, x.w};
   const bool fits = q.slot >= 0 && q.slot < a.table_rows && q.first >= 0 && q.count > 0 && q.count <= a.most_tokens && q.count <= 32 * a.words &&
                     q.first <= a.n - q.count && q.context >= 0 &&
-                    (long long)q.context + q.count <= (long long)a.table_stride * a.page_tokens;
+                    q.context <= a.most_keys - q.count;
   if (!fits) q.count = 0;
   return q;
 }
@@ -120,90 +126,86 @@ __device__ __forceinline__ float log2_score(float raw, float scale_log2, float c
 
 // ---- the shares of the CTAs ----------------------------------------------------------------------------------------------
 
-// The units of a request: tiles of ROWS rows times key heads, each of `tiles` key tiles of KEYS from tile `t_first` on.
-template <int ROWS, int KEYS>
+// How a kernel cuts: rows and keys of a tile, and what starting a unit costs in tiles.  All counts fit 32 bits (the launch sees to it).
+template <int R, int K, int L>
+struct Cut {
+  static constexpr int ROWS = R, KEYS = K, LEAD = L;
+};
+
+// The units of a request: tiles of ROWS rows times key heads, each of `tiles` key tiles from tile `t_first` on.
+template <typename C>
 __device__ __forceinline__ void unit_shape(const TreeArgs& a, const TreeReq& q, int& t_first, int& tiles, int& units) {
-  t_first = first_key(a, q) / KEYS;
-  tiles = q.count > 0 ? (q.context + q.count + KEYS - 1) / KEYS - t_first : 0;
-  units = q.count > 0 ? (q.count * (a.H / a.G) + ROWS - 1) / ROWS * a.G : 0;
+  t_first = first_key(a, q) / C::KEYS;
+  tiles = q.count > 0 ? (q.context + q.count + C::KEYS - 1) / C::KEYS - t_first : 0;
+  units = q.count > 0 ? (q.count * a.group + C::ROWS - 1) / C::ROWS * a.G : 0;
 }
 
-template <int ROWS, int KEYS>
-__device__ __forceinline__ long long tiles_of(const TreeArgs& a, int r) {
+template <typename C>
+__device__ __forceinline__ uint32_t size_of(const TreeArgs& a, int r) {
   if (r >= a.n_requests) return 0;
   int t_first, tiles, units;
-  unit_shape<ROWS, KEYS>(a, load_request(a, r), t_first, tiles, units);
-  return (long long)tiles * units;
+  unit_shape<C>(a, load_request(a, r), t_first, tiles, units);
+  return (uint32_t)(tiles + C::LEAD) * units;
 }
 
-__device__ __forceinline__ long long warp_sum64(long long v) {
+__device__ __forceinline__ uint32_t warp_sum32(uint32_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// By a whole warp: the tiles of all requests.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ long long count_tiles(const TreeArgs& a) {
-  long long t = 0;
-  for (int r = threadIdx.x & 31; r < a.n_requests; r += 32) t += tiles_of<ROWS, KEYS>(a, r);
-  return warp_sum64(t);
-}
-
-// Where a CTA is in its share.
+// Where a CTA is in its share: the place in a unit, LEAD before its first tile.
 struct Walk {
-  int r, unit, tile, left;
+  int r, unit, place, left;
 };
 struct Share {
   Walk w;
-  long long from, total;   // the share's first tile among all; all tiles
+  uint32_t from, total, each, wide;   // the share's first place among all; all of them: `wide` shares of each + 1, then shares of `each`
 };
-
-// `total` tiles in `shares` equal parts (the first of them one tile larger where they do not come out even).
-__device__ __forceinline__ long long divide(long long x, long long by) {
-  return (unsigned long long)(x | by) >> 32 ? x / by : (long long)((uint32_t)x / (uint32_t)by);      // a 64-bit division takes several times as long
-}
-__device__ __forceinline__ long long share_from(long long total, int shares, long long share) {
-  const long long each = divide(total, shares);
-  return each * share + min(share, total - each * shares);
-}
-__device__ __forceinline__ int share_of(long long total, int shares, long long tile) {
-  const long long each = divide(total, shares), wide = total - each * shares, edge = wide * (each + 1);
-  return (int)(tile < edge ? divide(tile, each + 1) : wide + divide(tile - edge, each));
+__device__ __forceinline__ uint32_t share_from(const Share& s, uint32_t share) { return s.each * share + min(share, s.wide); }
+__device__ __forceinline__ int share_of(const Share& s, uint32_t place) {
+  const uint32_t edge = s.wide * (s.each + 1);
+  return (int)(place < edge ? place / (s.each + 1) : s.wide + (place - edge) / s.each);
 }
 
 // By a whole warp: the start of share `cta` of `ctas`.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Share share_start(const TreeArgs& a, int cta, int ctas) {
+template <typename C>
+__device__ __forceinline__ Share share_start(const TreeArgs& a, uint32_t cta, uint32_t ctas) {
   const int lane = threadIdx.x & 31;
-  const long long total = count_tiles<ROWS, KEYS>(a);
-  ctas = (int)min((long long)ctas, total);               // no empty share between two of one unit
-  const long long from = cta < ctas ? share_from(total, ctas, cta) : 0, to = cta < ctas ? share_from(total, ctas, cta + 1) : 0;
-  Share share = {{a.n_requests, 0, 0, (int)(to - from)}, from, total};
-  Walk& w = share.w;
-  long long base = 0;
-  if (to > from) {
-    for (int r0 = 0; r0 < a.n_requests; r0 += 32) {
-      const long long n = tiles_of<ROWS, KEYS>(a, r0 + lane);
-      long long sum = n;
+  Share share = {{a.n_requests, 0, 0, 0}, 0, 0, 0, 0};
+  const uint32_t mine = size_of<C>(a, lane);
+  uint32_t total = mine;
+#pragma unroll 1
+  for (int r = lane + 32; r < a.n_requests; r += 32) total += size_of<C>(a, r);
+  share.total = total = warp_sum32(total);
+  ctas = min(ctas, total);                       // no empty share between two of one unit
+  if (cta >= ctas) return share;
+  share.each = total / ctas;
+  share.wide = total - share.each * ctas;
+  share.from = share_from(share, cta);
+  share.w.left = (int)(share.each + (cta < share.wide ? 1 : 0));
+  uint32_t base = 0;
+#pragma unroll 1
+  for (int r0 = 0; r0 < a.n_requests; r0 += 32) {
+    const uint32_t n = r0 == 0 ? mine : size_of<C>(a, r0 + lane);
+    uint32_t sum = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
-      }
-      const unsigned here = __ballot_sync(0xffffffffu, base + sum > from);
-      if (here) {
-        const int src = __ffs(here) - 1;
-        const long long start = base + __shfl_sync(0xffffffffu, sum - n, src);
-        w.r = r0 + src;
-        int t_first, tiles, units;
-        unit_shape<ROWS, KEYS>(a, load_request(a, w.r), t_first, tiles, units);
-        w.unit = (int)divide(from - start, tiles);
-        w.tile = (int)(from - start - (long long)w.unit * tiles);
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
     }
+    const unsigned here = __ballot_sync(0xffffffffu, base + sum > share.from);
+    if (here) {
+      const int src = __ffs(here) - 1;
+      const uint32_t in = share.from - base - __shfl_sync(0xffffffffu, sum - n, src);
+      share.w.r = r0 + src;
+      int t_first, tiles, units;
+      unit_shape<C>(a, load_request(a, share.w.r), t_first, tiles, units);
+      share.w.unit = (int)(in < (uint32_t)(tiles + C::LEAD) ? 0 : in / (uint32_t)(tiles + C::LEAD));
+      share.w.place = (int)in - share.w.unit * (tiles + C::LEAD);
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
   }
   return share;
 }
@@ -216,30 +218,35 @@ struct Segment {
   bool whole, begins;      // all of the unit's tiles; its first among them
 };
 
-template <int ROWS, int KEYS>
+template <typename C>
 __device__ __forceinline__ bool next_segment(const TreeArgs& a, Walk& w, Segment& s) {
-  if (w.left <= 0) return false;
   int t_first, tiles, units;
-  for (;; ++w.r, w.unit = 0, w.tile = 0) {
-    if (w.r >= a.n_requests) return false;
+#pragma unroll 1
+  while (w.left > 0 && w.r < a.n_requests) {
     s.q = load_request(a, w.r);
-    unit_shape<ROWS, KEYS>(a, s.q, t_first, tiles, units);
-    if (w.unit < units) break;
+    unit_shape<C>(a, s.q, t_first, tiles, units);
+    if (w.unit >= units) {
+      ++w.r;
+      w.unit = w.place = 0;
+      continue;
+    }
+    const int at = w.unit < a.G ? 0 : w.unit / a.G, begin = max(w.place - C::LEAD, 0), take = min(tiles + C::LEAD - w.place, w.left);
+    s.g = w.unit - at * a.G;
+    s.row0 = at * C::ROWS;
+    s.rows = min(C::ROWS, s.q.count * a.group - s.row0);
+    s.t0 = t_first + begin;
+    s.n = w.place + take - C::LEAD - begin;
+    s.whole = s.n == tiles;
+    s.begins = begin == 0;
+    w.left -= take;
+    w.place += take;
+    if (w.place == tiles + C::LEAD) {
+      w.place = 0;
+      ++w.unit;
+    }
+    if (s.n > 0) return true;
   }
-  s.g = w.unit % a.G;
-  s.row0 = w.unit / a.G * ROWS;
-  s.rows = min(ROWS, s.q.count * (a.H / a.G) - s.row0);
-  s.t0 = t_first + w.tile;
-  s.n = min(tiles - w.tile, w.left);
-  s.whole = s.n == tiles;
-  s.begins = w.tile == 0;
-  w.left -= s.n;
-  w.tile += s.n;
-  if (w.tile == tiles) {
-    w.tile = 0;
-    ++w.unit;
-  }
-  return true;
+  return false;
 }
 
 // Where a segment's partial result goes: a share's first segment may begin inside a unit (2 cta), its last may end inside the unit
@@ -261,42 +268,60 @@ __device__ __forceinline__ float* part_place(const TreeArgs& a, size_t slot, int
 // the first inside its unit, 32 of the unit's rows and 32 dims: a thread a row and eight dims.  It starts beside the kernel that leaves
 // the parts (which lets it only behind its own wait, so what that one reads is there) and waits with its unit found.
 constexpr int CW = 4;
-template <typename T, int HD, int ROWS, int KEYS>
+template <typename T, int HD, typename C>
 __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a, int ctas) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
-  const Share share = share_start<ROWS, KEYS>(a, c, ctas);
+  const Share share = share_start<C>(a, c, ctas);
   const Walk w = share.w;
-  if (w.left <= 0 || w.tile == 0) return;
-  ctas = (int)min((long long)ctas, share.total);
-  const long long start = share.from - w.tile;
-  if (share_from(share.total, ctas, c - 1) > start) return;
-  const TreeReq q = load_request(a, w.r);
-  int t_first, tiles, units;
-  unit_shape<ROWS, KEYS>(a, q, t_first, tiles, units);
-  const int parts = share_of(share.total, ctas, start + tiles - 1) - c + 2;        // shares c - 1, c, ...
-  const int group = a.H / a.G, g = w.unit % a.G, row0 = w.unit / a.G * ROWS, rows = min(ROWS, q.count * group - row0);
+  const uint32_t first = share.from - w.place + C::LEAD;                // the place of the unit's first tile
   const int row = blockIdx.y * 32 + lane, dim = blockIdx.z * 32 + warp * 8;
-  if (row >= rows) return;
-  const int token = (row0 + row) / group, head = g * group + (row0 + row) % group;
+  int t_first = 0, tiles = 0, units = 0, row0 = 0, rows = 0, g = 0;
+  TreeReq q = {0, 0, 0, 0};
+  if (w.left > 0 && w.place > C::LEAD && share_from(share, c - 1) <= first) {
+    q = load_request(a, w.r);
+    unit_shape<C>(a, q, t_first, tiles, units);
+    const int at = w.unit < a.G ? 0 : w.unit / a.G;
+    g = w.unit - at * a.G;
+    row0 = at * C::ROWS;
+    rows = min(C::ROWS, q.count * a.group - row0);
+  }
+  // (the first block waits in any case: this kernel must not be through before the one that it waits for)
+  if (row >= rows && blockIdx.x + blockIdx.y + blockIdx.z > 0) return;
+  const int parts = rows > 0 ? share_of(share, first + tiles - 1) - c + 2 : 0;        // shares c - 1, c, ...
+  const int token = token_of(a, row0 + row), head = g * a.group + row0 + row - token * a.group;
   pdl_wait();
-  auto slot = [&](int p) { return part_slot(c - 1 + p, p == 0); };
-  auto part = [&](int p) { return __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot(p) * a.rows_cap + row); };
-  float m = -CUDART_INF_F;
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, part(p).x);
-  const float safe = m == -CUDART_INF_F ? 0.f : m;
-  float l = 0.f, acc[8];
+  if (row >= rows) return;
+  constexpr int DEEP = 8;                // parts on their way at once
+  float m = -CUDART_INF_F, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = part(p);
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot(p), row, dim, HD)));
-    const float4 y = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot(p), row, dim + 4, HD)));
-    const float f = power<T>(ml.x - safe);
-    l = fmaf(ml.y, f, l);
-    acc[0] = fmaf(x.x, f, acc[0]), acc[1] = fmaf(x.y, f, acc[1]), acc[2] = fmaf(x.z, f, acc[2]), acc[3] = fmaf(x.w, f, acc[3]);
-    acc[4] = fmaf(y.x, f, acc[4]), acc[5] = fmaf(y.y, f, acc[5]), acc[6] = fmaf(y.z, f, acc[6]), acc[7] = fmaf(y.w, f, acc[7]);
+  for (int p0 = 0; p0 < parts; p0 += DEEP) {
+    float2 ml[DEEP];
+    float4 u[DEEP], v[DEEP];
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      const int p = min(p0 + i, parts - 1);
+      const size_t slot = part_slot(c - 1 + p, p == 0);
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot * a.rows_cap + row);
+      u[i] = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot, row, dim, HD)));
+      v[i] = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot, row, dim + 4, HD)));
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) mn = fmaxf(mn, ml[i].x);
+    const float safe = mn == -CUDART_INF_F ? 0.f : mn, old = power<T>(m - safe);
+    l *= old;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= old;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      if (p0 + i >= parts) break;
+      const float f = power<T>(ml[i].x - safe);
+      l = fmaf(ml[i].y, f, l);
+      acc[0] = fmaf(u[i].x, f, acc[0]), acc[1] = fmaf(u[i].y, f, acc[1]), acc[2] = fmaf(u[i].z, f, acc[2]), acc[3] = fmaf(u[i].w, f, acc[3]);
+      acc[4] = fmaf(v[i].x, f, acc[4]), acc[5] = fmaf(v[i].y, f, acc[5]), acc[6] = fmaf(v[i].z, f, acc[6]), acc[7] = fmaf(v[i].w, f, acc[7]);
+    }
   }
   float factor = 1.0f;
   if (a.sink) {
@@ -320,10 +345,17 @@ __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a,
   }
 }
 
-template <typename T, int HD, int ROWS, int KEYS>
+// Whether all places fit 32 bits.
+template <typename C>
+bool cut_fits(const TreeArgs& a) {
+  const unsigned long long units = ((unsigned long long)a.most_tokens * a.group + C::ROWS - 1) / C::ROWS * a.G;
+  return units * a.n_requests < (1ull << 31) / ((unsigned long long)a.most_keys / C::KEYS + 2 + C::LEAD);
+}
+
+template <typename T, int HD, typename C>
 int launch_combine(const TreeArgs& a, int ctas, cudaStream_t s) {
   if (ctas < 2) return 0;
-  return hk_launch_pdl(tree_combine_kernel<T, HD, ROWS, KEYS>, dim3((unsigned)(ctas - 1), (unsigned)((a.rows_cap + 31) / 32), HD / 32), dim3(CW * 32), 0, s,
+  return hk_launch_pdl(tree_combine_kernel<T, HD, C>, dim3((unsigned)(ctas - 1), (unsigned)((a.rows_cap + 31) / 32), HD / 32), dim3(CW * 32), 0, s,
                        a, ctas);
 }
 
@@ -339,7 +371,7 @@ __global__ void __launch_bounds__(GW * 32) tree_generic_kernel(const TreeArgs a)
   const TreeReq q = load_request(a, r);
   if (token >= q.count) return;
   const TreeRow w = tree_row(a, q, token, true);
-  const int g = head / (a.H / a.G), hd = a.hd;
+  const int g = head / a.group, hd = a.hd;
   const int* bt = a.block_table + (size_t)q.slot * a.table_stride;
   const T* qp = reinterpret_cast<const T*>(a.q) + ((size_t)(q.first + token) * a.H + head) * hd;
   float qr[8], acc[8];
@@ -428,6 +460,7 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 // tiles later, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
 // threads need not meet over it.  Where one tile jumps by more than 2^60 the row's sum is set to NaN, and the row is taken again (below).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 128;
+typedef Cut<2 * TC_ROWS, TC_KEYS, 4> TcCut;
 constexpr float MUCH = 16777216.0f, TOO_MUCH = 1152921504606846976.0f;      // 2^24, 2^60
 constexpr long long WAIT_CLOCKS = 1ll << 25;   // some 17 ms, far beyond any legitimate wait
 
@@ -570,7 +603,9 @@ struct TcSmem {
   float first[2][2][2][TC_ROWS], asked[4][2][2][TC_ROWS];   // [tile % 2][group][half of the keys][row]: a first tile's largest score;
                                                             // [tile % 4]..: the reference asked for
   float2 ml[2][2][TC_ROWS];   // the reference and the sum
-  Walk start;
+  Walk start;                 // the share behind its first segment
+  Segment segment;
+  int any;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -586,7 +621,7 @@ struct RowKeys {
   int j, end;
 };
 __device__ __forceinline__ RowKeys row_keys(const TreeArgs& a, const Segment& s, int row) {
-  const int group = a.H / a.G, token = (s.row0 + row) / group, head = s.g * group + (s.row0 + row) % group;
+  const int token = token_of(a, s.row0 + row), head = s.g * a.group + s.row0 + row - token * a.group;
   RowKeys k;
   k.w = tree_row(a, s.q, token, true);
   k.q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * a.hd;
@@ -639,7 +674,8 @@ __device__ __noinline__ float tree_row_again(const TreeArgs& a, const Segment& s
   return acc;
 }
 
-template <int HD>
+// CAP: with a soft cap on the scores (an instance of its own: its code would be in the way of every call)
+template <int HD, bool CAP>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeArgs a, float cap_log2, float cap_in2) {
   constexpr int STAGES = TcSmem<HD>::STAGES, CPR = HD / 8, KSTEPS = HD / 16, HALVES = HD / 64;
@@ -652,7 +688,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   TcSmem<HD>& sm = *reinterpret_cast<TcSmem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   volatile int* abort_flag = &sm.abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
     mbar_init(&sm.q_full, TC_SOFTMAX / 32);
@@ -681,20 +717,27 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   pdl_wait();
   pdl_launch_dependents();
   if (warp == 0) {
-    const Share share = share_start<2 * TC_ROWS, TC_KEYS>(a, blockIdx.x, gridDim.x);
-    if (lane == 0) sm.start = share.w;
+    Walk w = share_start<TcCut>(a, blockIdx.x, gridDim.x).w;
+    Segment s;
+    const bool any = next_segment<TcCut>(a, w, s);
+    if (lane == 0) {
+      sm.start = w;
+      sm.segment = s;
+      sm.any = any;
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   Walk w = sm.start;
-  Segment s;
+  Segment s = sm.segment;
+  bool more = sm.any != 0;
 
   if (warp >= LOAD_WARP) {
     // ================================================================= loads (a lane per box of a page's keys and half of the head)
-    const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows;
-    const int box = lane & (boxes - 1), h = lane / boxes;      // boxes: a power of two up to 16
+    const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS, boxes = TC_KEYS / box_rows, per_page = a.page_tokens <= TC_KEYS ? 1 : a.page_tokens / TC_KEYS;
+    const int box_shift = __ffs(box_rows) - 1, box = lane & (boxes - 1), h = lane >> (__ffs(boxes) - 1);      // powers of two, boxes up to 16
     // A warp for K and one for V: a stream's next scores want K tiles before the V tiles are free that one warp would have to send for first.
     const bool is_v = warp != LOAD_WARP;
     uint64_t *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
@@ -702,26 +745,27 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const CUtensorMap* map = is_v ? &map_v : &map_k;
     int n = 0;                    // tiles sent for so far
     bool alive = true;
-    while (alive && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+    for (; alive && more; more = next_segment<TcCut>(a, w, s)) {
       const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
-      const int first = first_key(a, s.q) / box_rows, last = (s.q.context + s.q.count - 1) / box_rows;
+      const int first = first_key(a, s.q) >> box_shift, last = (s.q.context + s.q.count - 1) >> box_shift;
       // Box b of the request: its page, and from that its first row of the pages, seen as one matrix.  A box that holds no key of the
       // request is the one of its nearest key, so that nothing but cache rows ever lies in a stage: an old NaN pattern there would not
       // be kept out of the sums by a probability of zero.
-      auto key_of = [&](int b) { return min(max(b, first), last) * box_rows; };
+      auto box_of = [&](int b) { return min(max(b, first), last); };
+      auto page_of = [&](int b) { return bt[per_page == 1 ? box_of(b) : box_of(b) / per_page]; };
       auto row_of = [&](int b, int page) {
-        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + key_of(b) % a.page_tokens : 0;
+        return page >= 0 && page < a.num_pages ? (page * a.G + s.g) * a.page_tokens + (per_page == 1 ? 0 : box_of(b) % per_page * box_rows) : 0;
       };
       // 32 boxes at a time, a lane each; the next 32 are on their way meanwhile
       int at = s.t0 * boxes + lane;
-      int row = row_of(at, bt[key_of(at) / a.page_tokens]);
-      int page = bt[key_of(at + 32) / a.page_tokens];
+      int row = row_of(at, page_of(at));
+      int page = page_of(at + 32);
       int sent = 0;
       for (int i = 0; i < s.n && alive; ++i, ++n) {
         if (sent == 32) {
           at += 32;
           row = row_of(at, page);
-          page = bt[key_of(at + 32) / a.page_tokens];
+          page = page_of(at + 32);
           sent = 0;
         }
         const int mine = __shfl_sync(0xffffffffu, row, sent + box), st = n % STAGES;
@@ -748,7 +792,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       const uint32_t sp = tmem + x * SP_COL[1], oc = tmem + O_COL[0] + x * HD;
       const uint64_t dq0 = desc_k_major(smem_u32(sm.q[0])), dk0 = desc_k_major(smem_u32(sm.k[0])), dv0 = desc_mn_major(smem_u32(sm.v[0]), TC_KEYS * 128);
       constexpr uint32_t STAGE16 = TC_KEYS * HD * 2 >> 4, HALF16 = TC_KEYS / 2 * 128 >> 4;      // descriptors count in 16 bytes
-      while (ok && next_segment<2 * TC_ROWS, TC_KEYS>(a, w, s)) {
+      for (; ok && more; more = ok && next_segment<TcCut>(a, w, s)) {
         const bool two = s.rows > TC_ROWS;
         const int jobs = two ? s.n : (s.n + 1 - (int)x) / 2;
         if (!mbar_wait(&sm.q_full, seg & 1u, abort_flag)) { ok = false; break; }
@@ -813,30 +857,29 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     constexpr int HK = TC_KEYS / 2, EC = 16;        // keys a thread; dims of the sums that a thread finishes at once
     const float scale_log2 = a.scale * 1.4426950408889634f;
-    const float sl = cap_log2 > 0.f ? 1.0f : scale_log2;       // capped scores are in the exponent's domain already
+    const float sl = CAP ? 1.0f : scale_log2;       // capped scores are in the exponent's domain already
     const uint32_t sp = lane_addr + (x ? SP_COL[1] : SP_COL[0]), oc = lane_addr + (x ? O_COL[1] : O_COL[0]);
     uint32_t jobs_done = 0, met = 0, o_done[2] = {0, 0};
     bool ok = true;
     // Q: the threads of a row share it out; rows past the unit are zeros
     auto send_q = [&](const Segment& u) {
       const bool two = u.rows > TC_ROWS;
-      const int row = two ? x * TC_ROWS + r : r, i = u.row0 + (row < u.rows ? row : 0);
-      const bf16* src = reinterpret_cast<const bf16*>(a.q) + ((size_t)(u.q.first + i / group) * a.H + u.g * group + i % group) * HD;
+      const int row = two ? x * TC_ROWS + r : r, i = u.row0 + (row < u.rows ? row : 0), token = token_of(a, i);
+      const bf16* src = reinterpret_cast<const bf16*>(a.q) + ((size_t)(u.q.first + token) * a.H + u.g * a.group + i - token * a.group) * HD;
       const uint32_t qs = smem_u32(sm.q[two ? x : 0]);
       const int c_from = two ? half * (CPR / 2) : (2 * x + half) * (CPR / 4), c_to = c_from + (two ? CPR / 2 : CPR / 4);
 #pragma unroll 4
       for (int c = c_from; c < c_to; ++c) cp_async16(qs + swz(r, c), src + c * 8, row < u.rows);
       cp_async_commit();
     };
-    Segment ahead;
-    bool more = next_segment<2 * TC_ROWS, TC_KEYS>(a, w, ahead);
+    Segment ahead = s;
     if (more) send_q(ahead);
     while (ok && more) {
       s = ahead;
       const bool two = s.rows > TC_ROWS;
       const int row = two ? x * TC_ROWS + r : r;
       const bool valid = row < s.rows, busy = row - lane < s.rows;        // busy: any row of the warp is one
-      const int token = valid ? (s.row0 + row) / group : 0;
+      const int token = valid ? token_of(a, s.row0 + row) : 0;
       const int lo = valid ? tree_row(a, s.q, token, true).lo : 0;
       cp_async_wait<0>();
       fence_async_proxy();
@@ -863,7 +906,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         auto load = [&](int c) {
           tmem_ld32(sp + (uint32_t)(half * HK + 32 * c), su);
           tmem_ld_wait();
-          if (cap_log2 > 0.f) {
+          if (CAP) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) su[i] = __float_as_uint(log2_score(__uint_as_float(su[i]), 1.0f, cap_log2, cap_in2));
           }
@@ -878,8 +921,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             load(c);
+            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(su[i]));
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(su[i]));
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
           sm.first[n & 1][x][half][r] = top * sl;
           __syncwarp();
@@ -919,8 +964,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           }
         }
         const float shift = m == -CUDART_INF_F ? 0.f : -m, l_before = l0 + l1;
-        // a half's P lies in the columns of its own scores that are read already
-#pragma unroll
+        // a half's P lies in the columns of its own scores that are read already (a loop: a short call waits for its instructions)
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           load(c);
           uint32_t pw[16];
@@ -962,7 +1007,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       ok = !softmax_any(!ok);
       if (!ok) break;
       tc_fence_after();
-      more = next_segment<2 * TC_ROWS, TC_KEYS>(a, w, ahead);
+      more = next_segment<TcCut>(a, w, ahead);
       if (more) send_q(ahead);                         // both groups' scores are through: Q is free
       if (busy) {
         float f[2] = {1.0f, 1.0f}, l;
@@ -976,7 +1021,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           f[1] = exp2f(v.x - safe);
           l = (u.y + sm.ml[0][1][r].y) * f[0] + (v.y + sm.ml[1][1][r].y) * f[1];
         }
-        const int head = s.g * group + (s.row0 + (valid ? row : 0)) % group;
+        const int head = s.g * a.group + (valid ? s.row0 + row - token * a.group : 0);
         const size_t slot = part_slot(blockIdx.x, s.begins);
         // one over a row's denominator, the sink's term in it
         auto finish = [&](float top, float sum, int of_head) {
@@ -1095,16 +1140,20 @@ int launch_tc(const TreeArgs& a, int ctas, cudaStream_t s) {
   if (!((pt % 8 == 0 && TC_KEYS % pt == 0) || pt % TC_KEYS == 0) || a.status == nullptr) return HK_ERR_UNSUPPORTED;
   if ((((uintptr_t)a.k | (uintptr_t)a.v) & 127) != 0) return HK_ERR_UNSUPPORTED;
   const unsigned long long rows = (unsigned long long)a.num_pages * a.G * pt;
-  if (rows > 0x7fffffffull || a.rows_cap < (a.most_tokens * (a.H / a.G) < 2 * TC_ROWS ? a.most_tokens * (a.H / a.G) : 2 * TC_ROWS)) return HK_ERR_UNSUPPORTED;
+  if (rows > 0x7fffffffull || a.rows_cap < (a.most_tokens * a.group < 2 * TC_ROWS ? a.most_tokens * a.group : 2 * TC_ROWS)) return HK_ERR_UNSUPPORTED;
   CUtensorMap mk, mv;
   const int box_rows = pt < TC_KEYS ? pt : TC_KEYS;
   if (!make_page_map(&mk, a.k, rows, HD, box_rows) || !make_page_map(&mv, a.v, rows, HD, box_rows)) return HK_ERR_UNSUPPORTED;
   const size_t smem = sizeof(TcSmem<HD>) + 1024;
-  if (int e = hk_allow_smem<tree_tc_kernel<HD>>(smem)) return e;
+  if (!cut_fits<TcCut>(a)) return HK_ERR_UNSUPPORTED;
   // a soft cap c in the base-2 domain: C = c log2(e), and 2 log2(e) scale / c, which takes a raw product to 2 z log2(e), z = score / c
   const float cap_log2 = a.softcap > 0.f ? a.softcap * 1.4426950408889634f : 0.f, cap_in2 = a.softcap > 0.f ? 2.8853900817779268f * a.scale / a.softcap : 0.f;
-  if (int e = hk_launch_pdl(tree_tc_kernel<HD>, dim3((unsigned)ctas), dim3(TC_THREADS), smem, s, mk, mv, a, cap_log2, cap_in2)) return e;
-  return launch_combine<bf16, HD, 2 * TC_ROWS, TC_KEYS>(a, ctas, s);
+  const dim3 grid((unsigned)ctas), block(TC_THREADS);
+  int e = a.softcap > 0.f ? hk_allow_smem<tree_tc_kernel<HD, true>>(smem) : hk_allow_smem<tree_tc_kernel<HD, false>>(smem);
+  if (!e) e = a.softcap > 0.f ? hk_launch_pdl(tree_tc_kernel<HD, true>, grid, block, smem, s, mk, mv, a, cap_log2, cap_in2)
+                              : hk_launch_pdl(tree_tc_kernel<HD, false>, grid, block, smem, s, mk, mv, a, cap_log2, cap_in2);
+  if (e) return e;
+  return launch_combine<bf16, HD, TcCut>(a, ctas, s);
 }
 
 // ---- float32 ------------------------------------------------------------------------------------------------------------------
@@ -1112,6 +1161,7 @@ int launch_tc(const TreeArgs& a, int ctas, cudaStream_t s) {
 // 16-byte loads (4 x 4 scores a thread along the head's dims, 4 rows x HD / 16 dims of sums).  The next tile's keys arrive while this
 // one's probabilities are made, the next values while the next scores are.
 constexpr int F32_ROWS = 32, F32_KEYS = 64, F32_THREADS = 128, F32_LDP = F32_KEYS + 4;
+typedef Cut<F32_ROWS, F32_KEYS, 1> F32Cut;
 
 template <int HD>
 struct F32Smem {
@@ -1128,18 +1178,18 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
   constexpr int LD = F32Smem<HD>::LD, C4 = HD / 4, B = HD / 64, RI = F32_ROWS / 8;
   extern __shared__ __align__(16) uint8_t f32_raw[];
   F32Smem<HD>& sm = *reinterpret_cast<F32Smem<HD>*>(f32_raw);
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.H / a.G;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.group;
   const float* qp = reinterpret_cast<const float*>(a.q);
   pdl_wait();
   pdl_launch_dependents();
   if (tid < 32) {
-    const Share share = share_start<F32_ROWS, F32_KEYS>(a, blockIdx.x, gridDim.x);
-    if (tid == 0) sm.start = share.w;
+    const Walk w = share_start<F32Cut>(a, blockIdx.x, gridDim.x).w;
+    if (tid == 0) sm.start = w;
   }
   __syncthreads();
   Walk w = sm.start;
   Segment s;
-  while (next_segment<F32_ROWS, F32_KEYS>(a, w, s)) {
+  while (next_segment<F32Cut>(a, w, s)) {
     const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
     const int end = s.q.context + s.q.count;
     // a tile's keys or values, what does not exist as zeros
@@ -1159,11 +1209,12 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
     for (int e = tid; e < F32_ROWS * C4; e += F32_THREADS) {
       const int r = e / C4, d = e % C4 * 4, i = s.row0 + r;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < s.rows) x = *reinterpret_cast<const float4*>(qp + ((size_t)(s.q.first + i / group) * a.H + s.g * group + i % group) * HD + d);
+      const int token = token_of(a, i);
+      if (r < s.rows) x = *reinterpret_cast<const float4*>(qp + ((size_t)(s.q.first + token) * a.H + s.g * group + i - token * group) * HD + d);
       *reinterpret_cast<float4*>(sm.q + r * LD + d) = make_float4(x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale);
     }
     const float cap = a.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
-    const TreeRow tr = tree_row(a, s.q, (s.row0 + (tid >> 1)) / group, tid < 2 * F32_ROWS && (tid >> 1) < s.rows);     // of row tid / 2
+    const TreeRow tr = tree_row(a, s.q, token_of(a, s.row0 + (tid >> 1)), tid < 2 * F32_ROWS && (tid >> 1) < s.rows);     // of row tid / 2
     // the softmax's state of row tid / 4, alike in its four threads
     const int sr = tid >> 2, sc = (tid & 3) * 16;
     float m = -CUDART_INF_F, l = 0.f;
@@ -1301,7 +1352,7 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
       float inv = 1.0f, total = l;
       if (s.whole) {
         if (a.sink && sr < s.rows) {
-          const float score = a.sinks ? a.sinks[s.g * group + (s.row0 + sr) % group] : 0.f, top = fmaxf(m, score);
+          const float score = a.sinks ? a.sinks[s.g * group + s.row0 + sr - token_of(a, s.row0 + sr) * group] : 0.f, top = fmaxf(m, score);
           inv = m == -CUDART_INF_F ? 0.f : expf(m - top);
           total = l * inv + expf(score - top);
         }
@@ -1317,7 +1368,8 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
       if (r >= s.rows) continue;
       const float inv = sm.inv[r];
       const size_t slot = part_slot(blockIdx.x, s.begins);
-      float* out = reinterpret_cast<float*>(a.out) + ((size_t)(s.q.first + at / group) * a.H + s.g * group + at % group) * HD;
+      const int token = token_of(a, at);
+      float* out = reinterpret_cast<float*>(a.out) + ((size_t)(s.q.first + token) * a.H + s.g * group + at - token * group) * HD;
 #pragma unroll
       for (int b = 0; b < B; ++b)
         *reinterpret_cast<float4*>(s.whole ? out + 64 * b + 4 * tx : part_place(a, slot, r, 64 * b + 4 * tx, HD)) =
@@ -1330,10 +1382,11 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
 
 template <int HD>
 int launch_f32(const TreeArgs& a, int ctas, cudaStream_t s) {
-  if (a.rows_cap < (a.most_tokens * (a.H / a.G) < F32_ROWS ? a.most_tokens * (a.H / a.G) : F32_ROWS)) return HK_ERR_UNSUPPORTED;
+  if (a.rows_cap < (a.most_tokens * a.group < F32_ROWS ? a.most_tokens * a.group : F32_ROWS)) return HK_ERR_UNSUPPORTED;
+  if (!cut_fits<F32Cut>(a)) return HK_ERR_UNSUPPORTED;
   if (int e = hk_allow_smem<tree_f32_kernel<HD>>(sizeof(F32Smem<HD>))) return e;
   if (int e = hk_launch_pdl(tree_f32_kernel<HD>, dim3((unsigned)ctas), dim3(F32_THREADS), sizeof(F32Smem<HD>), s, a)) return e;
-  return launch_combine<float, HD, F32_ROWS, F32_KEYS>(a, ctas, s);
+  return launch_combine<float, HD, F32Cut>(a, ctas, s);
 }
 
 }  // namespace
@@ -1343,16 +1396,18 @@ int launch_f32(const TreeArgs& a, int ctas, cudaStream_t s) {
 // of a token's row: it sees the drafted token j of its request; positions int32 [n] (read with a window only): drafted tokens stand
 // at their request's `context` or behind it.  Only rows of q that belong to a request are computed.  scale on q . k, softcap c (0:
 // none), window w (0: none): a key at position x is seen from position p if x > p - w; sink, sinks: one more term of the
-// denominator.  most_tokens, n_requests: bounds of the grid.  `kernel` 0: any size up to heads of 256.  `kernel` 1: heads of 64 and
+// denominator.  most_tokens, most_keys: a request with more drafted
+// tokens, or more rows with them, is left out.  `kernel` 0: any size up to heads of 256.  `kernel` 1: heads of 64 and
 // 128, in bfloat16 on the tensor cores (cache pages that are whole boxes of a 128-key tile: multiples of 8 that divide 128, and
 // multiples of 128), in float32 with multiply-adds; `ctas` shares, part_o float [2 ctas, hd / 4, rows_cap, 4] and part_ml [2 ctas,
 // rows_cap, 2] for what they leave, rows_cap at least the rows of a tile (256, in float32 32; or most_tokens * H / G where that is less); `status` is set to 4 if a bounded wait ran out.
 HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int* block_table, int table_rows,
-                             int table_stride, const int* requests, int n_requests, int most_tokens, const void* ancestors, int words,
+                             int table_stride, const int* requests, int n_requests, int most_tokens, int most_keys, const void* ancestors, int words,
                              const int* positions, int n, long long num_pages, int page_tokens, int H, int G, int hd, int window,
                              float scale, float softcap, int sink, const float* sinks, int kernel, int ctas, float* part_o,
                              float* part_ml, int rows_cap, int* status, void* stream) {
   if (n <= 0 || n_requests <= 0 || most_tokens <= 0) return 0;
+  if (most_keys < 1 || most_keys > (long long)table_stride * page_tokens || most_tokens > 256) return HK_ERR_UNSUPPORTED;
   if (H < 1 || G < 1 || H % G != 0 || hd < 1 || hd > 256 || page_tokens < 1 || table_rows < 1 || table_stride < 1 || words < 1 ||
       n_requests > 65535 || num_pages < 1 || softcap < 0.f || !(scale > 0.f) || (dtype != HK_F32 && dtype != HK_BF16) ||
       (((uintptr_t)requests) & 15) != 0)
@@ -1366,10 +1421,12 @@ HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* 
   a.sinks = sink ? sinks : nullptr;
   a.part_o = part_o; a.part_ml = part_ml; a.status = status;
   a.num_pages = num_pages;
-  a.n = n; a.n_requests = n_requests; a.most_tokens = most_tokens; a.words = words;
+  a.n = n; a.n_requests = n_requests; a.most_tokens = most_tokens; a.most_keys = most_keys; a.words = words;
   a.table_rows = table_rows; a.table_stride = table_stride; a.page_tokens = page_tokens;
   a.H = H; a.G = G; a.hd = hd; a.window = window > 0 ? window : 0; a.sink = sink; a.rows_cap = rows_cap;
   a.scale = scale; a.softcap = softcap;
+  a.group = H / G;
+  a.group_inverse = a.group == 1 ? 0u : (uint32_t)((0x100000000ull + a.group - 1) / a.group);
   cudaStream_t s = (cudaStream_t)stream;
   if (kernel == 0) return dtype == HK_F32 ? launch_generic<float>(a, s) : launch_generic<bf16>(a, s);
   if (kernel != 1 || ctas < 1 || part_o == nullptr || part_ml == nullptr) return HK_ERR_UNSUPPORTED;

@@ -1527,7 +1527,7 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
     32 of word j / 32: drafted token j of its request; for a tree its ancestors and itself); with `window` w only those at positions
     above its own less w, where a cached row's position is its place and a drafted token's is in `positions` int32 [n] (not below the
     request's cached rows).  A token that sees nothing gives zeros; rows of no request keep what they hold.  sink, sinks, softcap
-    as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them;
+    as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them: one beyond them is left out;
     all_keys: the rows of all requests together, where the caller knows it (0: as if all had the most)."""
     _need(q, "q", dims=2)
     _need(out, "out", q.dtype, 2)
@@ -1575,13 +1575,14 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
             if window > 0:
                 held = min(held, m * (window + most_tokens))
             tiles = -(-most_tokens * group // rows) * G * (held // keys + m)
-            ctas = max(1, min(gemm_fast._sms(q.device) * (2 if wide else 1), tiles))
+            # two tiles a share at least: one for either group of warps
+            ctas = max(1, min(gemm_fast._sms(q.device) * (2 if wide else 1), (tiles + 1) // 2))
             cap = min(rows, most_tokens * group)
             part_o = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
             part_ml = part_o.data_ptr() + 8 * ctas * cap * hd
             kernel, status = 1, 0 if wide else _ptr(gemm_fast.status_flag(q.device))
         args = (_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _dt(q), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(requests),
-                m, most_tokens, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
+                m, most_tokens, most_keys, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
                 scale, softcap, 1 if sink else 0, _ptr(sinks))
         if kernel:
             code = lib.hk_tree_attention(*args, kernel, ctas, _ptr(part_o), part_ml, cap, status, _stream())
