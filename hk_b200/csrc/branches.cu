@@ -60,69 +60,86 @@ struct RowArray {
   const int* block_table;
 };
 
-constexpr int KEEP_THREADS = 128, KEEP_DEEP = 8, KEEP_PATH = 256;
+constexpr int KEEP_THREADS = 256, KEEP_DEEP = 8, KEEP_PATH = 256;
 
-// A thread takes a column (array, request, head, 16 bytes of a row) and moves its rows in order: a path climbs, so a row that is
-// written (path[i] -> i, i <= path[i]) is none that a later step of the path reads.
+// A thread takes a column (head, 16 bytes of a row) of an array and moves its rows in order: a path climbs, so a row that is written
+// (path[i] -> i, i <= path[i]) is none that a later step of the path reads.  `from`, `to`: page, place in the page.
 template <typename V>
-__device__ __forceinline__ void move_rows(const RowArray& a, const long long* from, const long long* to, int n, long long head_bytes) {
+__device__ __forceinline__ void move_rows(const RowArray& a, const int2* from, const int2* to, int n, int page_tokens, int column) {
   const int per = (int)(a.row / (long long)sizeof(V));
-  for (long long c = (long long)blockIdx.z * KEEP_THREADS + threadIdx.x; c < a.heads * per; c += (long long)gridDim.z * KEEP_THREADS) {
-    uint8_t* base = reinterpret_cast<uint8_t*>(a.address) + (c / per) * head_bytes + (c % per) * (long long)sizeof(V);
-    for (int i0 = 0; i0 < n; i0 += KEEP_DEEP) {
-      V v[KEEP_DEEP];
+  const long long head_bytes = page_tokens * a.row, page_bytes = a.heads * head_bytes;
+  uint8_t* base = reinterpret_cast<uint8_t*>(a.address) + (column / per) * head_bytes + (column % per) * (long long)sizeof(V);
+  for (int i0 = 0; i0 < n; i0 += KEEP_DEEP) {
+    V v[KEEP_DEEP];
 #pragma unroll
-      for (int k = 0; k < KEEP_DEEP; ++k)
-        if (i0 + k < n) v[k] = *reinterpret_cast<const V*>(base + from[i0 + k]);
+    for (int k = 0; k < KEEP_DEEP; ++k)
+      if (i0 + k < n) v[k] = *reinterpret_cast<const V*>(base + from[i0 + k].x * page_bytes + from[i0 + k].y * a.row);
 #pragma unroll
-      for (int k = 0; k < KEEP_DEEP; ++k)
-        if (i0 + k < n) *reinterpret_cast<V*>(base + to[i0 + k]) = v[k];
-    }
+    for (int k = 0; k < KEEP_DEEP; ++k)
+      if (i0 + k < n) *reinterpret_cast<V*>(base + to[i0 + k].x * page_bytes + to[i0 + k].y * a.row) = v[k];
   }
 }
 
+// A block takes a request and some neighbouring arrays, and finds the pages of its path once for all that share a block table: finding
+// them is a chain of three reads, and as long as moving an array's rows.
 __global__ void __launch_bounds__(KEEP_THREADS)
-compact_rows_kernel(const RowArray* __restrict__ table, const int* __restrict__ paths, int width, int table_rows, int table_stride,
-                    int page_tokens, long long num_pages) {
-  __shared__ long long from[KEEP_PATH], to[KEEP_PATH];
+compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_block, const int* __restrict__ paths, int width, int table_rows,
+                    int table_stride, int page_tokens, long long num_pages) {
+  __shared__ int2 from[KEEP_PATH], to[KEEP_PATH];
   __shared__ int count;
-  const RowArray a = table[blockIdx.y];
   const int* path = paths + (size_t)blockIdx.x * (width + 2);
-  const int slot = path[0], first = path[1];
+  const int slot = path[0], first = path[1], a0 = blockIdx.y * per_block, a1 = min(arrays, a0 + per_block);
   if (slot < 0 || slot >= table_rows || first < 0) return;
-  const long long head_bytes = page_tokens * a.row, page_bytes = a.heads * head_bytes;
-  const int* pages = a.block_table + (size_t)slot * table_stride;
-  auto place = [&](long long row) -> long long {
-    if (row >= (long long)table_stride * page_tokens) return -1;
-    const int page = pages[row / page_tokens];
-    return page < 0 || page >= num_pages ? -1 : page * page_bytes + (row % page_tokens) * a.row;
-  };
   for (int done = 0; done < width; done += KEEP_PATH) {
-    if (threadIdx.x < 32) {            // the rows that move, in order
-      int n = 0;
-      for (int i0 = done; i0 < min(width, done + KEEP_PATH); i0 += 32) {
-        const int i = i0 + (int)threadIdx.x, row = i < width ? path[2 + i] : -1;
-        long long f = -1, t = -1;
-        if (row > i) {
-          f = place((long long)first + row);
-          t = place((long long)first + i);
+    const int* found = nullptr;
+    for (int i = a0; i < a1;) {
+      const int* block_table = table[i].block_table;
+      if (block_table != found) {
+        __syncthreads();
+        if (threadIdx.x < 32) {            // the rows that move, in order
+          const int* pages = block_table + (size_t)slot * table_stride;
+          auto place = [&](long long row) -> int2 {
+            const int at = (int)min(row / page_tokens, (long long)table_stride), page = at < table_stride ? pages[at] : -1;
+            return make_int2(page < 0 || page >= num_pages ? -1 : page, (int)(row - (long long)at * page_tokens));
+          };
+          int n = 0;
+          for (int i0 = done; i0 < min(width, done + KEEP_PATH); i0 += 32) {
+            const int k = i0 + (int)threadIdx.x, row = k < width ? path[2 + k] : -1;
+            int2 f = make_int2(-1, 0), t = f;
+            if (row > k) {
+              f = place((long long)first + row);
+              t = place((long long)first + k);
+            }
+            const bool moves = f.x >= 0 && t.x >= 0;
+            const unsigned all = __ballot_sync(0xffffffffu, moves);
+            if (moves) {
+              const int at = n + __popc(all & ((1u << threadIdx.x) - 1u));
+              from[at] = f;
+              to[at] = t;
+            }
+            n += __popc(all);
+          }
+          if (threadIdx.x == 0) count = n;
         }
-        const bool moves = f >= 0 && t >= 0;
-        const unsigned all = __ballot_sync(0xffffffffu, moves);
-        if (moves) {
-          const int at = n + __popc(all & ((1u << threadIdx.x) - 1u));
-          from[at] = f;
-          to[at] = t;
-        }
-        n += __popc(all);
+        __syncthreads();
+        found = block_table;
       }
-      if (threadIdx.x == 0) count = n;
+      // the arrays of one kind that follow: their columns side by side
+      const RowArray a = table[i];
+      int same = 1;
+      while (i + same < a1 && table[i + same].block_table == found && table[i + same].heads == a.heads && table[i + same].row == a.row) ++same;
+      long long low = 0;
+      for (int k = 0; k < same; ++k) low |= table[i + k].address;
+      const int wide = ((low | a.row) & 15) == 0 ? 16 : ((low | a.row) & 3) == 0 ? 4 : 1, columns = (int)(a.heads * (a.row / wide)), n = count;
+      for (int c = threadIdx.x; c < same * columns; c += KEEP_THREADS) {
+        RowArray b = a;
+        b.address = table[i + c / columns].address;
+        if (wide == 16) move_rows<uint4>(b, from, to, n, page_tokens, c % columns);
+        else if (wide == 4) move_rows<uint32_t>(b, from, to, n, page_tokens, c % columns);
+        else move_rows<uint8_t>(b, from, to, n, page_tokens, c % columns);
+      }
+      i += same;
     }
-    __syncthreads();
-    const int n = count;
-    if (((a.address | a.row) & 15) == 0) move_rows<uint4>(a, from, to, n, head_bytes);
-    else if (((a.address | a.row) & 3) == 0) move_rows<uint32_t>(a, from, to, n, head_bytes);
-    else move_rows<uint8_t>(a, from, to, n, head_bytes);
     __syncthreads();
   }
 }
@@ -132,18 +149,19 @@ compact_rows_kernel(const RowArray* __restrict__ table, const int* __restrict__ 
 // tokens, best first, of equal ones the one with the lower k V + v first.  A logit that is not finite counts as -inf, and so does
 // every continuation of a beam whose own score is not finite.
 //
-// One pass over the logits: a CTA takes a part of a row into registers, sums its exponentials against its own maximum (32 terms a
-// thread in float32, threads and parts in 64 bits) and leaves its best `choices` tokens in order; then a CTA a prompt joins the
-// parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order: two beams' continuations lie as little as 1e-7
-// apart often enough among a million, and which of them comes first must not hang on how a sum was rounded.
+// One pass over the logits: a CTA takes a part of a row through registers, a tile of 4,096 at a time with the next one on its way, and
+// keeps a sum of exponentials against a reference near their maximum (a tile's sixteen a thread in float32, all beyond that in 64 bits) and
+// the tokens that can be among its best `choices`: as many groups of threads hold a value each that reaches the smallest of the groups' maxima, so what is
+// below that bar is out.  A CTA a prompt then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order:
+// two beams' continuations lie as little as 1e-7 apart often enough among a million, and which of them comes first must not hang on how
+// a sum was rounded.
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
 constexpr int BC = 1024;              // candidates that are ranked side by side; more than that only among equal logits
 
 struct RowPart {
   double sum;                         // of exp(x - top)
-  float top;
-  int n;                              // tokens left
+  float top, pad;                     // (top: the part's reference, -inf if it holds nothing finite)
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
@@ -156,13 +174,14 @@ __device__ __forceinline__ bool ahead(F x, int i, F y, int j) {
 
 // `mine`: a thread's largest value.  Among the values of the threads, at least `groups` reach `bar`: each of that many groups of
 // neighbouring threads holds one.  `top`: the largest of all.
-template <typename F>
+template <int T, typename F>
 __device__ __forceinline__ void find_bar(F mine, int groups, F* s_group, F& bar, F& top) {
-  const int size = BT / groups;       // 1 to 32 threads
+  const int size = min(T / groups, 32);       // (a warp is at most one group: more of them than asked for)
   for (int o = 1; o < size; o <<= 1) {
     const F other = __shfl_xor_sync(0xffffffffu, mine, o);
     mine = other > mine ? other : mine;
   }
+  groups = T / size;
   if (threadIdx.x % size == 0) s_group[threadIdx.x / size] = mine;
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -183,7 +202,7 @@ __device__ __forceinline__ void find_bar(F mine, int groups, F* s_group, F& bar,
 }
 
 // The best of all threads' (value, index) that come behind (past, past_index); index -1 if there is none.
-template <typename F>
+template <int T, typename F>
 __device__ __forceinline__ void best_of_block(F& x, int& i, F* s_x, int* s_i) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -200,7 +219,7 @@ __device__ __forceinline__ void best_of_block(F& x, int& i, F* s_x, int* s_i) {
     s_i[threadIdx.x >> 5] = i;
   }
   __syncthreads();
-  for (int w = 0; w < BT / 32; ++w) {
+  for (int w = 0; w < T / 32; ++w) {
     const F y = s_x[w];
     const int j = s_i[w];
     if (j >= 0 && (i < 0 || ahead(y, j, x, i))) {
@@ -210,79 +229,128 @@ __device__ __forceinline__ void best_of_block(F& x, int& i, F* s_x, int* s_i) {
   }
 }
 
-// E: values a thread
-template <int E>
-__global__ void __launch_bounds__(BT)
-beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ scores, int V, int choices, int groups, int parts,
+constexpr int BE = 16;                // values of a tile a thread
+
+// The parts of a row are of `length` values (the last of what is left).
+__global__ void __launch_bounds__(BT, 4)
+beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ scores, int V, int choices, int groups, int parts, int length,
                  RowPart* __restrict__ part, float* __restrict__ part_x, int* __restrict__ part_i) {
-  __shared__ float s_group[BT], s_x[BC];
-  __shared__ int s_i[BC], s_n;
+  __shared__ float s_group[BT], s_x[2][BC];
+  __shared__ int s_i[2][BC], s_n;
   __shared__ double s_sum[BT / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x / parts, p = blockIdx.x % parts;
+  const int tid = threadIdx.x, row = blockIdx.x / parts, p = blockIdx.x % parts;
   const size_t at = (size_t)row * parts + p;
   if (!finite(scores[row])) {
-    if (threadIdx.x == 0) part[at] = RowPart{0.0, -CUDART_INF_F, 0};
+    if (tid == 0) part[at] = RowPart{0.0, -CUDART_INF_F, 0.f};
+    for (int c = tid; c < choices; c += BT) part_x[at * choices + c] = -CUDART_INF_F;
     return;
   }
   const float* x = logits + (size_t)row * V;
-  const int base = p * (BT * E);
-  float v[E];
-  const bool wide = (((uintptr_t)x) & 15) == 0;
+  const int begin = p * length, end = min(V, begin + length);
+  // A thread's values of a tile: four times four neighbours, or, where a part is short, single ones.  Which it has does not hang on where
+  // the row lies (equal rows have equal sums, to the bit); how they are read does.
+  const bool fours = length >= 4 * BT, wide = fours && (((uintptr_t)(x + begin)) & 15) == 0;
+  auto index = [&](int t, int e) { return begin + t * (BT * BE) + (fours ? (e / 4 * BT + tid) * 4 + (e & 3) : e * BT + tid); };
+  auto load = [&](int t, float* v) {
 #pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const int i = base + (e / 4 * BT + (int)threadIdx.x) * 4;
-    if (wide && i + 3 < V) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
-      v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-    } else {
+    for (int e = 0; e < BE; e += 4) {
+      const int i = index(t, e);
+      if (wide && i + 3 < end) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+      } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[e + c] = i + c < V ? __ldcs(x + i + c) : -CUDART_INF_F;
+        for (int c = 0; c < 4; ++c) v[e + c] = index(t, e + c) < end ? __ldg(x + index(t, e + c)) : -CUDART_INF_F;
+      }
+    }
+  };
+  if (tid == 0) s_n = 0;
+  const int tiles = (end - begin + BT * BE - 1) / (BT * BE);
+  float next[BE], mine = -CUDART_INF_F, bar = -CUDART_INF_F, top = -CUDART_INF_F, ref = -CUDART_INF_F;
+  double sum = 0.0;
+  int side = 0;                        // the list in use
+  load(0, next);
+  for (int t = 0; t < tiles; ++t) {
+    float v[BE], high = -CUDART_INF_F;
+#pragma unroll
+    for (int e = 0; e < BE; ++e) {
+      v[e] = finite(next[e]) ? next[e] : -CUDART_INF_F;
+      high = fmaxf(high, v[e]);
+    }
+    if (t + 1 < tiles) load(t + 1, next);
+    mine = fmaxf(mine, high);
+    __syncthreads();                   // the groups' maxima of the last tile are read, its tokens listed
+    const int listed = s_n;            // (read by all before any passes the barrier inside, behind which the list grows)
+    find_bar<BT>(mine, groups, s_group, bar, top);
+    if (top > ref + 20.0f) {           // alike in all threads; also true for the first finite value
+      sum *= ref == -CUDART_INF_F ? 0.0 : exp((double)ref - (double)top);
+      ref = top;
+    }
+    const float safe = ref == -CUDART_INF_F ? 0.f : ref;
+    float part_sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < BE; ++e) part_sum[e & 1] += expf(v[e] - safe);
+    sum += (double)(part_sum[0] + part_sum[1]);
+    if (listed > BC / 2 && listed <= BC) {       // the list anew, without what has fallen below the bar
+      __syncthreads();
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      for (int c = tid; c < listed; c += BT)
+        if (s_x[side][c] >= bar) {
+          const int to = atomicAdd(&s_n, 1);
+          s_x[side ^ 1][to] = s_x[side][c];
+          s_i[side ^ 1][to] = s_i[side][c];
+        }
+      side ^= 1;
+      __syncthreads();
+    }
+    if (high >= bar && high > -CUDART_INF_F) {
+#pragma unroll
+      for (int e = 0; e < BE; ++e)
+        if (v[e] >= bar && v[e] > -CUDART_INF_F) {
+          const int c = atomicAdd(&s_n, 1);
+          if (c < BC) {
+            s_x[side][c] = v[e];
+            s_i[side][c] = index(t, e);
+          }
+        }
     }
   }
-  float mine = -CUDART_INF_F;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (!finite(v[e])) v[e] = -CUDART_INF_F;
-    mine = fmaxf(mine, v[e]);
-  }
-  if (threadIdx.x == 0) s_n = 0;
-  float bar, top;
-  find_bar(mine, groups, s_group, bar, top);
-  const float safe = top == -CUDART_INF_F ? 0.f : top;
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) sum += expf(v[e] - safe);
   double all = sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = all;
-  if (mine >= bar && mine > -CUDART_INF_F) {
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (v[e] >= bar && v[e] > -CUDART_INF_F) {
-        const int c = atomicAdd(&s_n, 1);
-        if (c < BC) {
-          s_x[c] = v[e];
-          s_i[c] = base + (e / 4 * BT + (int)threadIdx.x) * 4 + (e & 3);
-        }
-      }
-  }
+  if ((tid & 31) == 0) s_sum[tid >> 5] = all;
   __syncthreads();
-  const int n = s_n;
-  if (threadIdx.x == 0) {
-    double t = 0.0;
+  int n = s_n;
+  if (tid == 0) {
+    double total = 0.0;
 #pragma unroll
-    for (int w = 0; w < BT / 32; ++w) t += s_sum[w];
-    part[at] = RowPart{t, top, min(n, choices)};
+    for (int w = 0; w < BT / 32; ++w) total += s_sum[w];
+    part[at] = RowPart{total, ref, 0.f};
   }
   if (n <= BC) {
-    for (int c = threadIdx.x; c < n; c += BT) {
-      const float mx = s_x[c];
-      const int mi = s_i[c];
+    // those that reach the last bar, ranked side by side
+    __syncthreads();
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    for (int c = tid; c < n; c += BT)
+      if (s_x[side][c] >= bar) {
+        const int to = atomicAdd(&s_n, 1);
+        s_x[side ^ 1][to] = s_x[side][c];
+        s_i[side ^ 1][to] = s_i[side][c];
+      }
+    side ^= 1;
+    __syncthreads();
+    n = s_n;
+    for (int c = n + tid; c < choices; c += BT) part_x[at * choices + c] = -CUDART_INF_F;
+    for (int c = tid; c < n; c += BT) {
+      const float mx = s_x[side][c];
+      const int mi = s_i[side][c];
       int rank = 0;
-      for (int o = 0; o < n; ++o) rank += ahead(s_x[o], s_i[o], mx, mi) ? 1 : 0;
+#pragma unroll 4
+      for (int o = 0; o < n; ++o) rank += ahead(s_x[side][o], s_i[side][o], mx, mi) ? 1 : 0;
       if (rank < choices) {
         part_x[at * choices + rank] = mx;
         part_i[at * choices + rank] = mi;
@@ -290,22 +358,21 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
     }
     return;
   }
-  // very many equal logits: one after the other
+  // very many equal logits: one after the other, from the row itself
   float past = CUDART_INF_F;
   int past_i = -1;
   for (int k = 0; k < choices; ++k) {
     float bx = -CUDART_INF_F;
     int bi = -1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = base + (e / 4 * BT + (int)threadIdx.x) * 4 + (e & 3);
-      if (v[e] > -CUDART_INF_F && ahead(past, past_i, v[e], i) && (bi < 0 || ahead(v[e], i, bx, bi))) {
-        bx = v[e];
+    for (int i = begin + tid; i < end; i += BT) {
+      const float y = x[i];
+      if (finite(y) && y >= bar && ahead(past, past_i, y, i) && (bi < 0 || ahead(y, i, bx, bi))) {
+        bx = y;
         bi = i;
       }
     }
-    best_of_block(bx, bi, s_x, s_i);
-    if (threadIdx.x == 0) {
+    best_of_block<BT>(bx, bi, s_x[0], s_i[0]);
+    if (tid == 0) {
       part_x[at * choices + k] = bx;
       part_i[at * choices + k] = bi;
     }
@@ -314,23 +381,30 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   }
 }
 
-__global__ void __launch_bounds__(BT)
+constexpr int CT = 512, CDEEP = 8;    // threads of the choice; candidates that a thread has on their way at once
+
+__global__ void __launch_bounds__(CT)
 beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, int groups, int parts, const RowPart* __restrict__ part,
                    const float* __restrict__ part_x, const int* __restrict__ part_i, float* __restrict__ out_scores,
                    int* __restrict__ out_beams, int* __restrict__ out_tokens) {
-  __shared__ double s_group[BT], s_x[BC], s_lift[BEAM_MOST];      // s_lift: a beam's score less the logarithm of its sum
+  __shared__ double s_group[CT], s_x[BC], s_lift[BEAM_MOST];      // s_lift: a beam's score less the logarithm of its sum
   __shared__ int s_i[BC], s_n, s_taken[BEAM_MOST];
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row0 = (size_t)b * K;
-  for (int k = warp; k < K; k += BT / 32) {
-    float top = -CUDART_INF_F;
-    for (int p = lane; p < parts; p += 32) top = fmaxf(top, part[(row0 + k) * parts + p].top);
+  for (int k = warp; k < K; k += CT / 32) {
+    const RowPart* of = part + (row0 + k) * parts;
+    RowPart first = {0.0, -CUDART_INF_F, 0.f};
+    if (lane < parts) first = of[lane];
+    float top = first.top;
+#pragma unroll 4
+    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, of[p].top);
     top = warp_max(top);
-    double sum = 0.0;
-    for (int p = lane; p < parts; p += 32) {
-      const RowPart r = part[(row0 + k) * parts + p];
+    double sum = first.sum > 0.0 ? first.sum * exp((double)first.top - (double)top) : 0.0;
+#pragma unroll 4
+    for (int p = lane + 32; p < parts; p += 32) {
+      const RowPart r = of[p];
       if (r.sum > 0.0) sum += r.sum * exp((double)r.top - (double)top);
     }
 #pragma unroll
@@ -339,34 +413,35 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
   }
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  // candidate c: the token of rank c % choices of part c / choices of the prompt's rows; its flat index is beam * V + token
-  const int all = K * parts * choices;
-  auto candidate = [&](int c, double& x, int& i) -> bool {
-    const int p = c / choices, k = p / parts;
-    if (c % choices >= part[row0 * parts + p].n) return false;
-    const size_t at = row0 * parts * choices + c;
-    x = (double)part_x[at] + s_lift[k];
-    i = k * V + part_i[at];
-    return true;
+  // candidate c: the token of rank c % choices of part c / choices of the prompt's rows (-inf where a part has fewer); its flat index
+  // is beam * V + token
+  const int of_beam = parts * choices, all = K * of_beam;
+  const float* xs = part_x + row0 * of_beam;
+  auto score = [&](int c, float x) { return x > -CUDART_INF_F ? (double)x + s_lift[c / of_beam] : -CUDART_INF; };
+  auto flat = [&](int c) { return c / of_beam * V + part_i[row0 * of_beam + c]; };
+  auto each = [&](auto&& take) {
+    for (int c0 = threadIdx.x; c0 < all; c0 += CT * CDEEP) {
+      float x[CDEEP];
+#pragma unroll
+      for (int j = 0; j < CDEEP; ++j) x[j] = c0 + j * CT < all ? xs[c0 + j * CT] : -CUDART_INF_F;
+#pragma unroll
+      for (int j = 0; j < CDEEP; ++j)
+        if (x[j] > -CUDART_INF_F) take(c0 + j * CT, score(c0 + j * CT, x[j]));
+    }
   };
   double mine = -CUDART_INF;
-  for (int c = threadIdx.x; c < all; c += BT) {
-    double x;
-    int i;
-    if (candidate(c, x, i) && x > mine) mine = x;
-  }
+  each([&](int, double x) { mine = x > mine ? x : mine; });
   double bar, top;
-  find_bar(mine, groups, s_group, bar, top);
-  for (int c = threadIdx.x; c < all; c += BT) {
-    double x;
-    int i;
-    if (!candidate(c, x, i) || x < bar) continue;
-    const int at = atomicAdd(&s_n, 1);
-    if (at < BC) {
-      s_x[at] = x;
-      s_i[at] = i;
-    }
-  }
+  find_bar<CT>(mine, groups, s_group, bar, top);
+  if (mine >= bar)
+    each([&](int c, double x) {
+      if (x < bar) return;
+      const int at = atomicAdd(&s_n, 1);
+      if (at < BC) {
+        s_x[at] = x;
+        s_i[at] = flat(c);
+      }
+    });
   __syncthreads();
   const int n = s_n;
   auto give = [&](int rank, double x, int i) {
@@ -376,7 +451,7 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
     s_taken[rank] = i;
   };
   if (n <= BC) {
-    for (int c = threadIdx.x; c < n; c += BT) {
+    for (int c = threadIdx.x; c < n; c += CT) {
       const double mx = s_x[c];
       const int mi = s_i[c];
       int rank = 0;
@@ -389,15 +464,15 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
     for (int k = 0; k < choices; ++k) {
       double bx = -CUDART_INF;
       int bi = -1;
-      for (int c = threadIdx.x; c < all; c += BT) {
-        double x;
-        int i;
-        if (candidate(c, x, i) && ahead(past, past_i, x, i) && (bi < 0 || ahead(x, i, bx, bi))) {
+      each([&](int c, double x) {
+        if (bi >= 0 && x < bx) return;
+        const int i = flat(c);
+        if (ahead(past, past_i, x, i) && (bi < 0 || ahead(x, i, bx, bi))) {
           bx = x;
           bi = i;
         }
-      }
-      best_of_block(bx, bi, s_x, s_i);
+      });
+      best_of_block<CT>(bx, bi, s_x, s_i);
       if (threadIdx.x == 0) give(k, bx, bi);
       past = bx;
       past_i = bi;
@@ -426,7 +501,14 @@ int beam_groups(int choices) {
   return g;
 }
 
-int beam_values(int rows, int V) { return (long long)rows * ((V + BT * 32 - 1) / (BT * 32)) >= 2 * 148 ? 32 : 8; }
+// How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part.
+void beam_cut(int rows, int V, int* parts, int* length) {
+  const int wave = 148 * 4, most = (V + BT * BE / 2 - 1) / (BT * BE / 2);
+  int n = wave / rows;
+  n = n < 1 ? 1 : n > most ? most : n;
+  *length = ((V + n - 1) / n + 3) & ~3;
+  *parts = (V + *length - 1) / *length;
+}
 
 }  // namespace
 
@@ -450,20 +532,21 @@ HK_API int hk_compact_rows(const long long* table, int arrays, const int* paths,
   if (arrays <= 0 || requests <= 0 || width <= 0) return 0;
   if (arrays > 65535 || table_rows < 1 || table_stride < 1 || page_tokens < 1 || heads < 1 || row_bytes < 1 || num_pages < 1)
     return HK_ERR_UNSUPPORTED;
-  const long long columns = (long long)heads * ((row_bytes + 15) / 16), blocks = (columns + KEEP_THREADS - 1) / KEEP_THREADS;
-  return hk_launch(compact_rows_kernel, dim3((unsigned)requests, (unsigned)arrays, (unsigned)(blocks < 64 ? blocks : 64)), dim3(KEEP_THREADS), 0,
-                   (cudaStream_t)stream, reinterpret_cast<const RowArray*>(table), paths, width, table_rows, table_stride, page_tokens, num_pages);
-}
-
-static long long beam_parts(int rows, int V) {
-  const int e = beam_values(rows, V);
-  return (V + BT * e - 1) / (BT * e);
+  if ((long long)heads * row_bytes > 0x7fffffffLL / 64) return HK_ERR_UNSUPPORTED;
+  // some two blocks of work a SM and more, but up to 8 arrays a block
+  int per_block = (int)((long long)arrays * requests / (148 * 4));
+  per_block = per_block < 1 ? 1 : per_block > 8 ? 8 : per_block;
+  return hk_launch(compact_rows_kernel, dim3((unsigned)requests, (unsigned)((arrays + per_block - 1) / per_block)), dim3(KEEP_THREADS), 0,
+                   (cudaStream_t)stream, reinterpret_cast<const RowArray*>(table), arrays, per_block, paths, width, table_rows, table_stride, page_tokens,
+                   num_pages);
 }
 
 // Bytes of scratch (16-byte aligned) that hk_beam_select wants.
 HK_API long long hk_beam_select_scratch(int rows, int V, int choices) {
   if (rows <= 0 || V <= 0 || choices <= 0) return 0;
-  return (long long)rows * beam_parts(rows, V) * ((long long)sizeof(RowPart) + 8LL * choices);
+  int parts, length;
+  beam_cut(rows, V, &parts, &length);
+  return (long long)rows * parts * ((long long)sizeof(RowPart) + 8LL * choices);
 }
 
 // logits float32 [prompts * beams, V], scores float32 [prompts * beams]; out_* [prompts, choices].
@@ -473,17 +556,17 @@ HK_API int hk_beam_select(const float* logits, const float* scores, int prompts,
   if (beams < 1 || beams > BEAM_MOST || V < 1 || choices < 1 || choices > BEAM_MOST || (long long)beams * V > 0x7fffffffLL ||
       choices > (long long)beams * V || (long long)prompts * beams > 0x7fffffffLL || (((uintptr_t)scratch) & 15) != 0)
     return HK_ERR_UNSUPPORTED;
-  const int rows = prompts * beams, parts = (int)beam_parts(rows, V), groups = beam_groups(choices);
+  const int rows = prompts * beams, groups = beam_groups(choices);
+  int parts, length;
+  beam_cut(rows, V, &parts, &length);
   if ((long long)rows * parts > 0x7fffffffLL || (long long)beams * parts * choices > 0x7fffffffLL) return HK_ERR_UNSUPPORTED;
   RowPart* part = static_cast<RowPart*>(scratch);
   float* part_x = reinterpret_cast<float*>(part + (size_t)rows * parts);
   int* part_i = reinterpret_cast<int*>(part_x + (size_t)rows * parts * choices);
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)(rows * parts)), block(BT);
-  const int e = beam_values(rows, V) == 32
-                    ? hk_launch_pdl(beam_rows_kernel<32>, grid, block, 0, s, logits, scores, V, choices, groups, parts, part, part_x, part_i)
-                    : hk_launch_pdl(beam_rows_kernel<8>, grid, block, 0, s, logits, scores, V, choices, groups, parts, part, part_x, part_i);
+  const int e = hk_launch_pdl(beam_rows_kernel, grid, block, 0, s, logits, scores, V, choices, groups, parts, length, part, part_x, part_i);
   if (e) return e;
-  return hk_launch_pdl(beam_choice_kernel, dim3((unsigned)prompts), block, 0, s, scores, beams, V, choices, groups, parts, part, part_x, part_i,
+  return hk_launch_pdl(beam_choice_kernel, dim3((unsigned)prompts), dim3(CT), 0, s, scores, beams, V, choices, groups, parts, part, part_x, part_i,
                        out_scores, out_beams, out_tokens);
 }

@@ -1570,13 +1570,13 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
         if hd in (64, 128) and choice != "generic":
             wide = q.dtype == torch.float32
             rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
-            # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), but no more shares than tiles
+            # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor
+            # cores of two: one for either group of warps
             held = all_keys if all_keys > 0 else m * most_keys
             if window > 0:
                 held = min(held, m * (window + most_tokens))
             tiles = -(-most_tokens * group // rows) * G * (held // keys + m)
-            # two tiles a share at least: one for either group of warps
-            ctas = max(1, min(gemm_fast._sms(q.device) * (2 if wide else 1), (tiles + 1) // 2))
+            ctas = max(1, min(gemm_fast._sms(q.device) * 2, tiles) if wide else min(gemm_fast._sms(q.device), (tiles + 1) // 2))
             cap = min(rows, most_tokens * group)
             part_o = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
             part_ml = part_o.data_ptr() + 8 * ctas * cap * hd

@@ -137,6 +137,16 @@ def test_equal_logits_and_equal_beams(V):
     check_beams(ops, np.zeros((8, V), dtype=np.float32), np.zeros(8, dtype=np.float32), 8, 64)
 
 
+def test_climbing_logits():
+    """Every tile's values above all before: the list of candidates is made anew again and again."""
+    from hk_b200.csrc import ops
+    rng = np.random.default_rng(8)
+    up = np.sort(rng.standard_normal((12, 151936)).astype(np.float32), axis=1)
+    for logits in (up, up[:, ::-1].copy()):
+        check_beams(ops, logits, -(rng.random(12) * 0.1).astype(np.float32), 4, 8)
+        check_beams(ops, np.repeat(logits, 60, axis=0)[:700], -(rng.random(700) * 0.1).astype(np.float32), 7, 100)
+
+
 def test_beams_that_are_not_there_and_masked_logits():
     from hk_b200.csrc import ops
     rng = np.random.default_rng(5)
