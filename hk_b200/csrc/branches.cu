@@ -150,11 +150,12 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
 // every continuation of a beam whose own score is not finite.
 //
 // One pass over the logits: a CTA takes a part of a row through registers, a tile of 4,096 at a time with the next one on its way, and
-// keeps a sum of exponentials against a reference near their maximum (a tile's sixteen a thread in float32, all beyond that in 64 bits) and
-// the tokens that can be among its best `choices`: as many groups of threads hold a value each that reaches the smallest of the groups' maxima, so what is
-// below that bar is out.  A CTA a prompt then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order:
-// two beams' continuations lie as little as 1e-7 apart often enough among a million, and which of them comes first must not hang on how
-// a sum was rounded.
+// keeps a sum of exponentials a thread against a reference of its own (a tile's sixteen in float32, all beyond that in 64 bits) and the
+// tokens that can be among its best `choices`: as many groups of threads hold a value each that reaches the smallest of the groups'
+// maxima, so what is below that bar is out; the bar is found anew after 1, 2, 4, ... tiles and where the list fills up.  A CTA a prompt
+// then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order: two beams' continuations lie as little
+// as 1e-7 apart often enough among a million, and which of them comes first must not hang on how a sum was rounded.
+// Bound by the instructions a logit: 8 or so, of which 5 are the exponential and its sum.
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
 constexpr int BC = 1024;              // candidates that are ranked side by side; more than that only among equal logits
@@ -229,6 +230,15 @@ __device__ __forceinline__ void best_of_block(F& x, int& i, F* s_x, int* s_i) {
   }
 }
 
+// e^x for x up to 20 and so: 2^(x log2 e) with the product in two parts, so that the constant's rounding adds no error that all terms
+// share; the product's own rounding is 2^-24 of it, the power's 2 units in the last place.
+__device__ __forceinline__ float exp_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, 1.9259629e-8f, x * 1.4426950216293335f)));
+  return y;
+}
+
+constexpr float LOWEST = -3.402823466e38f;
 constexpr int BE = 16;                // values of a tile a thread
 
 // The parts of a row are of `length` values (the last of what is left).
@@ -268,67 +278,81 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   };
   if (tid == 0) s_n = 0;
   const int tiles = (end - begin + BT * BE - 1) / (BT * BE);
-  float next[BE], mine = -CUDART_INF_F, bar = -CUDART_INF_F, top = -CUDART_INF_F, ref = -CUDART_INF_F;
+  float next[BE], mine = -CUDART_INF_F, bar = LOWEST, top = -CUDART_INF_F, ref = -CUDART_INF_F;
   double sum = 0.0;
   int side = 0;                        // the list in use
   load(0, next);
   for (int t = 0; t < tiles; ++t) {
-    float v[BE], high = -CUDART_INF_F;
+    float v[BE], high = -CUDART_INF_F, odd = 0.f;
 #pragma unroll
     for (int e = 0; e < BE; ++e) {
-      v[e] = finite(next[e]) ? next[e] : -CUDART_INF_F;
-      high = fmaxf(high, v[e]);
+      v[e] = next[e];
+      odd = fmaf(v[e], 0.f, odd);      // NaN where one is not finite
     }
+    if (odd != 0.f) {
+#pragma unroll
+      for (int e = 0; e < BE; ++e) v[e] = finite(v[e]) ? v[e] : -CUDART_INF_F;
+    }
+#pragma unroll
+    for (int e = 0; e < BE; ++e) high = fmaxf(high, v[e]);
     if (t + 1 < tiles) load(t + 1, next);
     mine = fmaxf(mine, high);
-    __syncthreads();                   // the groups' maxima of the last tile are read, its tokens listed
-    const int listed = s_n;            // (read by all before any passes the barrier inside, behind which the list grows)
-    find_bar<BT>(mine, groups, s_group, bar, top);
-    if (top > ref + 20.0f) {           // alike in all threads; also true for the first finite value
-      sum *= ref == -CUDART_INF_F ? 0.0 : exp((double)ref - (double)top);
-      ref = top;
+    // the barrier also says that the groups' maxima were read and the tokens of the last tile listed
+    if (__syncthreads_or(s_n > BC / 2) || (t & (t - 1)) == 0) {
+      const int listed = s_n;          // (read by all before any passes the barrier inside, behind which the list grows)
+      find_bar<BT>(mine, groups, s_group, bar, top);
+      bar = fmaxf(bar, LOWEST);
+      if (t == 0) ref = top;
+      if (listed > BC / 2 && listed <= BC) {       // the list anew, without what has fallen below the bar
+        __syncthreads();
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        for (int c = tid; c < listed; c += BT)
+          if (s_x[side][c] >= bar) {
+            const int to = atomicAdd(&s_n, 1);
+            s_x[side ^ 1][to] = s_x[side][c];
+            s_i[side ^ 1][to] = s_i[side][c];
+          }
+        side ^= 1;
+        __syncthreads();
+      }
+    }
+    if (high > ref + 20.0f) {          // also true for the first finite value behind a tile that had none
+      sum *= ref == -CUDART_INF_F ? 0.0 : exp((double)ref - (double)high);
+      ref = high;
     }
     const float safe = ref == -CUDART_INF_F ? 0.f : ref;
     float part_sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < BE; ++e) part_sum[e & 1] += expf(v[e] - safe);
+    for (int e = 0; e < BE; ++e) part_sum[e & 1] += exp_of(v[e] - safe);
     sum += (double)(part_sum[0] + part_sum[1]);
-    if (listed > BC / 2 && listed <= BC) {       // the list anew, without what has fallen below the bar
-      __syncthreads();
-      if (tid == 0) s_n = 0;
-      __syncthreads();
-      for (int c = tid; c < listed; c += BT)
-        if (s_x[side][c] >= bar) {
-          const int to = atomicAdd(&s_n, 1);
-          s_x[side ^ 1][to] = s_x[side][c];
-          s_i[side ^ 1][to] = s_i[side][c];
-        }
-      side ^= 1;
-      __syncthreads();
-    }
-    if (high >= bar && high > -CUDART_INF_F) {
+    if (high >= bar) {
+      uint32_t hits = 0;
 #pragma unroll
-      for (int e = 0; e < BE; ++e)
-        if (v[e] >= bar && v[e] > -CUDART_INF_F) {
-          const int c = atomicAdd(&s_n, 1);
-          if (c < BC) {
-            s_x[side][c] = v[e];
-            s_i[side][c] = index(t, e);
-          }
+      for (int e = 0; e < BE; ++e) hits |= v[e] >= bar ? 1u << e : 0u;
+      for (; hits; hits &= hits - 1) {
+        const int i = index(t, __ffs(hits) - 1), c = atomicAdd(&s_n, 1);
+        if (c < BC) {
+          s_x[side][c] = x[i];         // once more from the row: a register cannot be picked by a number
+          s_i[side][c] = i;
         }
+      }
     }
   }
-  double all = sum;
+  __syncthreads();
+  int n = s_n;
+  find_bar<BT>(mine, groups, s_group, bar, top);
+  bar = fmaxf(bar, LOWEST);
+  double all = ref == top || ref == -CUDART_INF_F ? sum : sum * exp((double)ref - (double)top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if ((tid & 31) == 0) s_sum[tid >> 5] = all;
   __syncthreads();
-  int n = s_n;
   if (tid == 0) {
     double total = 0.0;
 #pragma unroll
     for (int w = 0; w < BT / 32; ++w) total += s_sum[w];
-    part[at] = RowPart{total, ref, 0.f};
+    part[at] = RowPart{total, top, 0.f};
   }
   if (n <= BC) {
     // those that reach the last bar, ranked side by side
