@@ -4,6 +4,7 @@
   * `HKForCausalLM.from_pretrained(dir).generate(input_ids, max_new_tokens=20, temperature=1.0,
     top_k=50)`: the reference's signature and defaults (python/hk/modeling.py:621-664); like
     there the result is the input followed by the new tokens.
+  * `beam_search(model, prompts, num_beams=4, ...)`: the most probable continuations of every prompt.
   * `NativeHKEngine(dir).forward(tokens, pos)` -> logits after the last token, `forward_step`,
     `reset_cache`, `vocab_size`, `context_size` (python/hk/native.py:2298-2369).
 Texts, tokenizers and chat templates are outside this engine: prompts are token ids.
@@ -17,7 +18,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import numpy as np
 import torch
 
-from .engine import Engine, StepEntry
+from .engine import BeamSearch, Continuation, DraftDecoder, Engine, StepEntry
 from .engine.scheduler import Scheduler
 from .sampling import SamplingParams
 
@@ -56,14 +57,27 @@ def generate_with_engine(engine: Engine, prompts, max_new_tokens: int = 20, temp
                          top_k: int = 50, top_p: float = 1.0, min_p: float = 0.0, repeat_penalty: float = 1.0,
                          seed: int = 0, eos_token_ids: Optional[Sequence[int]] = None,
                          prefill_chunk: int = 512, stats: Optional[GenerationStats] = None,
-                         run_ahead: bool = True) -> List[List[int]]:
+                         run_ahead: bool = True, draft_tokens: int = 0) -> List[List[int]]:
     """Generates up to `max_new_tokens` for every prompt; returns the new tokens per prompt.
     temperature 0 picks the most likely token.  With seed != 0, request i draws from the
     stream of seed + i, so results do not depend on batching.  `run_ahead`: launch a decode step before
-    the host has read the previous step's tokens (same tokens, less idle GPU time)."""
+    the host has read the previous step's tokens (same tokens, less idle GPU time).  `draft_tokens` N > 0: a step verifies up to N
+    tokens guessed from the request's own text (`engine/drafts.py`); the output is the same, penalties are not taken."""
     plist, _ = _as_prompts(prompts)
     if eos_token_ids is None:
         eos_token_ids = getattr(engine.config, "eos_token_ids", ())
+    if draft_tokens:
+        params = [SamplingParams(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p),
+                                 repeat_penalty=float(repeat_penalty), seed=0 if seed == 0 else seed + i) for i in range(len(plist))]
+        decoder = DraftDecoder(engine, draft_tokens, max_new_tokens, eos_token_ids, prefill_chunk)
+        t0 = time.perf_counter()
+        out = decoder.run(plist, params)
+        if stats is not None:
+            stats.seconds = time.perf_counter() - t0
+            stats.prompt_tokens, stats.generated_tokens = sum(len(p) for p in plist), sum(len(o) for o in out)
+            stats.steps = stats.decode_steps = decoder.stats.steps
+            stats.decode_tokens = decoder.stats.tokens
+        return out
     sched = Scheduler(engine, prefill_chunk=prefill_chunk, eos_token_ids=eos_token_ids, run_ahead=run_ahead)
     ids = []
     for i, p in enumerate(plist):
@@ -106,15 +120,37 @@ def generate_with_engine(engine: Engine, prompts, max_new_tokens: int = 20, temp
 
 def generate(model: str, prompts, max_new_tokens: int = 20, temperature: float = 1.0, top_k: int = 50,
              top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, dtype: str = "bfloat16",
-             max_tokens: Optional[int] = None, **engine_options) -> List[List[int]]:
+             max_tokens: Optional[int] = None, draft_tokens: int = 0, **engine_options) -> List[List[int]]:
     """Loads the model folder `model` and generates for `prompts` (lists of token ids)."""
     plist, _ = _as_prompts(prompts)
     if max_tokens is None:
-        max_tokens = sum(-(-(len(p) + max_new_tokens) // 64) * 64 for p in plist)
+        max_tokens = sum(-(-(len(p) + max_new_tokens + draft_tokens) // 64) * 64 for p in plist)
     engine_options.setdefault("max_requests", max(1, min(len(plist), 64)))
     engine_options.setdefault("page_tokens", SERVING_PAGE_TOKENS)
     engine = Engine(model, dtype=dtype, max_tokens=max_tokens, **engine_options)
-    return generate_with_engine(engine, plist, max_new_tokens, temperature, top_k, top_p, min_p, seed=seed)
+    return generate_with_engine(engine, plist, max_new_tokens, temperature, top_k, top_p, min_p, seed=seed, draft_tokens=draft_tokens)
+
+
+def beam_search_with_engine(engine: Engine, prompts, num_beams: int = 4, max_new_tokens: int = 20, length_penalty: float = 1.0,
+                            eos_token_ids: Optional[Sequence[int]] = None, prefill_chunk: int = 2048) -> List[List[Continuation]]:
+    """The `num_beams` best continuations of every prompt, best first (`engine/beams.py`).  The engine needs a request slot a beam
+    and pages for what the beams do not share."""
+    plist, _ = _as_prompts(prompts)
+    if eos_token_ids is None:
+        eos_token_ids = getattr(engine.config, "eos_token_ids", ())
+    return BeamSearch(engine, num_beams, max_new_tokens, length_penalty, eos_token_ids, prefill_chunk).run(plist)
+
+
+def beam_search(model: str, prompts, num_beams: int = 4, max_new_tokens: int = 20, length_penalty: float = 1.0, dtype: str = "bfloat16",
+                max_tokens: Optional[int] = None, **engine_options) -> List[List[Continuation]]:
+    """Loads the model folder `model` and searches for the most probable continuations of `prompts` (lists of token ids)."""
+    plist, _ = _as_prompts(prompts)
+    page = engine_options.setdefault("page_tokens", SERVING_PAGE_TOKENS)
+    if max_tokens is None:         # the prompts' pages are shared; every beam may come to hold its continuation in pages of its own
+        max_tokens = sum((-(-len(p) // page) + num_beams * (max_new_tokens // page + 2)) * page for p in plist)
+    engine_options.setdefault("max_requests", max(1, num_beams * min(len(plist), max(1, 64 // num_beams))))
+    engine = Engine(model, dtype=dtype, max_tokens=max_tokens, **engine_options)
+    return beam_search_with_engine(engine, plist, num_beams, max_new_tokens, length_penalty)
 
 
 class HKForCausalLM:

@@ -8,12 +8,17 @@ per slot, [layer][kv head][position][head_dim]: src/cuda/engine.zig:234,393-401.
 table of a group is int32 [max_requests, max_pages_per_request] on the device, a copy of the
 host books' table; rows that changed are uploaded before a step runs.  A mixer with state of
 fixed size gets an array [max_requests, *shape], zeroed when a request takes its slot.
+
+A forked request shares the pages of the one that it was forked from and has a copy of its states; where one of them is about to
+write a shared page, its rows are copied first (`sync_tables`).  All arrays of a group, and all states, are copied by one launch
+each, and so are the rows of an accepted path moved (`keep`).
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..csrc import ops
@@ -83,11 +88,27 @@ class PagedCache:
                     self._states.append(st)
                     caches.append(LayerCache("state", state=st))
             self.layers.append(caches)
+        # what the kernels that copy blocks and move rows read, one record an array (see csrc/ops.py)
+        self._page_tables: List[torch.Tensor] = []
+        self._row_tables: List[torch.Tensor] = []
+        self._page_arrays: List[List[torch.Tensor]] = [[] for _ in keys]
+        for caches in self.layers:
+            for lc in caches:
+                if lc.kind == "pages":
+                    self._page_arrays[lc.group] += [t for t in (lc.k_pages, lc.v_pages) if t is not None]
+        for gi, arrays in enumerate(self._page_arrays):
+            row = [t.shape[3] * t.element_size() for t in arrays]
+            self._page_tables.append(torch.tensor([[t.data_ptr(), num_pages, t.shape[1], page_tokens * r, r] for t, r in zip(arrays, row)],
+                                                  dtype=torch.int64, device=dev))
+            self._row_tables.append(torch.tensor([[t.data_ptr(), t.shape[1], r, self.tables[gi].data_ptr()] for t, r in zip(arrays, row)],
+                                                 dtype=torch.int64, device=dev))
         sizes = [st[0].numel() * st.element_size() for st in self._states]
         self._state_bytes = max(sizes, default=0)
         self._state_table = None
         if self._states and torch.device(dev).type == "cuda":
             self._state_table = torch.tensor([[st.data_ptr(), b] for st, b in zip(self._states, sizes)], dtype=torch.int64, device=dev)
+            self._slot_table = torch.tensor([[st.data_ptr(), max_requests, 1, b, b] for st, b in zip(self._states, sizes)], dtype=torch.int64,
+                                            device=dev)
 
     def has_state(self) -> bool:
         """Whether any mixer keeps a state of fixed size (which running a row twice would advance twice)."""
@@ -106,11 +127,84 @@ class PagedCache:
     def close(self, slot: int) -> None:
         self.books.close(slot)
 
+    def fork(self, slots: Sequence[int]) -> List[int]:
+        """A new slot for each of `slots`, with its tokens: pages shared, states copied."""
+        new = []
+        try:
+            for s in slots:
+                new.append(self.books.fork(int(s)))
+        except Exception:
+            for s in new:
+                self.books.close(s)
+            raise
+        if self._states and new:
+            if self._state_table is not None:
+                moves = torch.tensor([[int(a), b, 1] for a, b in zip(slots, new)], dtype=torch.int32, device=self._slot_table.device)
+                ops.copy_blocks(self._slot_table, moves, self._state_bytes)
+            else:
+                for st in self._states:
+                    for a, b in zip(slots, new):
+                        st[b].copy_(st[int(a)])
+        return new
+
+    def keep(self, paths: Sequence[tuple]) -> None:
+        """Moves the accepted rows of drafted trees up in every cache of the model.  `paths`: (slot, the cache's row where the tree
+        begins, the accepted rows of the tree in ascending order); the books' lengths stay the caller's business."""
+        width = max((len(kept) for _, _, kept in paths), default=0)
+        if not any(list(kept) != list(range(len(kept))) for _, _, kept in paths):
+            return                              # every row is where it has to be
+        rec = np.full((len(paths), 2 + width), -1, dtype=np.int32)
+        for i, (slot, first, kept) in enumerate(paths):
+            rec[i, :2] = slot, first
+            rec[i, 2:2 + len(kept)] = kept
+        dev = torch.from_numpy(rec).to(self.precision.device)
+        self.uploaded_bytes += rec.nbytes
+        for table, arrays, bt in zip(self._row_tables, self._page_arrays, self.tables):
+            if arrays:
+                ops.compact_rows(table, dev, bt.shape[0], bt.shape[1], self.page_tokens, max(t.shape[1] for t in arrays),
+                                 max(t.shape[3] * t.element_size() for t in arrays), self.num_pages)
+
+    def _copy_pages(self) -> None:
+        """Makes the copies that the books owe.  One that reads or writes a page which an earlier one of them writes, or writes one which an
+        earlier one reads, waits for a launch of its own."""
+        owed = self.books.take_copies()
+        for gi, arrays in enumerate(self._page_arrays):
+            batch, busy_to, busy_from = [], set(), set()
+
+            def launch():
+                if not batch:
+                    return
+                if arrays[0].is_cuda:
+                    moves = torch.tensor(batch, dtype=torch.int32, device=arrays[0].device)
+                    ops.copy_blocks(self._page_tables[gi], moves, max(t[0].numel() * t.element_size() for t in arrays))
+                else:
+                    for a, b, rows in batch:
+                        for t in arrays:
+                            t[b, :, :rows].copy_(t[a, :, :rows])
+                self.uploaded_bytes += 12 * len(batch)
+                batch.clear(), busy_to.clear(), busy_from.clear()
+
+            for a, b, rows in owed[owed[:, 0] == gi, 1:].tolist():
+                if a in busy_to or b in busy_to or b in busy_from:
+                    launch()
+                batch.append((a, b, rows))
+                busy_to.add(b), busy_from.add(a)
+            launch()
+
     def sync_tables(self) -> None:
-        """Uploads the block-table rows that changed since the last call.  The copies read
+        """Makes the copies that the books owe and uploads the block-table rows that changed since the last call.  The copies read
         pageable host memory, so they are complete (staged) when the call returns and the
         books may change again at once."""
+        self._copy_pages()
         if not self.books.dirty:
+            return
+        if len(self.books.dirty) > 4:            # many rows (a batch of beams): one upload, not one a row
+            rows = sorted(self.books.dirty)
+            for g, dev_table in zip(self.books.groups, self.tables):
+                at = torch.tensor(rows, dtype=torch.int64, device=dev_table.device)
+                dev_table.index_copy_(0, at, torch.from_numpy(g.table[rows]).to(dev_table.device))
+                self.uploaded_bytes += (g.table.shape[1] * 4 + 8) * len(rows)
+            self.books.dirty.clear()
             return
         for slot in sorted(self.books.dirty):
             for g, dev_table in zip(self.books.groups, self.tables):

@@ -11,6 +11,9 @@ on the native side.  Nothing here touches the GPU, so every decision can be test
 * Pages are taken when a request's tokens need them, given back when the request ends and,
   in a windowed group, as soon as the window has passed them; freed pages are reused at once
   (last freed, first reused: stale contents meet new owners early, which the tests want).
+* A *fork* is a new slot with another's tokens.  It shares that one's pages: a page counts its holders and returns to the pool with the
+  last of them.  A request that is about to write a page which others hold too (the last, partly filled one) takes a page of its own
+  instead and owes a copy of the rows written so far (`take_copies`), to be made before anything else writes.
 * A *state slot* is a request's index into per-request arrays of fixed size: the block-table
   rows and any fixed-size mixer state.  The reference's analogues: a slot per sequence with a
   fixed region (src/cuda/engine.zig:393-401,556-572) and segments grown on demand and freed
@@ -66,7 +69,8 @@ def _runtime() -> ctypes.CDLL:
             ("hk_books_first_page", ctypes.POINTER(ctypes.c_int32), [vp, ci]), ("hk_books_n_pages", ctypes.POINTER(ctypes.c_int32), [vp, ci]),
             ("hk_books_open", ci, [vp]), ("hk_books_close", ci, [vp, ci]), ("hk_books_release_passed", ci, [vp, ci]),
             ("hk_books_pages_to_take", ci, [vp, ci, ci, ctypes.POINTER(ci)]), ("hk_books_pages_passed", ci, [vp, ci, ctypes.POINTER(ci)]), ("hk_books_free_pages", None, [vp, ctypes.POINTER(ci)]),
-            ("hk_books_extend", ci, [vp, ci, ci]), ("hk_books_truncate", ci, [vp, ci, ci]), ("hk_books_audit", ci, [vp]),
+            ("hk_books_shared_page", ci, [vp, ci, ctypes.POINTER(ci), ctypes.POINTER(ci)]), ("hk_books_fork", ci, [vp, ci]),
+            ("hk_books_copies", ci, [vp, ctypes.POINTER(ci), ci]), ("hk_books_extend", ci, [vp, ci, ci]), ("hk_books_truncate", ci, [vp, ci, ci]), ("hk_books_audit", ci, [vp]),
         ]:
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
@@ -161,6 +165,7 @@ class CacheBooks:
         self.live = as_array(rt.hk_books_live(self._h), shape=(max_requests,)).view(np.bool_)
         self.dirty: set = set()                                 # slots whose table rows changed
         self._take = (ctypes.c_int * max(1, len(windows)))()
+        self._holders = (ctypes.c_int * max(1, len(windows)))()
 
     def __del__(self):
         if getattr(self, "_h", None):
@@ -180,6 +185,12 @@ class CacheBooks:
         self._check(self._rt.hk_books_close(self._h, int(slot)))
         self.dirty.add(int(slot))
 
+    def fork(self, slot: int) -> int:
+        """A new slot with the tokens of `slot`, whose pages it shares."""
+        new = self._check(self._rt.hk_books_fork(self._h, int(slot)))
+        self.dirty.add(new)
+        return new
+
     # -- pages -----------------------------------------------------------------------------
     def release_passed(self, slot: int) -> int:
         """Gives back the pages of `slot` that its windows have passed; returns how many."""
@@ -189,7 +200,7 @@ class CacheBooks:
         return n
 
     def pages_passed(self, slot: int) -> List[int]:
-        """For each group: the pages `release_passed(slot)` would give back now."""
+        """For each group: the pages `release_passed(slot)` would give back to the pool now."""
         self._check(self._rt.hk_books_pages_passed(self._h, int(slot), self._take))
         return list(self._take[:len(self.groups)])
 
@@ -202,9 +213,24 @@ class CacheBooks:
         self._rt.hk_books_free_pages(self._h, self._take)
         return list(self._take[:len(self.groups)])
 
+    def shared_pages(self, slot: int) -> List[tuple]:
+        """For each group: (page, holders) of the page that the next token of `slot` would be written to while others hold it
+        too, or (-1, 0)."""
+        self._check(self._rt.hk_books_shared_page(self._h, int(slot), self._take, self._holders))
+        return list(zip(self._take[:len(self.groups)], self._holders[:len(self.groups)]))
+
+    def take_copies(self) -> np.ndarray:
+        """The copies owed since the last call, in order: int32 [n, 4] = (group, from page, to page, rows)."""
+        n = int(self._rt.hk_books_copies(self._h, None, 0))
+        out = np.empty((n, 4), dtype=np.int32)
+        if n:
+            self._rt.hk_books_copies(self._h, out.ctypes.data_as(ctypes.POINTER(ctypes.c_int)), n)
+        return out
+
     def extend(self, slot: int, n_new: int) -> None:
         """Makes room for `n_new` more tokens of `slot`: gives back pages the window has passed,
-        then takes the pages the new positions need.  Takes all of them or none."""
+        then takes the pages the new positions need, and one in the place of a page that it would write while others hold it
+        (`take_copies`).  Takes all of them or none."""
         if self._check(self._rt.hk_books_extend(self._h, int(slot), int(n_new))):
             self.dirty.add(int(slot))
 

@@ -30,6 +30,9 @@ USAGE = """Usage: hk run <model folder> [token ids | -p IDS] [options]
       --max-ctx N       context length to provide (default: prompt + max tokens, rounded up to 64)
       --prompt-len N    instead of a prompt: N token ids drawn uniformly from the vocabulary with --seed
       --page-tokens N   tokens per cache page (default 64)
+      --draft N         verify up to N tokens guessed from the text so far in a step (default 0: one token a step)
+      --beams K         the most probable continuation found with K beams; no sampling (default 1: off)
+      --length-penalty X  beams: a continuation's log probability is divided by its length to this power (default 1.0)
 
        hk random <config.json> <new model folder> [--seed N] [--dtype D] [--std S]
                         writes config.json and model.safetensors with seeded random weights
@@ -88,7 +91,8 @@ def parse_ids(text: str):
 def parse_run_args(args):
     """Returns a dict of settings; raises BadUsage on anything unknown or malformed."""
     g = dict(model=None, prompt=None, max_tokens=128, temperature=0.8, top_k=40, top_p=0.95, min_p=0.05,
-             repeat_penalty=1.0, seed=0, dtype="bfloat16", max_ctx=None, prompt_len=None, page_tokens=None)
+             repeat_penalty=1.0, seed=0, dtype="bfloat16", max_ctx=None, prompt_len=None, page_tokens=None, draft=0, beams=1,
+             length_penalty=1.0)
     i = 0
     while i < len(args):
         flag = args[i]
@@ -147,6 +151,19 @@ def parse_run_args(args):
         elif flag == "--page-tokens":
             g["page_tokens"] = _uint(args, i, flag, 1)
             i += 2
+        elif flag == "--draft":
+            g["draft"] = _uint(args, i, flag, 0)
+            if g["draft"] > 255:
+                _fail(f"Error: '--draft' got '{g['draft']}', expected at most 255")
+            i += 2
+        elif flag == "--beams":
+            g["beams"] = _uint(args, i, flag, 1)
+            if g["beams"] > 128:
+                _fail(f"Error: '--beams' got '{g['beams']}', expected at most 128")
+            i += 2
+        elif flag == "--length-penalty":
+            g["length_penalty"] = _float_in(args, i, flag, 0, 100, "a number from 0 up")
+            i += 2
         elif flag.startswith("-") and len(flag) > 1 and not flag[1:].replace(",", "").replace(" ", "").isdigit():
             _fail(f"Error: unknown argument '{flag}'")
         elif g["model"] is None:
@@ -159,6 +176,10 @@ def parse_run_args(args):
             i += 1
     if g["model"] is None:
         _fail("Error: no model folder was given")
+    if g["beams"] > 1 and g["draft"]:
+        _fail("Error: '--beams' and '--draft' do not go together")
+    if g["draft"] and g["repeat_penalty"] != 1.0:
+        _fail("Error: '--draft' does not go with '--repeat-penalty': a penalty follows the tokens drawn so far")
     if g["prompt"] is not None and g["prompt_len"] is not None:
         _fail("Error: both a prompt and '--prompt-len' were given")
     if g["prompt"] is None and g["prompt_len"] is None:
@@ -173,18 +194,19 @@ def cmd_run(args) -> int:
     except BadUsage as e:
         print(f"{e}\n{USAGE}", file=sys.stderr, end="")
         return 2
-    from .api import GenerationStats, generate_with_engine
+    from .api import SERVING_PAGE_TOKENS, beam_search_with_engine, generate_with_engine
     from .config import ConfigError
     from .engine import Engine, EngineError
     from .weights import SafetensorsError, WeightError
     ids = g["prompt_ids"]
     n_prompt = len(ids) if ids is not None else g["prompt_len"]
     ctx = g["max_ctx"] or -(-(n_prompt + g["max_tokens"]) // 64) * 64
+    page = g["page_tokens"] or SERVING_PAGE_TOKENS
+    pool = ctx + g["draft"] + (g["beams"] - 1) * (g["max_tokens"] + 2 * page) if g["beams"] > 1 or g["draft"] else ctx
     try:
         t0 = time.perf_counter()
-        from .api import SERVING_PAGE_TOKENS
-        engine = Engine(g["model"], dtype=g["dtype"], max_tokens=ctx, page_tokens=g["page_tokens"] or SERVING_PAGE_TOKENS,
-                        max_requests=1, max_context=ctx, max_batch_tokens=max(ctx, 1))
+        engine = Engine(g["model"], dtype=g["dtype"], max_tokens=pool, page_tokens=page, max_requests=g["beams"], max_context=ctx,
+                        max_batch_tokens=max(ctx, g["beams"]))
         if ids is None:
             import numpy as np
             ids = np.random.default_rng(g["seed"]).integers(0, engine.vocab, n_prompt).tolist()
@@ -196,6 +218,19 @@ def cmd_run(args) -> int:
         import torch
         from .engine.scheduler import Scheduler
         from .sampling import SamplingParams
+        if g["beams"] > 1 or g["draft"]:
+            t1 = time.perf_counter()
+            if g["beams"] > 1:
+                out = beam_search_with_engine(engine, [ids], g["beams"], g["max_tokens"], g["length_penalty"])[0][0].tokens
+            else:
+                out = generate_with_engine(engine, [ids], g["max_tokens"], g["temperature"], g["top_k"], g["top_p"], g["min_p"],
+                                           seed=g["seed"], prefill_chunk=2048, draft_tokens=g["draft"])[0]
+            torch.cuda.synchronize()
+            s = time.perf_counter() - t1
+            print(" ".join(str(t) for t in out))
+            print(f"\n[prompt {len(ids)} tok, generated {len(out)} tok, {len(out) / max(s, 1e-9):.1f} tok/s with the prompt | load {load_s:.1f} s]",
+                  file=sys.stderr)
+            return 0
         # one request, nobody waits behind its prompt: portions of 2,048 tokens, where the prefill kernels run best
         sched = Scheduler(engine, prefill_chunk=2048, eos_token_ids=getattr(engine.config, "eos_token_ids", ()))
         rid = sched.submit(ids, g["max_tokens"], SamplingParams(

@@ -253,7 +253,7 @@ __global__ void qk_norm_rope_kv_write_kernel(
     const int* __restrict__ slot_of_token, const int* __restrict__ block_table, int table_stride,
     T* __restrict__ k_pages, T* __restrict__ v_pages, int n, int H, int G, int hd, int page_tokens,
     int write_kv, const float* __restrict__ bias, int pairing, int norm_after, int tied_v, int vd, long long ld,
-    QueryFactor qt) {
+    QueryFactor qt, const int* __restrict__ rows) {
   __shared__ float buf[QKR_WARPS][QKR_MAX_HD];
   pdl_launch_dependents();
   pdl_wait();
@@ -280,12 +280,13 @@ __global__ void qk_norm_rope_kv_write_kernel(
   }
   __syncwarp();
   int pos = positions[t];
+  const int at = rows ? rows[t] : pos;       // the token's row in the cache
   int page = -1;
   if (kind != 0) {
-    page = block_table[(size_t)slot_of_token[t] * table_stride + pos / page_tokens];
+    page = block_table[(size_t)slot_of_token[t] * table_stride + at / page_tokens];
     if (page < 0) return;  // the host never schedules this; keeps a stale table from writing out of bounds
     if (kind == 1 && tied_v) {   // the value is the key as projected
-      T* vdst = v_pages + (((size_t)page * G + (hh - H)) * page_tokens + (pos % page_tokens)) * vd;
+      T* vdst = v_pages + (((size_t)page * G + (hh - H)) * page_tokens + (at % page_tokens)) * vd;
       for (int i = lane; i < vd; i += 32) vdst[i] = from_f32<T>(v[i]);
     }
   }
@@ -329,10 +330,10 @@ __global__ void qk_norm_rope_kv_write_kernel(
   if (kind == 0) {
     dst = q_out + (size_t)t * H * hd + (size_t)hh * hd;
   } else if (kind == 1) {
-    dst = k_pages + (((size_t)page * G + (hh - H)) * page_tokens + (pos % page_tokens)) * hd;
+    dst = k_pages + (((size_t)page * G + (hh - H)) * page_tokens + (at % page_tokens)) * hd;
   } else {
     width = vd;
-    dst = v_pages + (((size_t)page * G + (hh - H - G)) * page_tokens + (pos % page_tokens)) * vd;
+    dst = v_pages + (((size_t)page * G + (hh - H - G)) * page_tokens + (at % page_tokens)) * vd;
   }
   for (int i = lane; i < width; i += 32) dst[i] = from_f32<T>(v[i]);
 }
@@ -350,7 +351,7 @@ qk_norm_rope_kv_write_vec_kernel(
     const int* __restrict__ slot_of_token, const int* __restrict__ block_table, int table_stride,
     T* __restrict__ k_pages, T* __restrict__ v_pages, int n, int H, int G, int hd, int page_tokens,
     int write_kv, const float* __restrict__ bias, int pairing, int norm_after, int tied_v, int vd, long long ld,
-    QueryFactor qt) {
+    QueryFactor qt, const int* __restrict__ rows) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -371,11 +372,11 @@ qk_norm_rope_kv_write_vec_kernel(
     const float4 b = *reinterpret_cast<const float4*>(bias + col + d0);
     v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
   }
-  const int pos = positions[t];
+  const int pos = positions[t], at = rows ? rows[t] : pos;       // at: the token's row in the cache
   int page = 0;
-  if (kind != 0) page = block_table[(size_t)slot_of_token[t] * table_stride + pos / page_tokens];
+  if (kind != 0) page = block_table[(size_t)slot_of_token[t] * table_stride + at / page_tokens];
   if (kind == 1 && tied_v && page >= 0 && d0 < vd) {      // the value is the key as projected
-    T* vdst = v_pages + (((size_t)page * G + (hh - H)) * page_tokens + (pos % page_tokens)) * vd;
+    T* vdst = v_pages + (((size_t)page * G + (hh - H)) * page_tokens + (at % page_tokens)) * vd;
     if (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(reinterpret_cast<float*>(vdst) + d0) = v;
     } else {
@@ -443,9 +444,9 @@ qk_norm_rope_kv_write_vec_kernel(
   if (kind == 0) {
     dst = q_out + (size_t)t * H * hd + (size_t)hh * hd;
   } else if (kind == 1) {
-    dst = k_pages + (((size_t)page * G + (hh - H)) * page_tokens + (pos % page_tokens)) * hd;
+    dst = k_pages + (((size_t)page * G + (hh - H)) * page_tokens + (at % page_tokens)) * hd;
   } else {
-    dst = v_pages + (((size_t)page * G + (hh - H - G)) * page_tokens + (pos % page_tokens)) * vd;
+    dst = v_pages + (((size_t)page * G + (hh - H - G)) * page_tokens + (at % page_tokens)) * vd;
   }
   if (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + d0) = v;
@@ -470,19 +471,19 @@ qk_norm_rope_kv_write_halves_kernel(const float* __restrict__ qkv, T* __restrict
                                     const int* __restrict__ positions, const int* __restrict__ slot_of_token,
                                     const int* __restrict__ block_table, int table_stride, T* __restrict__ k_pages, T* __restrict__ v_pages,
                                     int H, int G, int page_tokens, int write_kv, const float* __restrict__ bias, int norm_after, long long ld,
-                                    QueryFactor qt) {
+                                    QueryFactor qt, const int* __restrict__ rows) {
   constexpr int HD = 128;
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = (lane & 15) * 4;
   const int heads = H + (write_kv ? 2 * G : 0), step = 2 * QKH_WARPS * gridDim.y;
   const float* src = qkv + (size_t)t * (size_t)ld + d0;
-  const int pos = positions[t];
+  const int pos = positions[t], at = rows ? rows[t] : pos;       // at: the token's row in the cache
   const float4 c = *reinterpret_cast<const float4*>(cos_t + (size_t)pos * (HD / 2) + d0);
   const float4 sn = *reinterpret_cast<const float4*>(sin_t + (size_t)pos * (HD / 2) + d0);
   int page = -1;
-  if (write_kv) page = block_table[(size_t)slot_of_token[t] * table_stride + pos / page_tokens];
-  const size_t place = ((size_t)max(page, 0) * G * page_tokens + pos % page_tokens) * HD + d0;      // of key head 0
+  if (write_kv) page = block_table[(size_t)slot_of_token[t] * table_stride + at / page_tokens];
+  const size_t place = ((size_t)max(page, 0) * G * page_tokens + at % page_tokens) * HD + d0;      // of key head 0
   const float one = 1.0f, factor = qt.every > 0 ? query_factor(qt, pos) : one;
   auto normed = [&](float4& a, float4& b, const float* w) {
     float ss = fmaf(a.x, a.x, fmaf(a.y, a.y, fmaf(a.z, a.z, a.w * a.w)));
@@ -556,7 +557,7 @@ HK_API int hk_qk_norm_rope_kv_write(const float* qkv, void* q_out, int dtype, co
                                     const int* block_table, int table_stride, void* k_pages,
                                     void* v_pages, int n, int H, int G, int hd, int page_tokens,
                                     int write_kv, const float* bias, int pairing, int norm_after, int tied_v, int vd,
-                                    long long ld, float qt_coef, int qt_every, void* stream) {
+                                    long long ld, float qt_coef, int qt_every, const int* rows, void* stream) {
   const QueryFactor qt = {qt_coef, qt_every};
   if (qt_every < 0) return HK_ERR_UNSUPPORTED;
   if (ld <= 0) ld = (long long)(H + G) * hd + (tied_v ? 0 : (long long)G * vd);
@@ -572,11 +573,11 @@ HK_API int hk_qk_norm_rope_kv_write(const float* qkv, void* q_out, int dtype, co
     if (dtype == HK_F32)
       return hk_launch_pdl(qk_norm_rope_kv_write_halves_kernel<float>, grid, block, 0, s, qkv, (float*)q_out, q_w, k_w, eps, cos_t, sin_t,
                            positions, slot_of_token, block_table, table_stride, (float*)k_pages, (float*)v_pages, H, G, page_tokens,
-                           write_kv, bias, norm_after, ld, qt);
+                           write_kv, bias, norm_after, ld, qt, rows);
     if (dtype == HK_BF16)
       return hk_launch_pdl(qk_norm_rope_kv_write_halves_kernel<bf16>, grid, block, 0, s, qkv, (bf16*)q_out, q_w, k_w, eps, cos_t, sin_t,
                            positions, slot_of_token, block_table, table_stride, (bf16*)k_pages, (bf16*)v_pages, H, G, page_tokens,
-                           write_kv, bias, norm_after, ld, qt);
+                           write_kv, bias, norm_after, ld, qt, rows);
     return HK_ERR_UNSUPPORTED;
   }
   if (hd <= 128 && vd <= 128 && (hd & 3) == 0 && (vd & 3) == 0 && (rot & 7) == 0 && (ld & 3) == 0 && aligned) {
@@ -584,22 +585,22 @@ HK_API int hk_qk_norm_rope_kv_write(const float* qkv, void* q_out, int dtype, co
     if (dtype == HK_F32)
       return hk_launch_pdl(qk_norm_rope_kv_write_vec_kernel<float>, dim3(vblocks), dim3(QKV_WARPS * 32), 0, s, qkv, (float*)q_out,
                        q_w, k_w, eps, cos_t, sin_t, rot, positions, slot_of_token, block_table, table_stride, (float*)k_pages,
-                       (float*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt);
+                       (float*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt, rows);
     if (dtype == HK_BF16)
       return hk_launch_pdl(qk_norm_rope_kv_write_vec_kernel<bf16>, dim3(vblocks), dim3(QKV_WARPS * 32), 0, s, qkv, (bf16*)q_out, q_w,
                        k_w, eps, cos_t, sin_t, rot, positions, slot_of_token, block_table, table_stride, (bf16*)k_pages,
-                       (bf16*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt);
+                       (bf16*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt, rows);
     return HK_ERR_UNSUPPORTED;
   }
   unsigned blocks = (unsigned)((items + QKR_WARPS - 1) / QKR_WARPS);
   if (dtype == HK_F32)
     return hk_launch(qk_norm_rope_kv_write_kernel<float>, dim3(blocks), dim3(QKR_WARPS * 32), 0, s, qkv, (float*)q_out, q_w,
                          k_w, eps, cos_t, sin_t, rot, positions, slot_of_token, block_table, table_stride, (float*)k_pages,
-                         (float*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt);
+                         (float*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt, rows);
   if (dtype == HK_BF16)
     return hk_launch(qk_norm_rope_kv_write_kernel<bf16>, dim3(blocks), dim3(QKR_WARPS * 32), 0, s, qkv, (bf16*)q_out, q_w,
                          k_w, eps, cos_t, sin_t, rot, positions, slot_of_token, block_table, table_stride, (bf16*)k_pages,
-                         (bf16*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt);
+                         (bf16*)v_pages, n, H, G, hd, page_tokens, write_kv, bias, pairing, norm_after, tied_v, vd, ld, qt, rows);
   return HK_ERR_UNSUPPORTED;
 }
 

@@ -315,7 +315,7 @@ PAIRINGS = {"half": 0, "adjacent": 1}
 def qk_norm_rope_kv_write(qkv, q_out, q_weight, k_weight, eps, cos, sin, rotary_dim, positions,
                           slot_of_token, block_table, k_pages, v_pages, n_heads, n_kv_heads, head_dim,
                           page_tokens, write_kv=True, bias=None, pairing="half", norm_after=False, tied_v=False,
-                          q_factor=None) -> None:
+                          q_factor=None, rows=None) -> None:
     """Splits the fused projection qkv[n, (H+G)*hd + G*vd] (float32; vd = v_pages' width, hd unless the values have a
     width of their own): q heads are normalised (if
     q_weight), rotated (if rotary_dim > 0) and stored to q_out[n, H*hd]; k heads likewise and
@@ -324,7 +324,8 @@ def qk_norm_rope_kv_write(qkv, q_out, q_weight, k_weight, eps, cos, sin, rotary_
     (i, i + rotary_dim/2), "adjacent" dims (2i, 2i+1).  `norm_after`: the per-head norm comes behind the
     rotation, and a missing weight then means a weight of ones.  `tied_v`: qkv is [n, (H+G)*hd] and a token's
     value is its key as projected (before norm and rotation), of which the first v_pages.shape[-1] dims are kept.
-    `q_factor` (coef, every): a query at position p is then multiplied by 1 + coef ln(floor((p + 1) / every) + 1)."""
+    `q_factor` (coef, every): a query at position p is then multiplied by 1 + coef ln(floor((p + 1) / every) + 1).  `rows` (int32
+    [n]): the tokens' rows in their requests' caches, where they are not their positions (the tokens of a drafted tree)."""
     if pairing not in PAIRINGS:
         raise KernelError(f"qk_norm_rope_kv_write: pairing {pairing!r} is neither 'half' nor 'adjacent'")
     if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
@@ -354,6 +355,10 @@ def qk_norm_rope_kv_write(qkv, q_out, q_weight, k_weight, eps, cos, sin, rotary_
             raise KernelError("rotation tables must be [positions, rotary_dim/2]")
     _need(positions, "positions", torch.int32, 1)
     _need(slot_of_token, "slot_of_token", torch.int32, 1)
+    if rows is not None:
+        _need(rows, "rows", torch.int32, 1)
+        if rows.shape[0] != n:
+            raise KernelError("qk_norm_rope_kv_write: one cache row per token")
     if write_kv:
         _need(block_table, "block_table", torch.int32, 2)
         _need(k_pages, "k_pages", q_out.dtype, 4)
@@ -369,7 +374,7 @@ def qk_norm_rope_kv_write(qkv, q_out, q_weight, k_weight, eps, cos, sin, rotary_
         int(block_table.shape[1]) if write_kv else 0, _ptr(k_pages if write_kv else None),
         _ptr(v_pages if write_kv else None), n, H, G, hd, int(page_tokens), 1 if write_kv else 0, _ptr(bias),
         PAIRINGS[pairing], 1 if norm_after else 0, 1 if tied_v else 0, vd, qkv.stride(0),
-        *_query_factor(q_factor), _stream()),
+        *_query_factor(q_factor), _ptr(rows), _stream()),
         "qk_norm_rope_kv_write")
 
 

@@ -1,6 +1,6 @@
 // Host-side runtime, in C++ behind a C interface.  The paged cache's books: page pools with ownership checks, block
-// tables for every layer group, request slots, window release, rewind and a full audit; and, at the end, the choice
-// between two matrix products.  Nothing here touches the GPU; the Python classes in hk_b200/cache/pages.py are thin views of these objects (tables and lengths are
+// tables for every layer group, request slots, window release, rewind, forks that share pages until one of their holders writes, and a
+// full audit; and, at the end, the choice between two matrix products.  Nothing here touches the GPU; the Python classes in hk_b200/cache/pages.py are thin views of these objects (tables and lengths are
 // read in place through numpy).
 //
 // Every call that can fail returns a negative code and leaves the books unchanged; hk_books_error() gives the
@@ -27,14 +27,15 @@ enum Error {
   ERR_VALUE = -5,        // an argument out of range
 };
 
-// Free list of page ids 0..n-1 with ownership checks; the page freed last is reused first.
+// Free list of page ids 0..n-1 with ownership checks and a count of each page's holders; the page freed last is reused first.
 struct Pool {
   int n = 0;
   std::vector<int> free_list;
   std::vector<uint8_t> held;
+  std::vector<int32_t> holders;     // 0 exactly where held is 0
   std::string error;
 
-  explicit Pool(int num_pages) : n(num_pages), held((size_t)num_pages, 0) {
+  explicit Pool(int num_pages) : n(num_pages), held((size_t)num_pages, 0), holders((size_t)num_pages, 0) {
     free_list.reserve((size_t)num_pages);
     for (int p = num_pages - 1; p >= 0; --p) free_list.push_back(p);     // take() gives 0 first
   }
@@ -50,13 +51,16 @@ struct Pool {
     }
     free_list.pop_back();
     held[(size_t)p] = 1;
+    holders[(size_t)p] = 1;
     return p;
   }
+  void share(int p) { ++holders[(size_t)p]; }      // one more holder of a held page
   int give(int p) {
     if (p < 0 || p >= n || !held[(size_t)p]) {
       error = "page " + std::to_string(p) + " is given back but not held";
       return ERR_CACHE;
     }
+    if (--holders[(size_t)p] > 0) return 0;
     held[(size_t)p] = 0;
     free_list.push_back(p);
     return 0;
@@ -74,7 +78,13 @@ struct Group {
         n_pages((size_t)max_requests, 0) {}
 };
 
+// A page that a request is about to write while others hold it too: its first `rows` rows are to be copied to a page of the request's own.
+struct PageCopy {
+  int group, from, to, rows;
+};
+
 struct Books {
+  std::vector<PageCopy> copies;     // owed by extend(), in order, until they are fetched
   int page_tokens, max_requests, max_context, max_pages;
   std::vector<Group> groups;
   std::vector<int> free_slots;
@@ -96,6 +106,14 @@ struct Books {
     if (g.window < 0) return g.first_page[(size_t)slot];
     const int64_t first_needed = std::max<int64_t>(0, cur - g.window + 1) / page_tokens;
     return (int)std::max<int64_t>(g.first_page[(size_t)slot], std::min<int64_t>(first_needed, g.n_pages[(size_t)slot]));
+  }
+
+  // Whether the next token of `slot` goes to a page of group g that others hold too.
+  bool writes_shared(Group& g, int slot) {
+    const int64_t cur = length[(size_t)slot];
+    if (cur % page_tokens == 0) return false;
+    const int p = entry(g, slot, (int)(cur / page_tokens));
+    return p >= 0 && g.pool.holders[(size_t)p] > 1;
   }
 
   int release_passed(int slot) {
@@ -189,12 +207,15 @@ HK_API int hk_books_close(void* h, int slot) {
 // Gives back the pages of `slot` that its windows have passed; returns how many.
 HK_API int hk_books_release_passed(void* h, int slot) { return static_cast<Books*>(h)->release_passed(slot); }
 
-// For each group: the pages hk_books_release_passed(slot) would give back now.
+// For each group: the pages hk_books_release_passed(slot) would give back to the pool now.
 HK_API int hk_books_pages_passed(void* h, int slot, int* out) {
   Books& b = *static_cast<Books*>(h);
   if (!b.is_live(slot)) return b.fail(ERR_CACHE, "slot " + std::to_string(slot) + " is not live");
-  for (size_t g = 0; g < b.groups.size(); ++g)
-    out[g] = b.passed_end(b.groups[g], slot, b.length[(size_t)slot]) - b.groups[g].first_page[(size_t)slot];
+  for (size_t g = 0; g < b.groups.size(); ++g) {
+    out[g] = 0;
+    for (int i = b.groups[g].first_page[(size_t)slot], end = b.passed_end(b.groups[g], slot, b.length[(size_t)slot]); i < end; ++i)
+      out[g] += b.groups[g].pool.holders[(size_t)b.entry(b.groups[g], slot, i)] == 1 ? 1 : 0;      // others may hold a page still
+  }
   return 0;
 }
 
@@ -203,7 +224,8 @@ HK_API int hk_books_pages_to_take(void* h, int slot, int n_new, int* out) {
   Books& b = *static_cast<Books*>(h);
   if (!b.is_live(slot)) return b.fail(ERR_CACHE, "slot " + std::to_string(slot) + " is not live");
   const int want = b.pages_for(b.length[(size_t)slot] + n_new);
-  for (size_t g = 0; g < b.groups.size(); ++g) out[g] = std::max(0, want - b.groups[g].n_pages[(size_t)slot]);
+  for (size_t g = 0; g < b.groups.size(); ++g)
+    out[g] = std::max(0, want - b.groups[g].n_pages[(size_t)slot]) + (n_new > 0 && b.writes_shared(b.groups[g], slot) ? 1 : 0);
   return 0;
 }
 
@@ -212,8 +234,56 @@ HK_API void hk_books_free_pages(void* h, int* out) {
   for (size_t g = 0; g < b.groups.size(); ++g) out[g] = (int)b.groups[g].pool.free_list.size();
 }
 
+// For each group: the page that the next token of `slot` would be written to while others hold it too, or -1; and how many hold it.
+HK_API int hk_books_shared_page(void* h, int slot, int* pages, int* holders) {
+  Books& b = *static_cast<Books*>(h);
+  if (!b.is_live(slot)) return b.fail(ERR_CACHE, "slot " + std::to_string(slot) + " is not live");
+  for (size_t g = 0; g < b.groups.size(); ++g) {
+    const bool shared = b.writes_shared(b.groups[g], slot);
+    pages[g] = shared ? b.entry(b.groups[g], slot, (int)(b.length[(size_t)slot] / b.page_tokens)) : -1;
+    holders[g] = shared ? b.groups[g].pool.holders[(size_t)pages[g]] : 0;
+  }
+  return 0;
+}
+
+// A new slot with the tokens of `slot`: it shares all of its pages.
+HK_API int hk_books_fork(void* h, int slot) {
+  Books& b = *static_cast<Books*>(h);
+  if (!b.is_live(slot)) return b.fail(ERR_CACHE, "slot " + std::to_string(slot) + " is not live");
+  if (b.free_slots.empty()) return b.fail(ERR_TOO_MANY_REQUESTS, "all " + std::to_string(b.max_requests) + " request slots are in use");
+  const int s = b.free_slots.back();
+  b.free_slots.pop_back();
+  b.live[(size_t)s] = 1;
+  b.length[(size_t)s] = b.length[(size_t)slot];
+  for (Group& g : b.groups) {
+    g.first_page[(size_t)s] = g.first_page[(size_t)slot];
+    g.n_pages[(size_t)s] = g.n_pages[(size_t)slot];
+    for (int i = g.first_page[(size_t)s]; i < g.n_pages[(size_t)s]; ++i) {
+      const int p = b.entry(g, slot, i);
+      b.entry(g, s, i) = p;
+      if (p >= 0) g.pool.share(p);
+    }
+  }
+  return s;
+}
+
+// The copies that extend() owes, as records of 4 ints {group, from, to, rows}: writes at most `most` of them to `out` (null: none) and
+// forgets those; returns how many there are (null) or were written.
+HK_API int hk_books_copies(void* h, int* out, int most) {
+  Books& b = *static_cast<Books*>(h);
+  if (out == nullptr) return (int)b.copies.size();
+  const int n = std::min(most, (int)b.copies.size());
+  for (int i = 0; i < n; ++i) {
+    const PageCopy& c = b.copies[(size_t)i];
+    out[4 * i] = c.group, out[4 * i + 1] = c.from, out[4 * i + 2] = c.to, out[4 * i + 3] = c.rows;
+  }
+  b.copies.erase(b.copies.begin(), b.copies.begin() + n);
+  return n;
+}
+
 // Makes room for n_new more tokens of `slot`: gives back pages the window has passed, then takes the pages the
-// new positions need - all of them or none.  Returns how many table entries changed.
+// new positions need, and one in the place of a page that it would write while others hold it (the copy is owed: hk_books_copies) - all
+// of them or none.  Returns how many table entries changed.
 HK_API int hk_books_extend(void* h, int slot, int n_new) {
   Books& b = *static_cast<Books*>(h);
   if (!b.is_live(slot)) return b.fail(ERR_CACHE, "slot " + std::to_string(slot) + " is not live");
@@ -225,14 +295,25 @@ HK_API int hk_books_extend(void* h, int slot, int n_new) {
   // what the window would give back counts as free for this check, but nothing is touched before the check passes
   const int want = b.pages_for(cur + n_new);
   for (Group& g : b.groups) {
-    const int k = std::max(0, want - g.n_pages[(size_t)slot]);
-    const int back = b.passed_end(g, slot, cur) - g.first_page[(size_t)slot];
+    const int k = std::max(0, want - g.n_pages[(size_t)slot]) + (b.writes_shared(g, slot) ? 1 : 0);
+    int back = 0;                                        // passed pages that nobody else holds
+    for (int i = g.first_page[(size_t)slot], end = b.passed_end(g, slot, cur); i < end; ++i)
+      back += g.pool.holders[(size_t)b.entry(g, slot, i)] == 1 ? 1 : 0;
     if (k > (int)g.pool.free_list.size() + back)
       return b.fail(ERR_OUT_OF_PAGES, std::to_string(k) + " pages needed, " + std::to_string((int)g.pool.free_list.size() + back) + " free");
   }
   int changed = b.release_passed(slot);
   if (changed < 0) return changed;
   for (Group& g : b.groups) {
+    if (b.writes_shared(g, slot)) {
+      const int p = g.pool.take();
+      if (p < 0) return b.fail(p, g.pool.error);         // cannot happen after the check above
+      int32_t& at = b.entry(g, slot, (int)(cur / b.page_tokens));
+      b.copies.push_back({(int)(&g - b.groups.data()), at, p, (int)(cur % b.page_tokens)});
+      g.pool.give(at);                                   // others hold it still
+      at = p;
+      ++changed;
+    }
     for (int i = g.n_pages[(size_t)slot]; i < want; ++i) {
       const int p = g.pool.take();
       if (p < 0) return b.fail(p, g.pool.error);         // cannot happen after the check above
@@ -273,14 +354,16 @@ HK_API int hk_books_audit(void* h) {
   Books& b = *static_cast<Books*>(h);
   for (size_t gi = 0; gi < b.groups.size(); ++gi) {
     Group& g = b.groups[gi];
-    std::map<int, std::pair<int, int>> seen;
+    std::map<int, std::pair<int, int>> seen;      // page -> where it was listed last
+    std::vector<int> times((size_t)g.pool.n, 0);
     for (int s = 0; s < b.max_requests; ++s) {
       for (int i = 0; i < b.max_pages; ++i) {
         const int p = b.entry(g, s, i);
         if (p < 0) continue;
         if (!b.live[(size_t)s]) return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": dead slot " + std::to_string(s) + " still lists pages");
+        if (p >= g.pool.n) return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": slot " + std::to_string(s) + " lists page " + std::to_string(p) + ", which there is not");
         auto it = seen.find(p);
-        if (it != seen.end())
+        if (++times[(size_t)p] > std::max(1, (int)g.pool.holders[(size_t)p]))
           return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": page " + std::to_string(p) + " is held twice ((" +
                                        std::to_string(it->second.first) + ", " + std::to_string(it->second.second) + ") and (" +
                                        std::to_string(s) + ", " + std::to_string(i) + "))");
@@ -292,6 +375,9 @@ HK_API int hk_books_audit(void* h) {
       const bool listed = seen.count(p) != 0;
       if (g.pool.held[(size_t)p] && !listed) return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": the pool holds page " + std::to_string(p) + " that no table lists");
       if (!g.pool.held[(size_t)p] && listed) return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": a table lists page " + std::to_string(p) + " that the pool does not hold");
+      if (g.pool.held[(size_t)p] && times[(size_t)p] != g.pool.holders[(size_t)p])
+        return b.fail(ERR_CACHE, "group " + std::to_string(gi) + ": page " + std::to_string(p) + " has " + std::to_string(g.pool.holders[(size_t)p]) +
+                                     " holders, but tables list it " + std::to_string(times[(size_t)p]) + " times");
       held += g.pool.held[(size_t)p];
     }
     if (held + (int)g.pool.free_list.size() != g.pool.n)

@@ -15,6 +15,38 @@ ALIGN = 8        # int32 elements: every packed array starts on a 32-byte bounda
 
 
 @dataclass
+class TreeStep:
+    """What a step of drafted token trees brings beside the rows (`ops.tree_attention`): requests int32 [m, 4] = (slot, first row,
+    tokens, cached rows before them), ancestors int32 [n, words], rows int32 [n] (each token's row in its request's cache), and
+    bounds on a request's tokens and rows, with the rows of all together."""
+    requests: torch.Tensor
+    ancestors: torch.Tensor
+    rows: torch.Tensor
+    most_tokens: int
+    most_keys: int
+    all_keys: int
+
+
+def pack_trees(slots, q_starts, q_lens, start_positions, parents) -> Tuple[np.ndarray, np.ndarray, int]:
+    """(requests | ancestors | rows as one int32 array, depth int32 [n] of every token in its tree, words).  `parents`: per request the
+    parent of each of its tokens among them, -1 for a root, or None for tokens that follow one another."""
+    n, m = sum(q_lens), len(slots)
+    words = -(-max(q_lens) // 32)
+    requests = np.array([slots, q_starts, q_lens, start_positions], dtype=np.int32).T
+    bits = np.zeros((n, words), dtype=np.uint32)
+    rows, depth = np.empty(n, dtype=np.int32), np.zeros(n, dtype=np.int32)
+    for q0, count, start, tree in zip(q_starts, q_lens, start_positions, parents):
+        rows[q0:q0 + count] = np.arange(start, start + count, dtype=np.int32)
+        for i in range(count):
+            p = i - 1 if tree is None else int(tree[i])
+            if p >= 0:
+                bits[q0 + i] = bits[q0 + p]
+                depth[q0 + i] = depth[q0 + p] + 1
+            bits[q0 + i, i // 32] |= np.uint32(1 << (i % 32))
+    return np.concatenate([requests.reshape(-1), bits.view(np.int32).reshape(-1), rows]), depth, words
+
+
+@dataclass
 class StepContext:
     """One step's batch, flattened.  Row t is a token; rows of one request are consecutive and
     in increasing position (the reference's rule for items that share a cache:
@@ -40,6 +72,7 @@ class StepContext:
     fixed_shape: bool = False
     max_context: int = 0
     page_tokens: int = 0        # tokens per cache page (0: not said); a part may cut its work to fit the pages
+    trees: Optional[TreeStep] = None   # this step's rows are drafted trees
     residual_narrow: Optional[torch.Tensor] = None   # the residual stream rounded to the compute type, while a layer keeps it up
 
 

@@ -24,7 +24,7 @@ from ..cache.pages import CacheError, ContextFull, OutOfPages
 from ..config import ModelConfig, load_config, resolve_architecture
 from ..parts.base import Precision
 from ..weights.loader import load_tensors, random_tensors
-from .context import StepContext, bind_step, pack_step, table_parts
+from .context import StepContext, TreeStep, bind_step, pack_step, pack_trees, table_parts
 
 
 class EngineError(RuntimeError):
@@ -62,10 +62,14 @@ class DeviceToken:
 @dataclass
 class StepEntry:
     """A request's share of a step: its next tokens and the places among them (indices into
-    `tokens`) whose logits are wanted.  `tokens` is a sequence of ids, or one `DeviceToken`."""
+    `tokens`) whose logits are wanted.  `tokens` is a sequence of ids, or one `DeviceToken`.
+    `parents` makes them a tree of drafted continuations: the parent of each token is an earlier one of them (its index), or -1: the
+    token follows the request's last one.  A token then sees the request's tokens and its own ancestors, and stands one position
+    behind its parent.  Behind such a step the request waits for `Engine.accept`."""
     request: Hashable
     tokens: object
     want: Sequence[int] = ()
+    parents: Optional[Sequence[int]] = None
 
 
 _DTYPES = {
@@ -142,6 +146,16 @@ class PinnedStager:
         return dev.view(arr.shape)
 
 
+def model_takes_trees(model) -> bool:
+    """Whether every mixer of the model is right for a step of drafted trees."""
+    from ..parts.base import mixer_classes
+    mixers = mixer_classes()
+
+    def takes(part) -> bool:
+        return (part.takes_trees or not isinstance(part, mixers)) and all(takes(c) for c in part.children())
+    return takes(model)
+
+
 class Engine:
     """A model bound to `cuda:device`, with a page pool for `max_tokens` cached tokens."""
 
@@ -190,6 +204,8 @@ class Engine:
                                 max_requests, self.max_context)
         self.vocab = self.model.vocab
         self._requests: Dict[Hashable, int] = {}
+        self._trees: Dict[int, tuple] = {}     # slot -> (rows before a drafted tree, its parents) until `accept`
+        self.takes_trees = model_takes_trees(self.model) and not self.cache.has_state()
         self.steps_run = 0
         self.stager = PinnedStager(self.device)
         # the word that a timed-out barrier wait inside a tensor-core kernel sets; its value travels to pinned
@@ -218,7 +234,62 @@ class Engine:
         slot = self._requests.pop(request, None)
         if slot is None:
             raise UnknownRequest(f"request {request!r} is not open")
+        self._trees.pop(slot, None)
         self.cache.close(slot)
+
+    # -- several continuations of one request ---------------------------------------------------
+    def fork_request(self, request: Hashable, new_request: Hashable) -> None:
+        """Opens `new_request` with the tokens of `request` in its cache: pages are shared until one of the two writes them, states
+        are copied."""
+        slot = self._settled_slot(request)
+        if new_request in self._requests:
+            raise EngineError(f"request {new_request!r} is already open")
+        self._requests[new_request] = self.cache.fork([slot])[0]
+
+    def reorder(self, requests: Sequence[Hashable], parents: Sequence[int]) -> None:
+        """Request i of `requests` goes on with the tokens of request parents[i] of them (beams after a choice).  What no request goes
+        on with is given up; what one does stays where it is, further ones are forks of it."""
+        if len(set(requests)) != len(requests) or len(parents) != len(requests) or any(not 0 <= int(p) < len(requests) for p in parents):
+            raise EngineError("reorder needs one parent, an index into the requests, for each of different requests")
+        slots = [self._settled_slot(r) for r in requests]
+        parents = [int(p) for p in parents]
+        now, first = [None] * len(slots), {}
+        for i in [i for i, p in enumerate(parents) if i == p] + list(range(len(slots))):       # a request that goes on with its own keeps it
+            if parents[i] not in first:
+                first[parents[i]] = i
+                now[i] = slots[parents[i]]
+        for p, s in enumerate(slots):
+            if p not in first:
+                self.cache.close(s)
+        rest = [i for i in range(len(slots)) if now[i] is None]
+        for i, s in zip(rest, self.cache.fork([slots[parents[i]] for i in rest])):
+            now[i] = s
+        for r, s in zip(requests, now):
+            self._requests[r] = s
+
+    def accept(self, accepted: Dict[Hashable, Sequence[int]]) -> None:
+        """Ends the steps of drafted trees: of request r's tree the tokens accepted[r] (indices, from a root on, each a child of the one
+        before) stay, in this order, and the others are forgotten."""
+        plan = []
+        for r, kept in accepted.items():
+            slot = self.slot_of(r)
+            if slot not in self._trees:
+                raise EngineError(f"request {r!r} has no drafted tree")
+            first, parents = self._trees[slot]
+            kept = [int(i) for i in kept]
+            if not kept or any(not 0 <= i < len(parents) for i in kept) or [parents[i] for i in kept] != [-1] + kept[:-1]:
+                raise EngineError(f"{kept} is no path through the tree of request {r!r}")
+            plan.append((slot, first, kept))
+        self.cache.keep(plan)
+        for slot, first, kept in plan:
+            self.cache.books.truncate(slot, first + len(kept))
+            del self._trees[slot]
+
+    def _settled_slot(self, request: Hashable) -> int:
+        slot = self.slot_of(request)
+        if slot in self._trees:
+            raise EngineError(f"request {request!r} has a drafted tree that waits for accept")
+        return slot
 
     def has_request(self, request: Hashable) -> bool:
         return request in self._requests
@@ -243,14 +314,24 @@ class Engine:
         total = 0
         seen = set()
         take = [0] * len(books.groups)
+        shared: Dict[tuple, list] = {}         # (group, page) that several hold -> [writers in this step, holders]
+        trees = any(e.parents is not None for e in entries)
+        if trees and not self.takes_trees:
+            raise EngineError("this model does not take trees of drafted tokens (a mixer keeps a state, or an attention that knows no trees)")
         for e in entries:
-            slot = self.slot_of(e.request)
+            slot = self._settled_slot(e.request)
             if e.request in seen:
                 raise EngineError(f"request {e.request!r} appears twice in one step")
             seen.add(e.request)
             n = len(e.tokens)
             if n < 1:
                 raise EngineError(f"request {e.request!r} brings no tokens")
+            if trees:
+                from ..csrc.ops import TREE_TOKENS
+                if isinstance(e.tokens, DeviceToken) or n > TREE_TOKENS:
+                    raise EngineError(f"a step with drafted trees takes up to {TREE_TOKENS} tokens a request, known to the host")
+                if e.parents is not None and (len(e.parents) != n or any(not -1 <= int(p) < i for i, p in enumerate(e.parents))):
+                    raise EngineError(f"the parents of request {e.request!r}'s tokens must be earlier ones of them, or -1")
             if not isinstance(e.tokens, DeviceToken):       # a sampler's output is inside the vocabulary
                 for tok in e.tokens:
                     if not 0 <= int(tok) < self.vocab:
@@ -266,6 +347,12 @@ class Engine:
             passed = books.pages_passed(slot)
             for gi, k in enumerate(books.pages_to_take(slot, n)):
                 take[gi] += k - passed[gi]
+            for gi, (page, holders) in enumerate(books.shared_pages(slot)):
+                if page >= 0:
+                    shared.setdefault((gi, page), [0, holders])[0] += 1
+        for (gi, _), (writers, holders) in shared.items():
+            if writers == holders:             # the last of a page's holders writes it where it is
+                take[gi] -= 1
         if total > self.max_batch_tokens:
             raise BatchTooLarge(f"{total} tokens in one step; the engine takes {self.max_batch_tokens}")
         for gi, k in enumerate(take):
@@ -315,6 +402,7 @@ class Engine:
             books.extend(s, len(e.tokens))
         self.cache.sync_tables()
 
+        trees = any(e.parents is not None for e in entries)
         n = sum(len(e.tokens) for e in entries)
         meta = np.empty((3, n), dtype=np.int32)
         q_starts, q_lens, rows = [], [], []
@@ -333,7 +421,7 @@ class Engine:
             q_starts.append(r)
             q_lens.append(m)
             r += m
-        if self.decode_graphs and n == len(entries) and all(list(e.want) == [0] for e in entries):
+        if not trees and self.decode_graphs and n == len(entries) and all(list(e.want) == [0] for e in entries):
             from .graphs import DecodeGraph, graph_batch
             # a graph per batch size would be captured again whenever a request comes or goes; sizes above 8 are
             # rounded up to the next multiple of 8 and the batch is filled with repeats of its last row (the same
@@ -352,7 +440,17 @@ class Engine:
             return g.run(meta, slots, starts, on_device, n)
         ctx = StepContext(self.precision, n, None, None, None, slots, q_starts, q_lens, starts,
                           max_context=self.max_context, page_tokens=self.cache.page_tokens)
-        packed = pack_step(meta, ctx, self._table_parts)
+        if trees:
+            packed_trees, depth, words = pack_trees(slots, q_starts, q_lens, starts, [e.parents for e in entries])
+            meta[1] = np.repeat(np.asarray(starts, dtype=np.int32), q_lens) + depth
+            dev = self.stager.upload(packed_trees)
+            m = 4 * len(slots)
+            ctx.trees = TreeStep(dev[:m].view(-1, 4), dev[m:m + n * words].view(n, words), dev[m + n * words:], max(q_lens),
+                                 max(st + q for st, q in zip(starts, q_lens)), sum(starts) + n)
+            for s, st, e in zip(slots, starts, entries):
+                if e.parents is not None:
+                    self._trees[s] = (st, [int(p) for p in e.parents])
+        packed = pack_step(meta, ctx, () if trees else self._table_parts)
         bind_step(ctx, packed, self.stager.upload(packed.host))
         fill_device_tokens(ctx.token_ids, on_device)
         x = self.model.forward(ctx, self.cache.layers)

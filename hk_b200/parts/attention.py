@@ -209,6 +209,12 @@ class GQAAttention(Part):
         self._sm_count = 0
 
     # -- declaration ---------------------------------------------------------------------
+    @property
+    def takes_trees(self) -> bool:
+        """Drafted trees: every option but those that look at a key's distance or block, norms over whole projections and values of
+        another width than the keys."""
+        return not self.chunk and self.bias_max is None and not self.qk_norm_rows and self.vd == self.hd
+
     def kernel_libraries(self, bfloat16: bool):
         """The flash kernels are compiled only for a model one of whose attention parts can use them."""
         from ..csrc import attention_fast
@@ -347,8 +353,17 @@ class GQAAttention(Part):
                 qkv, q, self.q_norm, self.k_norm, self.qk_norm_eps or 0.0, cos, sin, rot, ctx.positions,
                 ctx.slot_of_token, cache.block_table, cache.k_pages, cache.v_pages, H, G, hd, cache.page_tokens,
                 write_kv=write_cache, bias=self.b_qkv, pairing=pairing, norm_after=self.qk_norm_after,
-                tied_v=self.value_from_key, q_factor=self.q_factor)
+                tied_v=self.value_from_key, q_factor=self.q_factor, rows=ctx.trees.rows if ctx.trees is not None else None)
         att = torch.empty((n, H * self.vd), dtype=xb.dtype, device=xb.device)
+        if ctx.trees is not None:
+            t = ctx.trees
+            ops.tree_attention(q, cache.k_pages, cache.v_pages, cache.block_table, t.requests, t.ancestors, ctx.positions, att, H, G, hd,
+                               cache.page_tokens, self.window or 0, self.scale, t.most_tokens, t.most_keys, all_keys=t.all_keys,
+                               sink=self.sink, sinks=self.sinks, softcap=self.softcap)
+            if gate is not None:
+                ops.sigmoid_gate(att, gate, att, self.out_scale)
+            ops.gemm(att, self.w_o, residual, accumulate=accumulate, bias=self.b_o if add_bias else None)
+            return
         ops.paged_attention(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.positions, ctx.slot_of_token,
                             att, H, G, hd, cache.page_tokens, self.window or 0, self.scale,
                             plan=plan, sink=self.sink, sinks=self.sinks, softcap=self.softcap, chunk=self.chunk, gate=gate,

@@ -133,6 +133,9 @@ class Part:
     and value again changes nothing, advancing a state again does."""
 
     graph_safe = False
+    # A mixer whose `forward` is right for a step of drafted trees (`ctx.trees`): rows that branch, whose place in the cache is not
+    # their position.  Looked at for mixers alone: other parts take rows one by one.
+    takes_trees = False
 
     def children(self) -> Iterable["Part"]:
         return ()
@@ -185,3 +188,8 @@ def part_class(kind: str, name: str) -> type:
         return _KINDS[kind][name]
     except KeyError:
         raise KeyError(f"no {kind} part named '{name}' (registered: {', '.join(sorted(_KINDS.get(kind, {})))})") from None
+
+
+def mixer_classes() -> tuple:
+    """Every class that is registered as a mixer."""
+    return tuple(set(_KINDS["mixer"].values()))
