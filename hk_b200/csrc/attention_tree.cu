@@ -478,9 +478,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"      // sleeps until the phase comes, or some 100 us
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(100000u) : "memory");
   return ok != 0;
 }
 // Waits for the phase of this parity, a bounded time; false (and the flag set) if it did not come or another gave up.  (Without sleeps
@@ -488,10 +488,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long start = clock64();
-  for (uint32_t i = 1;; ++i) {
+  while (!*abort_flag && clock64() - start < WAIT_CLOCKS)
     if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 0u && (*abort_flag || clock64() - start > WAIT_CLOCKS)) break;
-  }
   *abort_flag = 1;
   return false;
 }
@@ -604,8 +602,10 @@ struct TcSmem {
                                                             // [tile % 4]..: the reference asked for
   float2 ml[2][2][TC_ROWS];   // the reference and the sum
   Walk start;                 // the share behind its first segment
-  Segment segment;
-  int any;
+  Segment lead;               // its first segment, if it has any
+  int led;
+  Segment segment[3];         // the softmax warps' segments: the last one (until its results are out), the one in hand, the next one
+  int any[3];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -722,8 +722,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const bool any = next_segment<TcCut>(a, w, s);
     if (lane == 0) {
       sm.start = w;
-      sm.segment = s;
-      sm.any = any;
+      sm.lead = sm.segment[0] = s;
+      sm.led = any;
     }
   }
   tc_fence_before();
@@ -731,8 +731,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   Walk w = sm.start;
-  Segment s = sm.segment;
-  bool more = sm.any != 0;
+  Segment s = sm.lead;
+  bool more = sm.led != 0;
 
   if (warp >= LOAD_WARP) {
     // ================================================================= loads (a lane per box of a page's keys and half of the head)
@@ -872,13 +872,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       for (int c = c_from; c < c_to; ++c) cp_async16(qs + swz(r, c), src + c * 8, row < u.rows);
       cp_async_commit();
     };
-    Segment ahead = s;
-    if (more) send_q(ahead);
-    while (ok && more) {
-      s = ahead;
+    // (the segment stays in shared memory, and the next one is found by one thread: registers are what these threads are short of, and
+    // what they would spill comes back late)
+    if (more) send_q(sm.segment[0]);
+    for (int at = 0, next = 1; ok && more; at = next, next = next == 2 ? 0 : next + 1) {
+      const Segment& s = sm.segment[at];
+      if (threadIdx.x == 0) sm.any[next] = next_segment<TcCut>(a, w, sm.segment[next]);
       const bool two = s.rows > TC_ROWS;
       const int row = two ? x * TC_ROWS + r : r;
       const bool valid = row < s.rows, busy = row - lane < s.rows;        // busy: any row of the warp is one
+      const int t0 = s.t0, context = s.q.context;
       const int token = valid ? token_of(a, s.row0 + row) : 0;
       const int lo = valid ? tree_row(a, s.q, token, true).lo : 0;
       cp_async_wait<0>();
@@ -893,8 +896,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           if (lane == 0) mbar_arrive(&sm.p_full[x][half]);
           continue;
         }
-        const int j0 = (s.t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
-        const bool part = j0 < lo || j0 + HK > s.q.context;
+        const int j0 = (t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
+        const bool part = j0 < lo || j0 + HK > context;
         uint32_t see[2] = {0xffffffffu, 0xffffffffu}, su[32];
         if (part) {
           const TreeRow tr = tree_row(a, s.q, token, valid);
@@ -1007,8 +1010,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       ok = !softmax_any(!ok);
       if (!ok) break;
       tc_fence_after();
-      more = next_segment<TcCut>(a, w, ahead);
-      if (more) send_q(ahead);                         // both groups' scores are through: Q is free
+      more = sm.any[next] != 0;
+      if (more) send_q(sm.segment[next]);              // both groups' scores are through: Q is free
       if (busy) {
         float f[2] = {1.0f, 1.0f}, l;
         if (two) {
@@ -1072,21 +1075,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         for (unsigned again = __ballot_sync(0xffffffffu, valid && odd != 0.f); again; again &= again - 1) {
           const Segment unit = s;
           __syncwarp();
-          const int from = __ffs(again) - 1, at = row - lane + from;
+          const int from = __ffs(again) - 1, odd_row = row - lane + from;
           float m_row = __shfl_sync(0xffffffffu, m, from), l_row = __shfl_sync(0xffffffffu, l, from), inv_row = __shfl_sync(0xffffffffu, inv, from);
           bf16* op_row = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)op, from));
           const int head_row = __shfl_sync(0xffffffffu, head, from);
           if (!(l_row <= CUDART_MAX_NORMAL_F)) {        // the reference and the sum as well
-            tree_row_top(a, unit, at, cap_log2, cap_in2, m_row, l_row);
+            tree_row_top(a, unit, odd_row, cap_log2, cap_in2, m_row, l_row);
             if (s.whole) inv_row = finish(m_row, l_row, head_row);
-            else if (lane == 0 && half == 0 && (two || x == 0)) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + at) = make_float2(m_row, l_row);
+            else if (lane == 0 && half == 0 && (two || x == 0)) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + odd_row) = make_float2(m_row, l_row);
           }
           for (int c0 = c_from; c0 < c_to; c0 += 32) {
             const int dim = c0 + lane;
-            const float y = tree_row_again(a, unit, at, min(dim, HD - 1), m_row, cap_log2, cap_in2);
+            const float y = tree_row_again(a, unit, odd_row, min(dim, HD - 1), m_row, cap_log2, cap_in2);
             if (dim < c_to) {
               if (s.whole) op_row[dim] = __float2bfloat16_rn(y * inv_row);
-              else part_place(a, slot, at, dim, HD)[dim & 3] = y;
+              else part_place(a, slot, odd_row, dim, HD)[dim & 3] = y;
             }
           }
         }

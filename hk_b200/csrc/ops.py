@@ -1534,6 +1534,65 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
     request's cached rows).  A token that sees nothing gives zeros; rows of no request keep what they hold.  sink, sinks, softcap
     as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them: one beyond them is left out;
     all_keys: the rows of all requests together, where the caller knows it (0: as if all had the most)."""
+    H, G, hd = n_heads, n_kv_heads, head_dim
+    # The usual call in one condition (a call of one user's tree costs the host as much as the GPU); what it does not let through goes
+    # through the checks one by one, for their messages.
+    dtype, i32, dev = q.dtype, torch.int32, q.get_device()
+    try:
+        (n, width), shape, (m, four), (marks, words) = q.shape, k_pages.shape, requests.shape, ancestors.shape
+        (table_rows, stride), (pages, _, _, _) = block_table.shape, shape
+    except ValueError:
+        _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, scale, most_tokens, most_keys,
+                     all_keys, sink, sinks, softcap)
+        raise
+    if not (dev >= 0 and out.dtype is dtype and k_pages.dtype is dtype and v_pages.dtype is dtype and block_table.dtype is i32
+            and requests.dtype is i32 and ancestors.dtype is i32 and positions.dtype is i32
+            and out.get_device() == dev and k_pages.get_device() == dev and v_pages.get_device() == dev and block_table.get_device() == dev
+            and requests.get_device() == dev and ancestors.get_device() == dev and positions.get_device() == dev
+            and q.is_contiguous() and out.is_contiguous() and k_pages.is_contiguous() and v_pages.is_contiguous() and block_table.is_contiguous()
+            and requests.is_contiguous() and ancestors.is_contiguous() and positions.is_contiguous()
+            and H >= 1 and G >= 1 and H % G == 0 and 1 <= hd <= 256 and width == H * hd and out.shape == q.shape
+            and shape == (pages, G, page_tokens, hd) and v_pages.shape == shape and four == 4 and marks == n and positions.shape == (n,)
+            and 1 <= most_tokens <= TREE_TOKENS and most_tokens <= 32 * words and 1 <= most_keys <= stride * page_tokens and all_keys >= 0
+            and scale > 0 and softcap >= 0 and sinks is None and (dtype is torch.float32 or dtype is torch.bfloat16)):
+        _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, scale, most_tokens, most_keys,
+                     all_keys, sink, sinks, softcap)
+    if n == 0 or m == 0:
+        return
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, window, scale,
+                                  most_tokens, most_keys, all_keys, sink, sinks, softcap)
+    lib, choice, wide = build.load("attention_tree"), _forced["attention"], dtype is torch.float32
+    args = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), F32 if wide else BF16, block_table.data_ptr(), table_rows, stride,
+            requests.data_ptr(), m, most_tokens, most_keys, ancestors.data_ptr(), words, positions.data_ptr(), n, pages, page_tokens, H, G, hd,
+            window, scale, softcap, 1 if sink else 0, _ptr(sinks))
+    if (hd == 128 or hd == 64) and choice != "generic":
+        rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
+        # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor
+        # cores of two: one for either group of warps
+        held = all_keys if all_keys > 0 else m * most_keys
+        if window > 0:
+            held = min(held, m * (window + most_tokens))
+        tall = most_tokens * (H // G)
+        tiles = -(-tall // rows) * G * (held // keys + m)
+        sms = gemm_fast._sms(q.device)
+        ctas = max(1, min(sms * 2, tiles) if wide else min(sms, (tiles + 1) // 2))
+        cap = min(rows, tall)
+        part = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
+        at = part.data_ptr()
+        code = lib.hk_tree_attention(*args, 1, ctas, at, at + 8 * ctas * cap * hd, cap, 0 if wide else gemm_fast.status_flag(q.device).data_ptr(),
+                                     torch._C._cuda_getCurrentRawStream(dev))
+        if code != _ERR_UNSUPPORTED:
+            return _check(code, "tree_attention", 2 if ctas > 1 else 1)
+    if choice not in (None, "generic"):
+        raise KernelError(f"tree_attention: the '{choice}' kernel refuses head_dim={hd} page_tokens={page_tokens}")
+    _check(lib.hk_tree_attention(*args, 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
+
+
+def _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, scale, most_tokens, most_keys,
+                 all_keys, sink, sinks, softcap) -> None:
+    _dt(q)
     _need(q, "q", dims=2)
     _need(out, "out", q.dtype, 2)
     _need(k_pages, "k_pages", q.dtype, 4)
@@ -1542,15 +1601,15 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
     _need(requests, "requests", torch.int32, 2)
     _need(ancestors, "ancestors", torch.int32, 2)
     _need(positions, "positions", torch.int32, 1)
-    n, H, G, hd = q.shape[0], n_heads, n_kv_heads, head_dim
+    n = q.shape[0]
     if H < 1 or G < 1 or H % G != 0:
         raise KernelError(f"tree_attention: {H} heads are not a multiple of {G} groups")
     if tuple(q.shape) != (n, H * hd) or out.shape != q.shape:
         raise KernelError("tree_attention: q and out must be [n, H*head_dim]")
     if tuple(k_pages.shape[1:]) != (G, page_tokens, hd) or v_pages.shape != k_pages.shape:
         raise KernelError("tree_attention: cache pages must be [pages, G, page_tokens, head_dim]")
-    if hd > 256:
-        raise KernelError(f"tree_attention: head_dim {hd} is above 256")
+    if not 1 <= hd <= 256:
+        raise KernelError(f"tree_attention: head_dim {hd} is outside 1..256")
     if requests.shape[1] != 4 or ancestors.shape[0] != n or positions.shape[0] != n:
         raise KernelError("tree_attention: requests must be [m, 4], ancestors [n, words] and positions [n]")
     if not 1 <= most_tokens <= TREE_TOKENS or most_tokens > 32 * ancestors.shape[1]:
@@ -1565,37 +1624,6 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
             raise KernelError("tree_attention: sinks must hold one score per query head (and sink be set)")
     if not _one_device(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, sinks):
         raise KernelError("tree_attention: all tensors must be on one device")
-    m = requests.shape[0]
-    if n == 0 or m == 0:
-        return
-    lib = build.load("attention_tree")
-    group, kernel, ctas, cap, part_o, part_ml, status = H // G, 0, 0, 0, None, None, 0
-    choice = _forced["attention"]
-    with _on(q):
-        if hd in (64, 128) and choice != "generic":
-            wide = q.dtype == torch.float32
-            rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
-            # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor
-            # cores of two: one for either group of warps
-            held = all_keys if all_keys > 0 else m * most_keys
-            if window > 0:
-                held = min(held, m * (window + most_tokens))
-            tiles = -(-most_tokens * group // rows) * G * (held // keys + m)
-            ctas = max(1, min(gemm_fast._sms(q.device) * 2, tiles) if wide else min(gemm_fast._sms(q.device), (tiles + 1) // 2))
-            cap = min(rows, most_tokens * group)
-            part_o = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
-            part_ml = part_o.data_ptr() + 8 * ctas * cap * hd
-            kernel, status = 1, 0 if wide else _ptr(gemm_fast.status_flag(q.device))
-        args = (_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _dt(q), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(requests),
-                m, most_tokens, most_keys, _ptr(ancestors), ancestors.shape[1], _ptr(positions), n, k_pages.shape[0], page_tokens, H, G, hd, window,
-                scale, softcap, 1 if sink else 0, _ptr(sinks))
-        if kernel:
-            code = lib.hk_tree_attention(*args, kernel, ctas, _ptr(part_o), part_ml, cap, status, _stream())
-            if code != _ERR_UNSUPPORTED:
-                return _check(code, "tree_attention", launches=2 if ctas > 1 else 1)
-        if choice not in (None, "generic"):
-            raise KernelError(f"tree_attention: the '{choice}' kernel refuses head_dim={hd} page_tokens={page_tokens}")
-        _check(lib.hk_tree_attention(*args, 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
 
 
 _TREE_ROWS_TC, _TREE_ROWS_F32 = 256, 32      # rows of a tile (TC_ROWS twice, F32_ROWS in csrc/attention_tree.cu)
@@ -1604,14 +1632,6 @@ _TREE_ROWS_TC, _TREE_ROWS_F32 = 256, 32      # rows of a tile (TC_ROWS twice, F3
 def _one_device(first: torch.Tensor, *others) -> bool:
     index = first.device.index
     return all(t is None or t.device.index == index for t in others)
-
-
-_here = contextlib.nullcontext()
-
-
-def _on(t: torch.Tensor):
-    """The device of `t` as the current one (a launch goes to the current device's stream)."""
-    return _here if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device.index)
 
 
 def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, table_stride: int, page_tokens: int, heads: int,
@@ -1629,9 +1649,11 @@ def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, tabl
         raise KernelError("compact_rows: the sizes must be positive")
     if not _one_device(table, paths):
         raise KernelError("compact_rows: table and paths must be on one device")
-    with _on(table):
-        _check(build.load("branches").hk_compact_rows(_ptr(table), table.shape[0], _ptr(paths), paths.shape[0], paths.shape[1] - 2, table_rows,
-                                                      table_stride, page_tokens, heads, row_bytes, num_pages, _stream()), "compact_rows")
+    if table.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(table.get_device()):
+            return compact_rows(table, paths, table_rows, table_stride, page_tokens, heads, row_bytes, num_pages)
+    _check(build.load("branches").hk_compact_rows(table.data_ptr(), table.shape[0], paths.data_ptr(), paths.shape[0], paths.shape[1] - 2, table_rows,
+                                                  table_stride, page_tokens, heads, row_bytes, num_pages, _stream()), "compact_rows")
 
 
 def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> None:
@@ -1647,8 +1669,11 @@ def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> No
         raise KernelError("copy_blocks: most_bytes must be positive")
     if not _one_device(table, moves):
         raise KernelError("copy_blocks: table and moves must be on one device")
-    with _on(table):
-        _check(build.load("branches").hk_copy_blocks(_ptr(table), table.shape[0], _ptr(moves), moves.shape[0], most_bytes, _stream()), "copy_blocks")
+    if table.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(table.get_device()):
+            return copy_blocks(table, moves, most_bytes)
+    _check(build.load("branches").hk_copy_blocks(table.data_ptr(), table.shape[0], moves.data_ptr(), moves.shape[0], most_bytes, _stream()),
+           "copy_blocks")
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_beams: torch.Tensor,
@@ -1663,23 +1688,25 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     _need(out_scores, "out_scores", torch.float32, 2)
     _need(out_beams, "out_beams", torch.int32, 2)
     _need(out_tokens, "out_tokens", torch.int32, 2)
-    rows, vocab = logits.shape
-    prompts, choices = out_scores.shape
-    if n_beams < 1 or rows != prompts * n_beams or scores.shape[0] != rows:
+    (rows, vocab), shape, dev = logits.shape, out_scores.shape, logits.get_device()
+    prompts, choices = shape
+    if n_beams < 1 or rows != prompts * n_beams or scores.shape != (rows,):
         raise KernelError(f"beam_select: {rows} rows of logits and {scores.shape[0]} scores for {prompts} prompts of {n_beams} beams")
-    if out_beams.shape != out_scores.shape or out_tokens.shape != out_scores.shape:
+    if out_beams.shape != shape or out_tokens.shape != shape:
         raise KernelError("beam_select: the three results must have one shape")
     if prompts == 0:
         return
     if n_beams > 256 or not 1 <= choices <= min(256, n_beams * vocab) or n_beams * vocab >= 1 << 31:
         raise KernelError(f"beam_select: {choices} choices of {n_beams} beams and {vocab} tokens; up to 256 beams and 256 choices are taken, no more than there are")
-    if not _one_device(logits, scores, out_scores, out_beams, out_tokens):
+    if not (scores.get_device() == dev and out_scores.get_device() == dev and out_beams.get_device() == dev and out_tokens.get_device() == dev):
         raise KernelError("beam_select: all tensors must be on one device")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, n_beams, out_scores, out_beams, out_tokens)
     lib = build.load("branches")
-    with _on(logits):
-        scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
-        _check(lib.hk_beam_select(_ptr(logits), _ptr(scores), prompts, n_beams, vocab, choices, _ptr(out_scores), _ptr(out_beams), _ptr(out_tokens),
-                                  _ptr(scratch), _stream()), "beam_select", launches=2)
+    scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
+    _check(lib.hk_beam_select(logits.data_ptr(), scores.data_ptr(), prompts, n_beams, vocab, choices, out_scores.data_ptr(), out_beams.data_ptr(),
+                              out_tokens.data_ptr(), scratch.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "beam_select", 2)
 
 
 from . import attention_fast, gemm_fast  # noqa: E402  (they use this module; looked up once, not on each call)
