@@ -1173,6 +1173,7 @@ struct F32Smem {
   float corr[F32_ROWS], inv[F32_ROWS];
   float2 ml[F32_ROWS];
   uint32_t see[F32_ROWS][2];
+  long long at[2][F32_KEYS];      // [parity of the tile]: where a key's row lies in the pages, -1 where there is none
   Walk start;
 };
 
@@ -1195,18 +1196,23 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
   while (next_segment<F32Cut>(a, w, s)) {
     const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
     const int end = s.q.context + s.q.count;
+    // where the keys of a tile lie: found once for keys and values, by threads that nothing else waits for
+    auto find = [&](int tile, int r) {
+      const int j = (s.t0 + tile) * F32_KEYS + r, page = j < end ? bt[j / a.page_tokens] : -1;
+      sm.at[tile & 1][r] = page >= 0 && page < a.num_pages ? (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * HD : -1;
+    };
     // a tile's keys or values, what does not exist as zeros
     auto fetch = [&](const void* pages, float* dst, int tile) {
-#pragma unroll 4
+#pragma unroll 8
       for (int e = tid; e < F32_KEYS * C4; e += F32_THREADS) {
-        const int r = e / C4, d = e % C4 * 4, j = (s.t0 + tile) * F32_KEYS + r;
-        const int page = j < end ? bt[j / a.page_tokens] : -1;
-        const bool in = page >= 0 && page < a.num_pages;
-        const float* src = reinterpret_cast<const float*>(pages) + (in ? (((size_t)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * HD + d : 0);
-        cp_async16(smem_u32(dst + r * LD + d), src, in);
+        const int r = e / C4, d = e % C4 * 4;
+        const long long at = sm.at[tile & 1][r];
+        cp_async16(smem_u32(dst + r * LD + d), reinterpret_cast<const float*>(pages) + (at >= 0 ? at + d : 0), at >= 0);
       }
       cp_async_commit();
     };
+    if (tid < F32_KEYS) find(0, tid);
+    __syncthreads();
     fetch(a.k, sm.k, 0);
     fetch(a.v, sm.v, 0);
     for (int e = tid; e < F32_ROWS * C4; e += F32_THREADS) {
@@ -1233,6 +1239,8 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
         const uint32_t see = visible32(tr, j0 + 32 * (tid & 1));
         sm.see[tid >> 1][tid & 1] = see;
         part = (tid >> 1) < s.rows && see != 0xffffffffu;
+      } else if (t + 1 < s.n) {
+        find(t + 1, tid - 2 * F32_ROWS);
       }
       cp_async_wait<1>();          // the keys
       part = __syncthreads_or(part);

@@ -82,7 +82,7 @@ __device__ __forceinline__ void move_rows(const RowArray& a, const int2* from, c
 
 // A block takes a request and some neighbouring arrays, and finds the pages of its path once for all that share a block table: finding
 // them is a chain of three reads, and as long as moving an array's rows.
-__global__ void __launch_bounds__(KEEP_THREADS)
+__global__ void __launch_bounds__(KEEP_THREADS, 4)
 compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_block, const int* __restrict__ paths, int width, int table_rows,
                     int table_stride, int page_tokens, long long num_pages) {
   __shared__ int2 from[KEEP_PATH], to[KEEP_PATH];
@@ -98,17 +98,18 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
         __syncthreads();
         if (threadIdx.x < 32) {            // the rows that move, in order
           const int* pages = block_table + (size_t)slot * table_stride;
-          auto place = [&](long long row) -> int2 {
-            const int at = (int)min(row / page_tokens, (long long)table_stride), page = at < table_stride ? pages[at] : -1;
-            return make_int2(page < 0 || page >= num_pages ? -1 : page, (int)(row - (long long)at * page_tokens));
+          auto place = [&](uint32_t row) -> int2 {           // row: below 2^32, two non-negative ints added
+            const uint32_t at = row / (uint32_t)page_tokens;
+            const int page = at < (uint32_t)table_stride ? pages[at] : -1;
+            return make_int2(page < 0 || page >= num_pages ? -1 : page, (int)(row - at * (uint32_t)page_tokens));
           };
           int n = 0;
           for (int i0 = done; i0 < min(width, done + KEEP_PATH); i0 += 32) {
             const int k = i0 + (int)threadIdx.x, row = k < width ? path[2 + k] : -1;
             int2 f = make_int2(-1, 0), t = f;
             if (row > k) {
-              f = place((long long)first + row);
-              t = place((long long)first + k);
+              f = place((uint32_t)first + (uint32_t)row);
+              t = place((uint32_t)first + (uint32_t)k);
             }
             const bool moves = f.x >= 0 && t.x >= 0;
             const unsigned all = __ballot_sync(0xffffffffu, moves);
@@ -557,8 +558,8 @@ HK_API int hk_compact_rows(const long long* table, int arrays, const int* paths,
   if (arrays > 65535 || table_rows < 1 || table_stride < 1 || page_tokens < 1 || heads < 1 || row_bytes < 1 || num_pages < 1)
     return HK_ERR_UNSUPPORTED;
   if ((long long)heads * row_bytes > 0x7fffffffLL / 64) return HK_ERR_UNSUPPORTED;
-  // some two blocks of work a SM and more, but up to 8 arrays a block
-  int per_block = (int)((long long)arrays * requests / (148 * 4));
+  // one wave of blocks (four a SM) where that is up to 8 arrays a block
+  int per_block = (int)(((long long)arrays * requests + 148 * 4 - 1) / (148 * 4));
   per_block = per_block < 1 ? 1 : per_block > 8 ? 8 : per_block;
   return hk_launch(compact_rows_kernel, dim3((unsigned)requests, (unsigned)((arrays + per_block - 1) / per_block)), dim3(KEEP_THREADS), 0,
                    (cudaStream_t)stream, reinterpret_cast<const RowArray*>(table), arrays, per_block, paths, width, table_rows, table_stride, page_tokens,
