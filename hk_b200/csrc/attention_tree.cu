@@ -141,12 +141,12 @@ __device__ __forceinline__ void unit_shape(const TreeArgs& a, const TreeReq& q, 
 }
 
 template <typename C>
-__device__ __forceinline__ uint32_t size_of(const TreeArgs& a, int r) {
-  if (r >= a.n_requests) return 0;
+__device__ __forceinline__ uint32_t size_of(const TreeArgs& a, const TreeReq& q) {
   int t_first, tiles, units;
-  unit_shape<C>(a, load_request(a, r), t_first, tiles, units);
+  unit_shape<C>(a, q, t_first, tiles, units);
   return (uint32_t)(tiles + C::LEAD) * units;
 }
+__device__ __forceinline__ TreeReq request_or_none(const TreeArgs& a, int r) { return r < a.n_requests ? load_request(a, r) : TreeReq{0, 0, 0, 0}; }
 
 __device__ __forceinline__ uint32_t warp_sum32(uint32_t v) {
 #pragma unroll
@@ -154,9 +154,10 @@ __device__ __forceinline__ uint32_t warp_sum32(uint32_t v) {
   return v;
 }
 
-// Where a CTA is in its share: the place in a unit, LEAD before its first tile.
+// Where a CTA is in its share: a request (`q`, as it was loaded), a unit of it and the place in that, LEAD before its first tile.
 struct Walk {
   int r, unit, place, left;
+  TreeReq q;
 };
 struct Share {
   Walk w;
@@ -172,11 +173,11 @@ __device__ __forceinline__ int share_of(const Share& s, uint32_t place) {
 template <typename C>
 __device__ __forceinline__ Share share_start(const TreeArgs& a, uint32_t cta, uint32_t ctas) {
   const int lane = threadIdx.x & 31;
-  Share share = {{a.n_requests, 0, 0, 0}, 0, 0, 0, 0};
-  const uint32_t mine = size_of<C>(a, lane);
-  uint32_t total = mine;
+  Share share = {{a.n_requests, 0, 0, 0, {0, 0, 0, 0}}, 0, 0, 0, 0};
+  TreeReq q = request_or_none(a, lane);
+  uint32_t total = size_of<C>(a, q);
 #pragma unroll 1
-  for (int r = lane + 32; r < a.n_requests; r += 32) total += size_of<C>(a, r);
+  for (int r = lane + 32; r < a.n_requests; r += 32) total += size_of<C>(a, load_request(a, r));
   share.total = total = warp_sum32(total);
   ctas = min(ctas, total);                       // no empty share between two of one unit
   if (cta >= ctas) return share;
@@ -187,7 +188,8 @@ __device__ __forceinline__ Share share_start(const TreeArgs& a, uint32_t cta, ui
   uint32_t base = 0;
 #pragma unroll 1
   for (int r0 = 0; r0 < a.n_requests; r0 += 32) {
-    const uint32_t n = r0 == 0 ? mine : size_of<C>(a, r0 + lane);
+    if (r0 > 0) q = request_or_none(a, r0 + lane);
+    const uint32_t n = size_of<C>(a, q);
     uint32_t sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -199,8 +201,10 @@ __device__ __forceinline__ Share share_start(const TreeArgs& a, uint32_t cta, ui
       const int src = __ffs(here) - 1;
       const uint32_t in = share.from - base - __shfl_sync(0xffffffffu, sum - n, src);
       share.w.r = r0 + src;
+      share.w.q = {__shfl_sync(0xffffffffu, q.slot, src), __shfl_sync(0xffffffffu, q.first, src), __shfl_sync(0xffffffffu, q.count, src),
+                   __shfl_sync(0xffffffffu, q.context, src)};
       int t_first, tiles, units;
-      unit_shape<C>(a, load_request(a, share.w.r), t_first, tiles, units);
+      unit_shape<C>(a, share.w.q, t_first, tiles, units);
       share.w.unit = (int)(in < (uint32_t)(tiles + C::LEAD) ? 0 : in / (uint32_t)(tiles + C::LEAD));
       share.w.place = (int)in - share.w.unit * (tiles + C::LEAD);
       break;
@@ -223,13 +227,13 @@ __device__ __forceinline__ bool next_segment(const TreeArgs& a, Walk& w, Segment
   int t_first, tiles, units;
 #pragma unroll 1
   while (w.left > 0 && w.r < a.n_requests) {
-    s.q = load_request(a, w.r);
-    unit_shape<C>(a, s.q, t_first, tiles, units);
+    unit_shape<C>(a, w.q, t_first, tiles, units);
     if (w.unit >= units) {
-      ++w.r;
+      w.q = request_or_none(a, ++w.r);
       w.unit = w.place = 0;
       continue;
     }
+    s.q = w.q;
     const int at = w.unit < a.G ? 0 : w.unit / a.G, begin = max(w.place - C::LEAD, 0), take = min(tiles + C::LEAD - w.place, w.left);
     s.g = w.unit - at * a.G;
     s.row0 = at * C::ROWS;
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a,
   int t_first = 0, tiles = 0, units = 0, row0 = 0, rows = 0, g = 0;
   TreeReq q = {0, 0, 0, 0};
   if (w.left > 0 && w.place > C::LEAD && share_from(share, c - 1) <= first) {
-    q = load_request(a, w.r);
+    q = w.q;
     unit_shape<C>(a, q, t_first, tiles, units);
     const int at = w.unit < a.G ? 0 : w.unit / a.G;
     g = w.unit - at * a.G;
@@ -295,16 +299,24 @@ __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a,
   float m = -CUDART_INF_F, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  // slot 2 (c - 1) + 1, then every second one from 2 c on
+  const float2* ml_at = reinterpret_cast<const float2*>(a.part_ml) + part_slot(c - 1, true) * a.rows_cap + row;
+  const float* o_at = part_place(a, part_slot(c - 1, true), row, dim, HD);
+  const int ml_step = 2 * a.rows_cap, o_step = 2 * HD * a.rows_cap, o_next = 4 * a.rows_cap;
   for (int p0 = 0; p0 < parts; p0 += DEEP) {
     float2 ml[DEEP];
     float4 u[DEEP], v[DEEP];
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
-      const int p = min(p0 + i, parts - 1);
-      const size_t slot = part_slot(c - 1 + p, p == 0);
-      ml[i] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot * a.rows_cap + row);
-      u[i] = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot, row, dim, HD)));
-      v[i] = __ldcg(reinterpret_cast<const float4*>(part_place(a, slot, row, dim + 4, HD)));
+      ml[i] = make_float2(-CUDART_INF_F, 0.f);
+      u[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p0 + i < parts) {
+        ml[i] = __ldcg(ml_at);
+        u[i] = __ldcg(reinterpret_cast<const float4*>(o_at));
+        v[i] = __ldcg(reinterpret_cast<const float4*>(o_at + o_next));
+      }
+      ml_at += p0 + i == 0 ? a.rows_cap : ml_step;
+      o_at += p0 + i == 0 ? HD * a.rows_cap : o_step;
     }
     float mn = m;
 #pragma unroll
@@ -316,8 +328,7 @@ __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a,
     m = mn;
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
-      if (p0 + i >= parts) break;
-      const float f = power<T>(ml[i].x - safe);
+      const float f = power<T>(ml[i].x - safe);      // a part that there is not: 0
       l = fmaf(ml[i].y, f, l);
       acc[0] = fmaf(u[i].x, f, acc[0]), acc[1] = fmaf(u[i].y, f, acc[1]), acc[2] = fmaf(u[i].z, f, acc[2]), acc[3] = fmaf(u[i].w, f, acc[3]);
       acc[4] = fmaf(v[i].x, f, acc[4]), acc[5] = fmaf(v[i].y, f, acc[5]), acc[6] = fmaf(v[i].z, f, acc[6]), acc[7] = fmaf(v[i].w, f, acc[7]);
