@@ -46,7 +46,8 @@ struct TreeArgs {
 };
 
 // Row `i` of a request (token * group + head of the group, at most 256 tokens): its token.  A division by a variable takes a hundred and
-// more clocks, of which the start of a short kernel has none to spare; i < 2^16 and group < 2^16 make this exact for their product below 2^32.
+// more clocks, of which the start of a short kernel has none to spare.  Exact while
+// i * group < 2^32: groups of up to 4,095 heads.
 __device__ __forceinline__ int token_of(const TreeArgs& a, int i) { return a.group == 1 ? i : (int)__umulhi((uint32_t)i, a.group_inverse); }
 
 // A request as the kernels take it: with nothing to do (count 0) where its numbers lie outside the arrays.
@@ -1453,7 +1454,7 @@ HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* 
   if (kernel == 0) return dtype == HK_F32 ? launch_generic<float>(a, s) : launch_generic<bf16>(a, s);
   if (kernel != 1 || ctas < 1 || part_o == nullptr || part_ml == nullptr) return HK_ERR_UNSUPPORTED;
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)part_o) & 15) != 0 || (((uintptr_t)part_ml) & 7) != 0) return HK_ERR_UNSUPPORTED;
-  if (hd != 64 && hd != 128) return HK_ERR_UNSUPPORTED;
+  if ((hd != 64 && hd != 128) || a.group > 4095) return HK_ERR_UNSUPPORTED;
   if (dtype == HK_F32) return hd == 128 ? launch_f32<128>(a, ctas, s) : launch_f32<64>(a, ctas, s);
   return hd == 128 ? launch_tc<128>(a, ctas, s) : launch_tc<64>(a, ctas, s);
 }

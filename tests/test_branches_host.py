@@ -64,3 +64,54 @@ def test_command_line_options():
                 ["--draft", "4", "--repeat-penalty", "1.2"]):
         with pytest.raises(BadUsage):
             parse_run_args(["m", "1,2"] + bad)
+
+
+def test_launches_go_to_the_device_of_their_tensors(monkeypatch):
+    """With another device current, every entry point launches on its tensors' device and that one's stream (against stand-ins)."""
+    import contextlib
+    import types
+
+    import torch
+
+    from hk_b200.csrc import build, gemm_fast, ops
+    current, launched = [1], []
+
+    @contextlib.contextmanager
+    def device(index):
+        old, current[0] = current[0], index
+        yield
+        current[0] = old
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(ops, "_need", lambda *a, **k: None)
+    monkeypatch.setattr(gemm_fast, "_sms", lambda d: 148)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: types.SimpleNamespace(data_ptr=lambda: 4096))
+
+    def tell(*args):
+        launched.append((current[0], args[-1]))
+        return 0
+    lib = types.SimpleNamespace(hk_copy_blocks=tell, hk_compact_rows=tell, hk_beam_select=tell, hk_beam_select_scratch=lambda *a: 64, hk_tree_attention=tell)
+    monkeypatch.setattr(build, "load", lambda name: lib)
+
+    class Fake:
+        def __init__(self, index, shape, dtype=None):
+            self.device, self.shape, self.dtype = types.SimpleNamespace(index=index), torch.Size(shape), dtype
+
+        def get_device(self):
+            return self.device.index
+
+        def data_ptr(self):
+            return 1024
+
+        def is_contiguous(self):
+            return True
+
+    f, n = torch.float32, torch.int32
+    for i in (0, 1):
+        ops.copy_blocks(Fake(i, (2, 5)), Fake(i, (3, 3)), 64)
+        ops.compact_rows(Fake(i, (2, 4)), Fake(i, (3, 6)), 4, 8, 16, 2, 256, 32)
+        ops.beam_select(Fake(i, (6, 50), f), Fake(i, (6,), f), 3, Fake(i, (2, 6), f), Fake(i, (2, 6), n), Fake(i, (2, 6), n))
+        ops.tree_attention(Fake(i, (4, 256), f), Fake(i, (9, 2, 16, 64), f), Fake(i, (9, 2, 16, 64), f), Fake(i, (2, 5), n), Fake(i, (1, 4), n),
+                           Fake(i, (4, 1), n), Fake(i, (4,), n), Fake(i, (4, 256), f), 4, 2, 64, 16, 0, 0.125, 4, 60)
+    assert launched == [(0, 100)] * 4 + [(1, 101)] * 4 and current == [1]
