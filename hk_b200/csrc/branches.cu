@@ -152,14 +152,15 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
 //
 // One pass over the logits: a CTA takes a part of a row through registers, a tile of 4,096 at a time with the next one on its way, and
 // keeps a sum of exponentials a thread against a reference of its own (a tile's sixteen in float32, all beyond that in 64 bits) and the
-// tokens that can be among its best `choices`: as many groups of threads hold a value each that reaches the smallest of the groups'
-// maxima, so what is below that bar is out; the bar is found anew after 1, 2, 4, ... tiles and where the list fills up.  A CTA a prompt
+// largest of each thread's sixteen.  When the part is through, a bar is found that at least `choices` of those reach, and only the few
+// sixteens that reach it are read again for the tokens that can be among the part's best.  (Looking for them on the way took a barrier
+// a tile and, with some lane over the bar in most tiles, one and a half times the instructions.)  A CTA a prompt
 // then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order: two beams' continuations lie as little
 // as 1e-7 apart often enough among a million, and which of them comes first must not hang on how a sum was rounded.
-// Bound by the instructions a logit: 8 or so, of which 5 are the exponential and its sum.
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
-constexpr int BC = 1024;              // candidates that are ranked side by side; more than that only among equal logits
+constexpr int BC = 2048;              // candidates that are ranked side by side; more than that only among equal logits
+constexpr int SLOTS = 16;             // maxima that a thread keeps
 
 struct RowPart {
   double sum;                         // of exp(x - top)
@@ -167,6 +168,39 @@ struct RowPart {
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Numbers as integers of the same order, and back.
+__device__ __forceinline__ uint32_t in_order(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+
+__device__ __forceinline__ uint64_t in_order(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double from_order(uint64_t u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
+
+// Raises a bar that at least `choices` numbers reach, by halves between it and the largest, until no more than `enough` do (or it is
+// found as far as the steps go); reach(to, step) counts how many reach `to`.
+template <int STEPS, typename F, typename R>
+__device__ __forceinline__ int raise_bar(F& bar, F top, int choices, int enough, R&& reach) {
+  int found = reach(bar, 0);
+  auto lo = in_order(bar), hi = in_order(top);
+  for (int step = 1; step <= STEPS && found > enough && hi - lo > 1; ++step) {
+    const auto middle = lo + (hi - lo) / 2;
+    const int n = reach(from_order(middle), step);
+    if (n >= choices) {
+      lo = middle;
+      found = n;
+    } else {
+      hi = middle;
+    }
+  }
+  bar = from_order(lo);
+  return found;
+}
 
 // (value, index) pairs: more, or as much and further ahead
 template <typename F>
@@ -231,23 +265,58 @@ __device__ __forceinline__ void best_of_block(F& x, int& i, F* s_x, int* s_i) {
   }
 }
 
-// e^x for x up to 20 and so: 2^(x log2 e) with the product in two parts, so that the constant's rounding adds no error that all terms
-// share; the product's own rounding is 2^-24 of it, the power's 2 units in the last place.
-__device__ __forceinline__ float exp_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, 1.9259629e-8f, x * 1.4426950216293335f)));
-  return y;
+constexpr int BE = 16;                // values of a tile a thread
+
+// Two float32 numbers an instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// The sum of e^(v - safe), differences up to 20 and so: 2^(x log2 e) with the product in two parts, so that the constant's rounding adds
+// no error that all terms share; the product's own rounding is 2^-24 of it, the power's 2 units in the last place.
+__device__ __forceinline__ float tile_sum(const float* v, float safe) {
+  const uint64_t less = two(-safe, -safe), high = two(1.4426950216293335f, 1.4426950216293335f), low = two(1.9259629e-8f, 1.9259629e-8f);
+  uint64_t sum = two(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < BE; e += 2) {
+    const uint64_t x = add_two(two(v[e], v[e + 1]), less), z = fma_two(x, low, mul_two(x, high));
+    float y0, y1;
+    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %2;\n\tex2.approx.ftz.f32 %0, a;\n\tex2.approx.ftz.f32 %1, b;\n\t}"
+        : "=f"(y0), "=f"(y1) : "l"(z));
+    sum = add_two(sum, two(y0, y1));
+  }
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum));
+  return a + b;
 }
 
 constexpr float LOWEST = -3.402823466e38f;
-constexpr int BE = 16;                // values of a tile a thread
+constexpr int BAR_STEPS = 12;
 
 // The parts of a row are of `length` values (the last of what is left).
 __global__ void __launch_bounds__(BT, 4)
 beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ scores, int V, int choices, int groups, int parts, int length,
                  RowPart* __restrict__ part, float* __restrict__ part_x, int* __restrict__ part_i) {
-  __shared__ float s_group[BT], s_x[2][BC];
-  __shared__ int s_i[2][BC], s_n;
+  __shared__ float s_group[BT], s_high[SLOTS][BT], s_x[BC];
+  __shared__ int s_i[BC], s_n, s_found[BAR_STEPS + 1];
+  __shared__ uint16_t s_pair[BC];
   __shared__ double s_sum[BT / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -263,119 +332,128 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   // A thread's values of a tile: four times four neighbours, or, where a part is short, single ones.  Which it has does not hang on where
   // the row lies (equal rows have equal sums, to the bit); how they are read does.
   const bool fours = length >= 4 * BT, wide = fours && (((uintptr_t)(x + begin)) & 15) == 0;
-  auto index = [&](int t, int e) { return begin + t * (BT * BE) + (fours ? (e / 4 * BT + tid) * 4 + (e & 3) : e * BT + tid); };
+  auto index = [&](int t, int e, int of) { return begin + t * (BT * BE) + (fours ? (e / 4 * BT + of) * 4 + (e & 3) : e * BT + of); };
   auto load = [&](int t, float* v) {
+    if (wide && begin + (t + 1) * (BT * BE) <= end) {
+      const float* from = x + begin + t * (BT * BE) + 4 * tid;
 #pragma unroll
-    for (int e = 0; e < BE; e += 4) {
-      const int i = index(t, e);
-      if (wide && i + 3 < end) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+      for (int e = 0; e < BE; e += 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(from + e * BT));
         v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[e + c] = index(t, e + c) < end ? __ldg(x + index(t, e + c)) : -CUDART_INF_F;
       }
+      return;
     }
+#pragma unroll
+    for (int e = 0; e < BE; ++e) v[e] = index(t, e, tid) < end ? __ldg(x + index(t, e, tid)) : -CUDART_INF_F;
   };
-  if (tid == 0) s_n = 0;
-  const int tiles = (end - begin + BT * BE - 1) / (BT * BE);
-  float next[BE], mine = -CUDART_INF_F, bar = LOWEST, top = -CUDART_INF_F, ref = -CUDART_INF_F;
+  const int tiles = (end - begin + BT * BE - 1) / (BT * BE), per = (tiles + SLOTS - 1) / SLOTS;
+  float slot_high = -CUDART_INF_F, mine = -CUDART_INF_F, ref = -CUDART_INF_F;
   double sum = 0.0;
-  int side = 0;                        // the list in use
-  load(0, next);
-  for (int t = 0; t < tiles; ++t) {
-    float v[BE], high = -CUDART_INF_F, odd = 0.f;
-#pragma unroll
-    for (int e = 0; e < BE; ++e) {
-      v[e] = next[e];
-      odd = fmaf(v[e], 0.f, odd);      // NaN where one is not finite
-    }
-    if (odd != 0.f) {
-#pragma unroll
-      for (int e = 0; e < BE; ++e) v[e] = finite(v[e]) ? v[e] : -CUDART_INF_F;
-    }
+  int slot = 0, in_slot = 0;
+  auto tile = [&](int t, float* v, float* next) {
+    if (t + 1 < tiles) load(t + 1, next);
+    float high = -CUDART_INF_F;        // (a maximum passes NaN by)
 #pragma unroll
     for (int e = 0; e < BE; ++e) high = fmaxf(high, v[e]);
-    if (t + 1 < tiles) load(t + 1, next);
-    mine = fmaxf(mine, high);
-    // the barrier also says that the groups' maxima were read and the tokens of the last tile listed
-    if (__syncthreads_or(s_n > BC / 2) || (t & (t - 1)) == 0) {
-      const int listed = s_n;          // (read by all before any passes the barrier inside, behind which the list grows)
-      find_bar<BT>(mine, groups, s_group, bar, top);
-      bar = fmaxf(bar, LOWEST);
-      if (t == 0) ref = top;
-      if (listed > BC / 2 && listed <= BC) {       // the list anew, without what has fallen below the bar
-        __syncthreads();
-        if (tid == 0) s_n = 0;
-        __syncthreads();
-        for (int c = tid; c < listed; c += BT)
-          if (s_x[side][c] >= bar) {
-            const int to = atomicAdd(&s_n, 1);
-            s_x[side ^ 1][to] = s_x[side][c];
-            s_i[side ^ 1][to] = s_i[side][c];
-          }
-        side ^= 1;
-        __syncthreads();
+    if (high == CUDART_INF_F) {
+      high = -CUDART_INF_F;
+#pragma unroll
+      for (int e = 0; e < BE; ++e) {
+        v[e] = finite(v[e]) ? v[e] : -CUDART_INF_F;
+        high = fmaxf(high, v[e]);
       }
     }
-    if (high > ref + 20.0f) {          // also true for the first finite value behind a tile that had none
+    slot_high = fmaxf(slot_high, high);
+    if (++in_slot == per || t + 1 == tiles) {
+      s_high[slot++][tid] = slot_high;
+      mine = fmaxf(mine, slot_high);
+      slot_high = -CUDART_INF_F;
+      in_slot = 0;
+    }
+    if (high > ref + 20.0f) {          // also true for the first finite value
       sum *= ref == -CUDART_INF_F ? 0.0 : exp((double)ref - (double)high);
       ref = high;
     }
     const float safe = ref == -CUDART_INF_F ? 0.f : ref;
-    float part_sum[2] = {0.f, 0.f};
+    float s = tile_sum(v, safe);
+    if (s != s) {                      // NaN where a value is
 #pragma unroll
-    for (int e = 0; e < BE; ++e) part_sum[e & 1] += exp_of(v[e] - safe);
-    sum += (double)(part_sum[0] + part_sum[1]);
-    if (high >= bar) {
-      uint32_t hits = 0;
-#pragma unroll
-      for (int e = 0; e < BE; ++e) hits |= v[e] >= bar ? 1u << e : 0u;
-      for (; hits; hits &= hits - 1) {
-        const int i = index(t, __ffs(hits) - 1), c = atomicAdd(&s_n, 1);
-        if (c < BC) {
-          s_x[side][c] = x[i];         // once more from the row: a register cannot be picked by a number
-          s_i[side][c] = i;
-        }
-      }
+      for (int e = 0; e < BE; ++e) v[e] = finite(v[e]) ? v[e] : -CUDART_INF_F;
+      s = tile_sum(v, safe);
     }
+    sum += (double)s;
+  };
+  float one[BE], other[BE];
+  load(0, one);
+  for (int t = 0; t < tiles; t += 2) {
+    tile(t, one, other);
+    if (t + 1 < tiles) tile(t + 1, other, one);
   }
-  __syncthreads();
-  int n = s_n;
+  const int slots = slot;
+  if (tid <= BAR_STEPS) s_found[tid] = 0;
+  if (tid == 0) s_n = 0;
+  float bar, top;
   find_bar<BT>(mine, groups, s_group, bar, top);
   bar = fmaxf(bar, LOWEST);
   double all = ref == top || ref == -CUDART_INF_F ? sum : sum * exp((double)ref - (double)top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if ((tid & 31) == 0) s_sum[tid >> 5] = all;
-  __syncthreads();
+  // how many slots reach a bar
+  auto reach = [&](float to, int step) {
+    int n = 0;
+    if (mine >= to)
+      for (int k = 0; k < slots; ++k) n += s_high[k][tid] >= to ? 1 : 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0 && n > 0) atomicAdd(&s_found[step], n);
+    __syncthreads();
+    return s_found[step];
+  };
+  const int found = raise_bar<BAR_STEPS>(bar, top, choices, choices + choices / 4 + 16, reach);
   if (tid == 0) {
     double total = 0.0;
 #pragma unroll
     for (int w = 0; w < BT / 32; ++w) total += s_sum[w];
     part[at] = RowPart{total, top, 0.f};
   }
-  if (n <= BC) {
-    // those that reach the last bar, ranked side by side
+  int n = BC + 1;
+  if (found <= BC) {
+    // the slots that reach the bar, and their values that do: four threads a slot
+    if (mine >= bar)
+      for (int k = 0; k < slots; ++k)
+        if (s_high[k][tid] >= bar) s_pair[atomicAdd(&s_n, 1)] = (uint16_t)(k * BT + tid);
     __syncthreads();
     if (tid == 0) s_n = 0;
     __syncthreads();
-    for (int c = tid; c < n; c += BT)
-      if (s_x[side][c] >= bar) {
-        const int to = atomicAdd(&s_n, 1);
-        s_x[side ^ 1][to] = s_x[side][c];
-        s_i[side ^ 1][to] = s_i[side][c];
+    for (int c = tid / 4; c < found; c += BT / 4) {
+      const int of = s_pair[c] % BT, t0 = s_pair[c] / BT * per;
+      for (int t = t0; t < min(tiles, t0 + per); ++t) {
+        float y[4];
+        int i[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          i[e] = index(t, tid % 4 * 4 + e, of);
+          y[e] = i[e] < end ? __ldg(x + i[e]) : -CUDART_INF_F;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (y[e] >= bar && finite(y[e])) {
+            const int to = atomicAdd(&s_n, 1);
+            if (to < BC) s_x[to] = y[e], s_i[to] = i[e];
+          }
       }
-    side ^= 1;
+    }
     __syncthreads();
     n = s_n;
+  }
+  if (n <= BC) {
     for (int c = n + tid; c < choices; c += BT) part_x[at * choices + c] = -CUDART_INF_F;
     for (int c = tid; c < n; c += BT) {
-      const float mx = s_x[side][c];
-      const int mi = s_i[side][c];
+      const float mx = s_x[c];
+      const int mi = s_i[c];
       int rank = 0;
 #pragma unroll 4
-      for (int o = 0; o < n; ++o) rank += ahead(s_x[side][o], s_i[side][o], mx, mi) ? 1 : 0;
+      for (int o = 0; o < n; ++o) rank += ahead(s_x[o], s_i[o], mx, mi) ? 1 : 0;
       if (rank < choices) {
         part_x[at * choices + rank] = mx;
         part_i[at * choices + rank] = mi;
@@ -396,7 +474,7 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
         bi = i;
       }
     }
-    best_of_block<BT>(bx, bi, s_x[0], s_i[0]);
+    best_of_block<BT>(bx, bi, s_x, s_i);
     if (tid == 0) {
       part_x[at * choices + k] = bx;
       part_i[at * choices + k] = bi;
@@ -406,18 +484,34 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   }
 }
 
-constexpr int CT = 512, CDEEP = 8;    // threads of the choice; candidates that a thread has on their way at once
+constexpr int CT = 512, CDEEP = 8, CHOICE_STEPS = 24;    // threads of the choice; candidates that a thread has on their way at once
 
 __global__ void __launch_bounds__(CT)
-beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, int groups, int parts, const RowPart* __restrict__ part,
+beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, int groups, int parts, int ranks, uint32_t ranks_inverse,
+                   uint32_t beam_inverse, const RowPart* __restrict__ part,
                    const float* __restrict__ part_x, const int* __restrict__ part_i, float* __restrict__ out_scores,
                    int* __restrict__ out_beams, int* __restrict__ out_tokens) {
   __shared__ double s_group[CT], s_x[BC], s_lift[BEAM_MOST];      // s_lift: a beam's score less the logarithm of its sum
-  __shared__ int s_i[BC], s_n, s_taken[BEAM_MOST];
+  __shared__ int s_i[BC], s_n, s_taken[BEAM_MOST], s_found[CHOICE_STEPS + 1];
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row0 = (size_t)b * K;
+  // candidate c: the token of rank c % choices of part c / choices of the prompt's rows (-inf where a part has fewer); its flat index
+  // is beam * V + token.  The threads hold as many of them as they have registers for, all or the first `ranks` of each part; those are
+  // on their way while the rows' sums are joined.
+  const int of_beam = parts * choices, all = K * of_beam, held = K * parts * ranks;
+  const float* xs = part_x + row0 * of_beam;
+  const int* is = part_i + row0 * of_beam;
+  const bool kept = ranks == choices;
+  float keep_x[CDEEP];
+  int keep_i[CDEEP];
+#pragma unroll
+  for (int j = 0; j < CDEEP; ++j) {
+    const int m = threadIdx.x + j * CT, p = ranks == 1 ? m : (int)__umulhi((uint32_t)m, ranks_inverse), c = p * choices + m - p * ranks;
+    keep_x[j] = m < held ? xs[c] : -CUDART_INF_F;
+    keep_i[j] = m < held ? is[c] : 0;
+  }
   for (int k = warp; k < K; k += CT / 32) {
     const RowPart* of = part + (row0 + k) * parts;
     RowPart first = {0.0, -CUDART_INF_F, 0.f};
@@ -437,38 +531,68 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
     if (lane == 0) s_lift[k] = top == -CUDART_INF_F ? -CUDART_INF : (double)scores[row0 + k] - ((double)top + log(sum));
   }
   if (threadIdx.x == 0) s_n = 0;
+  if (threadIdx.x <= CHOICE_STEPS) s_found[threadIdx.x] = 0;
   __syncthreads();
-  // candidate c: the token of rank c % choices of part c / choices of the prompt's rows (-inf where a part has fewer); its flat index
-  // is beam * V + token
-  const int of_beam = parts * choices, all = K * of_beam;
-  const float* xs = part_x + row0 * of_beam;
-  auto score = [&](int c, float x) { return x > -CUDART_INF_F ? (double)x + s_lift[c / of_beam] : -CUDART_INF; };
-  auto flat = [&](int c) { return c / of_beam * V + part_i[row0 * of_beam + c]; };
+  double mine = -CUDART_INF, keep[CDEEP];
+#pragma unroll
+  for (int j = 0; j < CDEEP; ++j) {
+    const uint32_t m = threadIdx.x + j * CT;
+    const int k = ranks * parts == 1 ? m : __umulhi(m, beam_inverse);
+    keep[j] = keep_x[j] > -CUDART_INF_F ? (double)keep_x[j] + s_lift[k] : -CUDART_INF;
+    keep_i[j] += k * V;
+    mine = keep[j] > mine ? keep[j] : mine;
+  }
+  auto each_kept = [&](auto&& take) {
+#pragma unroll
+    for (int j = 0; j < CDEEP; ++j)
+      if (keep[j] > -CUDART_INF) take(keep[j], keep_i[j]);
+  };
   auto each = [&](auto&& take) {
+    if (kept) return each_kept(take);
     for (int c0 = threadIdx.x; c0 < all; c0 += CT * CDEEP) {
       float x[CDEEP];
 #pragma unroll
       for (int j = 0; j < CDEEP; ++j) x[j] = c0 + j * CT < all ? xs[c0 + j * CT] : -CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < CDEEP; ++j)
-        if (x[j] > -CUDART_INF_F) take(c0 + j * CT, score(c0 + j * CT, x[j]));
+        if (x[j] > -CUDART_INF_F) {
+          const int c = c0 + j * CT, k = c / of_beam;
+          take((double)x[j] + s_lift[k], k * V + is[c]);
+        }
     }
   };
-  double mine = -CUDART_INF;
-  each([&](int, double x) { mine = x > mine ? x : mine; });
   double bar, top;
   find_bar<CT>(mine, groups, s_group, bar, top);
-  if (mine >= bar)
-    each([&](int c, double x) {
+  auto reach = [&](auto&& each, double to, int step) {
+    int n = 0;
+    each([&](double x, int) { n += x >= to ? 1 : 0; });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0 && n > 0) atomicAdd(&s_found[step], n);
+    __syncthreads();
+    return s_found[step];
+  };
+  raise_bar<CHOICE_STEPS>(bar, top, choices, choices + choices / 4 + 16, [&](double to, int step) { return reach(each_kept, to, step); });
+  auto gather = [&] {
+    each([&](double x, int i) {
       if (x < bar) return;
       const int at = atomicAdd(&s_n, 1);
       if (at < BC) {
         s_x[at] = x;
-        s_i[at] = flat(c);
+        s_i[at] = i;
       }
     });
-  __syncthreads();
-  const int n = s_n;
+    __syncthreads();
+    return s_n;
+  };
+  int n = gather();
+  if (n > BC && !kept) {               // a part's further ranks are before the others' first ones: the bar among all
+    __syncthreads();
+    if (threadIdx.x == 0) s_n = 0;
+    if (threadIdx.x <= CHOICE_STEPS) s_found[threadIdx.x] = 0;
+    __syncthreads();
+    raise_bar<CHOICE_STEPS>(bar, top, choices, BC / 2, [&](double to, int step) { return reach(each, to, step); });
+    n = gather();
+  }
   auto give = [&](int rank, double x, int i) {
     out_scores[(size_t)b * choices + rank] = (float)x;
     out_beams[(size_t)b * choices + rank] = i / V;
@@ -489,9 +613,7 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
     for (int k = 0; k < choices; ++k) {
       double bx = -CUDART_INF;
       int bi = -1;
-      each([&](int c, double x) {
-        if (bi >= 0 && x < bx) return;
-        const int i = flat(c);
+      each([&](double x, int i) {
         if (ahead(past, past_i, x, i) && (bi < 0 || ahead(x, i, bx, bi))) {
           bx = x;
           bi = i;
@@ -578,7 +700,7 @@ HK_API long long hk_beam_select_scratch(int rows, int V, int choices) {
 HK_API int hk_beam_select(const float* logits, const float* scores, int prompts, int beams, int V, int choices, float* out_scores,
                           int* out_beams, int* out_tokens, void* scratch, void* stream) {
   if (prompts <= 0) return 0;
-  if (beams < 1 || beams > BEAM_MOST || V < 1 || choices < 1 || choices > BEAM_MOST || (long long)beams * V > 0x7fffffffLL ||
+  if (beams < 1 || beams > BEAM_MOST || V < 1 || V > (1 << 30) || choices < 1 || choices > BEAM_MOST || (long long)beams * V > 0x7fffffffLL ||
       choices > (long long)beams * V || (long long)prompts * beams > 0x7fffffffLL || (((uintptr_t)scratch) & 15) != 0)
     return HK_ERR_UNSUPPORTED;
   const int rows = prompts * beams, groups = beam_groups(choices);
@@ -592,6 +714,10 @@ HK_API int hk_beam_select(const float* logits, const float* scores, int prompts,
   const dim3 grid((unsigned)(rows * parts)), block(BT);
   const int e = hk_launch_pdl(beam_rows_kernel, grid, block, 0, s, logits, scores, V, choices, groups, parts, length, part, part_x, part_i);
   if (e) return e;
-  return hk_launch_pdl(beam_choice_kernel, dim3((unsigned)prompts), dim3(CT), 0, s, scores, beams, V, choices, groups, parts, part, part_x, part_i,
+  // (m / d is the upper half of m times 2^32 / d, rounded up, while m d < 2^32)
+  const int most = CT * CDEEP / (beams * parts), ranks = choices < most ? choices : most;
+  auto inverse = [](long long d) { return (uint32_t)(d == 1 ? 0 : ((1ll << 32) + d - 1) / d); };
+  return hk_launch_pdl(beam_choice_kernel, dim3((unsigned)prompts), dim3(CT), 0, s, scores, beams, V, choices, groups, parts, ranks, inverse(ranks),
+                       inverse((long long)ranks * parts), part, part_x, part_i,
                        out_scores, out_beams, out_tokens);
 }

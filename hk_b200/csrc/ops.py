@@ -1696,7 +1696,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
         raise KernelError("beam_select: the three results must have one shape")
     if prompts == 0:
         return
-    if n_beams > 256 or not 1 <= choices <= min(256, n_beams * vocab) or n_beams * vocab >= 1 << 31:
+    if n_beams > 256 or not 1 <= choices <= min(256, n_beams * vocab) or vocab > 1 << 30 or n_beams * vocab >= 1 << 31:
         raise KernelError(f"beam_select: {choices} choices of {n_beams} beams and {vocab} tokens; up to 256 beams and 256 choices are taken, no more than there are")
     if not (scores.get_device() == dev and out_scores.get_device() == dev and out_beams.get_device() == dev and out_tokens.get_device() == dev):
         raise KernelError("beam_select: all tensors must be on one device")

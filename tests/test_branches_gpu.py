@@ -147,6 +147,32 @@ def test_climbing_logits():
         check_beams(ops, np.repeat(logits, 60, axis=0)[:700], -(rng.random(700) * 0.1).astype(np.float32), 7, 100)
 
 
+@pytest.mark.parametrize("leading", [1, 7, 40, 128])
+def test_many_beams_and_choices(leading):
+    """More parts' tokens than the threads of the choice hold: the best lie in a few beams, or in all."""
+    from hk_b200.csrc import ops
+    rng = np.random.default_rng(leading)
+    logits = (rng.standard_normal((128, 40000)) * 3).astype(np.float32)
+    scores = -(rng.random(128) * 2).astype(np.float32)
+    scores[leading:] -= 40.0
+    order = rng.permutation(128)
+    check_beams(ops, logits[order], scores[order], 128, 256)
+
+
+@pytest.mark.parametrize("V,allowed,choices", [(40000, 500, 16), (40000, 300, 256), (3000, 3000, 200), (5000, 4000, 256), (1500, 40, 100)])
+def test_rows_that_allow_few_tokens(V, allowed, choices):
+    """Most tokens masked, by -inf or NaN: groups of threads that hold nothing, and bars that are found late."""
+    from hk_b200.csrc import ops
+    rng = np.random.default_rng(V + choices)
+    logits = (rng.standard_normal((6, V)) * 3).astype(np.float32)
+    for row in logits:
+        row[rng.permutation(V)[allowed:]] = -np.inf
+        row[rng.random(V) < 0.02] = np.nan
+    logits[1, rng.random(V) < 0.01] = np.inf
+    check_beams(ops, logits, -(rng.random(6) * 3).astype(np.float32), 2, choices)
+    check_beams(ops, np.repeat(logits, 120, axis=0)[:700], -(rng.random(700) * 3).astype(np.float32), 7, choices)
+
+
 def test_beams_that_are_not_there_and_masked_logits():
     from hk_b200.csrc import ops
     rng = np.random.default_rng(5)

@@ -115,3 +115,18 @@ def test_launches_go_to_the_device_of_their_tensors(monkeypatch):
         ops.tree_attention(Fake(i, (4, 256), f), Fake(i, (9, 2, 16, 64), f), Fake(i, (9, 2, 16, 64), f), Fake(i, (2, 5), n), Fake(i, (1, 4), n),
                            Fake(i, (4, 1), n), Fake(i, (4,), n), Fake(i, (4, 256), f), 4, 2, 64, 16, 0, 0.125, 4, 60)
     assert launched == [(0, 100)] * 4 + [(1, 101)] * 4 and current == [1]
+
+
+def test_beam_selection_refuses_rows_that_its_indexes_do_not_hold(monkeypatch):
+    import types
+
+    import torch
+
+    from hk_b200.csrc import ops
+    monkeypatch.setattr(ops, "_need", lambda *a, **k: None)
+
+    def fake(*shape):
+        return types.SimpleNamespace(shape=torch.Size(shape), get_device=lambda: 0)
+    for vocab, beams in (((1 << 30) + 1, 1), (1 << 30, 2), (1 << 23, 256), (50, 257)):
+        with pytest.raises(ops.KernelError, match="are taken"):
+            ops.beam_select(fake(beams, vocab), fake(beams), beams, fake(1, 4), fake(1, 4), fake(1, 4))
