@@ -650,7 +650,7 @@ int beam_groups(int choices) {
 
 // How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part.
 void beam_cut(int rows, int V, int* parts, int* length) {
-  const int wave = 148 * 4, most = (V + BT * BE / 2 - 1) / (BT * BE / 2);
+  const int wave = 148 * 4, most = (V + BT * BE - 1) / (BT * BE);
   int n = wave / rows;
   n = n < 1 ? 1 : n > most ? most : n;
   *length = ((V + n - 1) / n + 3) & ~3;
