@@ -29,6 +29,24 @@ struct TreeReq {
   int slot, first, count, context;
 };
 
+}  // namespace
+
+// What a call says, in one piece: the host's language takes longer to hand over thirty numbers than to pack them.
+struct TreeCall {
+  const void *q, *k, *v;
+  void* out;
+  const int *block_table, *requests;
+  const void* ancestors;
+  const int* positions;
+  const float* sinks;
+  long long num_pages;
+  int dtype, table_rows, table_stride, n_requests, most_tokens, most_keys, words, n, page_tokens, H, G, hd, window, sink;
+  float scale, softcap;
+};
+static_assert(sizeof(TreeCall) == 10 * 8 + 16 * 4, "packed without gaps");
+
+namespace {
+
 struct TreeArgs {
   const void *q, *k, *v;
   void* out;
@@ -1424,37 +1442,34 @@ int launch_f32(const TreeArgs& a, int ctas, cudaStream_t s) {
 // 128, in bfloat16 on the tensor cores (cache pages that are whole boxes of a 128-key tile: multiples of 8 that divide 128, and
 // multiples of 128), in float32 with multiply-adds; `ctas` shares, part_o float [2 ctas, hd / 4, rows_cap, 4] and part_ml [2 ctas,
 // rows_cap, 2] for what they leave, rows_cap at least the rows of a tile (256, in float32 32; or most_tokens * H / G where that is less); `status` is set to 4 if a bounded wait ran out.
-HK_API int hk_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const int* block_table, int table_rows,
-                             int table_stride, const int* requests, int n_requests, int most_tokens, int most_keys, const void* ancestors, int words,
-                             const int* positions, int n, long long num_pages, int page_tokens, int H, int G, int hd, int window,
-                             float scale, float softcap, int sink, const float* sinks, int kernel, int ctas, float* part_o,
-                             float* part_ml, int rows_cap, int* status, void* stream) {
-  if (n <= 0 || n_requests <= 0 || most_tokens <= 0) return 0;
-  if (most_keys < 1 || most_keys > (long long)table_stride * page_tokens || most_tokens > 256) return HK_ERR_UNSUPPORTED;
-  if (H < 1 || G < 1 || H % G != 0 || hd < 1 || hd > 256 || page_tokens < 1 || table_rows < 1 || table_stride < 1 || words < 1 ||
-      n_requests > 65535 || num_pages < 1 || softcap < 0.f || !(scale > 0.f) || (dtype != HK_F32 && dtype != HK_BF16) ||
-      (((uintptr_t)requests) & 15) != 0)
+HK_API int hk_tree_attention(const TreeCall* call, int kernel, int ctas, float* part_o, float* part_ml, int rows_cap, int* status, void* stream) {
+  const TreeCall& c = *call;
+  if (c.n <= 0 || c.n_requests <= 0 || c.most_tokens <= 0) return 0;
+  if (c.most_keys < 1 || c.most_keys > (long long)c.table_stride * c.page_tokens || c.most_tokens > 256) return HK_ERR_UNSUPPORTED;
+  if (c.H < 1 || c.G < 1 || c.H % c.G != 0 || c.hd < 1 || c.hd > 256 || c.page_tokens < 1 || c.table_rows < 1 || c.table_stride < 1 || c.words < 1 ||
+      c.n_requests > 65535 || c.num_pages < 1 || c.softcap < 0.f || !(c.scale > 0.f) || (c.dtype != HK_F32 && c.dtype != HK_BF16) ||
+      (((uintptr_t)c.requests) & 15) != 0)
     return HK_ERR_UNSUPPORTED;
   TreeArgs a;
-  a.q = q; a.k = k; a.v = v; a.out = out;
-  a.block_table = block_table;
-  a.requests = reinterpret_cast<const TreeReq*>(requests);
-  a.ancestors = static_cast<const uint32_t*>(ancestors);
-  a.positions = positions;
-  a.sinks = sink ? sinks : nullptr;
+  a.q = c.q; a.k = c.k; a.v = c.v; a.out = c.out;
+  a.block_table = c.block_table;
+  a.requests = reinterpret_cast<const TreeReq*>(c.requests);
+  a.ancestors = static_cast<const uint32_t*>(c.ancestors);
+  a.positions = c.positions;
+  a.sinks = c.sink ? c.sinks : nullptr;
   a.part_o = part_o; a.part_ml = part_ml; a.status = status;
-  a.num_pages = num_pages;
-  a.n = n; a.n_requests = n_requests; a.most_tokens = most_tokens; a.most_keys = most_keys; a.words = words;
-  a.table_rows = table_rows; a.table_stride = table_stride; a.page_tokens = page_tokens;
-  a.H = H; a.G = G; a.hd = hd; a.window = window > 0 ? window : 0; a.sink = sink; a.rows_cap = rows_cap;
-  a.scale = scale; a.softcap = softcap;
-  a.group = H / G;
+  a.num_pages = c.num_pages;
+  a.n = c.n; a.n_requests = c.n_requests; a.most_tokens = c.most_tokens; a.most_keys = c.most_keys; a.words = c.words;
+  a.table_rows = c.table_rows; a.table_stride = c.table_stride; a.page_tokens = c.page_tokens;
+  a.H = c.H; a.G = c.G; a.hd = c.hd; a.window = c.window > 0 ? c.window : 0; a.sink = c.sink; a.rows_cap = rows_cap;
+  a.scale = c.scale; a.softcap = c.softcap;
+  a.group = c.H / c.G;
   a.group_inverse = a.group == 1 ? 0u : (uint32_t)((0x100000000ull + a.group - 1) / a.group);
   cudaStream_t s = (cudaStream_t)stream;
-  if (kernel == 0) return dtype == HK_F32 ? launch_generic<float>(a, s) : launch_generic<bf16>(a, s);
+  if (kernel == 0) return c.dtype == HK_F32 ? launch_generic<float>(a, s) : launch_generic<bf16>(a, s);
   if (kernel != 1 || ctas < 1 || part_o == nullptr || part_ml == nullptr) return HK_ERR_UNSUPPORTED;
-  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)part_o) & 15) != 0 || (((uintptr_t)part_ml) & 7) != 0) return HK_ERR_UNSUPPORTED;
-  if ((hd != 64 && hd != 128) || a.group > 4095) return HK_ERR_UNSUPPORTED;
-  if (dtype == HK_F32) return hd == 128 ? launch_f32<128>(a, ctas, s) : launch_f32<64>(a, ctas, s);
-  return hd == 128 ? launch_tc<128>(a, ctas, s) : launch_tc<64>(a, ctas, s);
+  if ((((uintptr_t)c.q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.out | (uintptr_t)part_o) & 15) != 0 || (((uintptr_t)part_ml) & 7) != 0) return HK_ERR_UNSUPPORTED;
+  if ((c.hd != 64 && c.hd != 128) || a.group > 4095) return HK_ERR_UNSUPPORTED;
+  if (c.dtype == HK_F32) return c.hd == 128 ? launch_f32<128>(a, ctas, s) : launch_f32<64>(a, ctas, s);
+  return c.hd == 128 ? launch_tc<128>(a, ctas, s) : launch_tc<64>(a, ctas, s);
 }

@@ -155,8 +155,8 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
 // largest of each thread's sixteen.  When the part is through, a bar is found that at least `choices` of those reach, and only the few
 // sixteens that reach it are read again for the tokens that can be among the part's best.  (Looking for them on the way took a barrier
 // a tile and, with some lane over the bar in most tiles, one and a half times the instructions.)  A CTA a prompt
-// then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them.  A 64-bit order: two beams' continuations lie as little
-// as 1e-7 apart often enough among a million, and which of them comes first must not hang on how a sum was rounded.
+// then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them: rounded to float32, scores of some -10 lie 1e-6 apart,
+// and neighbours among a million would be equal often enough.  What is left is the error of the exponentials, some 1e-8 of a sum.
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
 constexpr int BC = 2048;              // candidates that are ranked side by side; more than that only among equal logits
@@ -648,9 +648,11 @@ int beam_groups(int choices) {
   return g;
 }
 
-// How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part.
+// How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part,
+// of rows with 32 tiles and more a tile (more parts than a warp has lanes take the choice longer than they save: 4 rows of 151,936
+// 14.6 us in half tiles, 12.6 in whole ones).
 void beam_cut(int rows, int V, int* parts, int* length) {
-  const int wave = 148 * 4, most = (V + BT * BE - 1) / (BT * BE);
+  const int wave = 148 * 4, tile = BT * BE, least = V >= 32 * tile ? tile : tile / 2, most = (V - 1) / least + 1;
   int n = wave / rows;
   n = n < 1 ? 1 : n > most ? most : n;
   *length = ((V + n - 1) / n + 3) & ~3;

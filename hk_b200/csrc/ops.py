@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 from typing import Optional
 
 import numpy as np
@@ -1554,7 +1555,9 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
             and H >= 1 and G >= 1 and H % G == 0 and 1 <= hd <= 256 and width == H * hd and out.shape == q.shape
             and shape == (pages, G, page_tokens, hd) and v_pages.shape == shape and four == 4 and marks == n and positions.shape == (n,)
             and 1 <= most_tokens <= TREE_TOKENS and most_tokens <= 32 * words and 1 <= most_keys <= stride * page_tokens and all_keys >= 0
-            and scale > 0 and softcap >= 0 and sinks is None and (dtype is torch.float32 or dtype is torch.bfloat16)):
+            and scale > 0 and softcap >= 0 and (sinks is None or (sink and sinks.dtype is torch.float32 and sinks.shape == (H,) and sinks.get_device() == dev
+                                                     and sinks.is_contiguous()))
+            and (dtype is torch.float32 or dtype is torch.bfloat16)):
         _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, scale, most_tokens, most_keys,
                      all_keys, sink, sinks, softcap)
     if n == 0 or m == 0:
@@ -1564,9 +1567,11 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
             return tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, window, scale,
                                   most_tokens, most_keys, all_keys, sink, sinks, softcap)
     lib, choice, wide = build.load("attention_tree"), _forced["attention"], dtype is torch.float32
-    args = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), F32 if wide else BF16, block_table.data_ptr(), table_rows, stride,
-            requests.data_ptr(), m, most_tokens, most_keys, ancestors.data_ptr(), words, positions.data_ptr(), n, pages, page_tokens, H, G, hd,
-            window, scale, softcap, 1 if sink else 0, _ptr(sinks))
+    if window >= 1 << 31:
+        window = 0                         # no position is that far
+    call = _tree_call(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), requests.data_ptr(),
+                      ancestors.data_ptr(), positions.data_ptr(), 0 if sinks is None else sinks.data_ptr(), pages, F32 if wide else BF16,
+                      table_rows, stride, m, most_tokens, most_keys, words, n, page_tokens, H, G, hd, window, 1 if sink else 0, scale, softcap)
     if (hd == 128 or hd == 64) and choice != "generic":
         rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
         # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor
@@ -1581,13 +1586,13 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
         cap = min(rows, tall)
         part = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
         at = part.data_ptr()
-        code = lib.hk_tree_attention(*args, 1, ctas, at, at + 8 * ctas * cap * hd, cap, 0 if wide else gemm_fast.status_flag(q.device).data_ptr(),
+        code = lib.hk_tree_attention(call, 1, ctas, at, at + 8 * ctas * cap * hd, cap, 0 if wide else gemm_fast.status_flag(q.device).data_ptr(),
                                      torch._C._cuda_getCurrentRawStream(dev))
         if code != _ERR_UNSUPPORTED:
             return _check(code, "tree_attention", 2 if ctas > 1 else 1)
     if choice not in (None, "generic"):
         raise KernelError(f"tree_attention: the '{choice}' kernel refuses head_dim={hd} page_tokens={page_tokens}")
-    _check(lib.hk_tree_attention(*args, 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
+    _check(lib.hk_tree_attention(call, 0, 0, 0, 0, 0, 0, _stream()), "tree_attention")
 
 
 def _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, positions, out, H, G, hd, page_tokens, scale, most_tokens, most_keys,
@@ -1627,11 +1632,12 @@ def _tree_checks(q, k_pages, v_pages, block_table, requests, ancestors, position
 
 
 _TREE_ROWS_TC, _TREE_ROWS_F32 = 256, 32      # rows of a tile (TC_ROWS twice, F32_ROWS in csrc/attention_tree.cu)
+_tree_call = struct.Struct("=10Q14i2f").pack        # `TreeCall` of attention_tree.cu
 
 
 def _one_device(first: torch.Tensor, *others) -> bool:
-    index = first.device.index
-    return all(t is None or t.device.index == index for t in others)
+    index = first.get_device()
+    return all(t is None or t.get_device() == index for t in others)
 
 
 def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, table_stride: int, page_tokens: int, heads: int,
@@ -1649,11 +1655,13 @@ def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, tabl
         raise KernelError("compact_rows: the sizes must be positive")
     if not _one_device(table, paths):
         raise KernelError("compact_rows: table and paths must be on one device")
-    if table.get_device() != torch._C._cuda_getDevice():
-        with torch.cuda.device(table.get_device()):
+    dev = table.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
             return compact_rows(table, paths, table_rows, table_stride, page_tokens, heads, row_bytes, num_pages)
     _check(build.load("branches").hk_compact_rows(table.data_ptr(), table.shape[0], paths.data_ptr(), paths.shape[0], paths.shape[1] - 2, table_rows,
-                                                  table_stride, page_tokens, heads, row_bytes, num_pages, _stream()), "compact_rows")
+                                                  table_stride, page_tokens, heads, row_bytes, num_pages, torch._C._cuda_getCurrentRawStream(dev)),
+           "compact_rows")
 
 
 def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> None:
@@ -1669,11 +1677,12 @@ def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> No
         raise KernelError("copy_blocks: most_bytes must be positive")
     if not _one_device(table, moves):
         raise KernelError("copy_blocks: table and moves must be on one device")
-    if table.get_device() != torch._C._cuda_getDevice():
-        with torch.cuda.device(table.get_device()):
+    dev = table.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
             return copy_blocks(table, moves, most_bytes)
-    _check(build.load("branches").hk_copy_blocks(table.data_ptr(), table.shape[0], moves.data_ptr(), moves.shape[0], most_bytes, _stream()),
-           "copy_blocks")
+    _check(build.load("branches").hk_copy_blocks(table.data_ptr(), table.shape[0], moves.data_ptr(), moves.shape[0], most_bytes,
+                                                torch._C._cuda_getCurrentRawStream(dev)), "copy_blocks")
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_beams: torch.Tensor,
@@ -1682,13 +1691,37 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     log softmax(logits[b, k])[v], best first, of equal ones the lowest k * vocab + v first.  logits float32 [prompts * n_beams,
     vocab], scores float32 [prompts * n_beams]; out_scores float32, out_beams (k) and out_tokens (v) int32 [prompts, choices].  A logit
     that is not finite counts as -inf, and so do all continuations of a beam whose score is not finite (one that is not there yet, or no
-    longer).  Up to 256 beams and 256 choices."""
+    longer).  Scores are compared in 64 bits; the exponentials in a beam's sum have 32, so continuations of two beams that lie within some
+    1e-7 of each other may come in either order (always the same one).  Up to 256 beams and 256 choices."""
+    # (the usual call in one condition, as in `tree_attention`)
+    f32, i32, dev = torch.float32, torch.int32, logits.get_device()
+    shape, size, row = out_scores.shape, logits.shape, scores.shape
+    if not (dev >= 0 and logits.dtype is f32 and scores.dtype is f32 and out_scores.dtype is f32 and out_beams.dtype is i32 and out_tokens.dtype is i32
+            and scores.get_device() == dev and out_scores.get_device() == dev and out_beams.get_device() == dev and out_tokens.get_device() == dev
+            and logits.is_contiguous() and scores.is_contiguous() and out_scores.is_contiguous() and out_beams.is_contiguous()
+            and out_tokens.is_contiguous() and len(size) == 2 and len(row) == 1 and len(shape) == 2 and out_beams.shape == shape
+            and out_tokens.shape == shape and size[0] == row[0] == shape[0] * n_beams and 1 <= n_beams <= 256
+            and 1 <= shape[1] <= 256 and shape[1] <= n_beams * size[1] and size[1] <= 1 << 30 and n_beams * size[1] < 1 << 31):
+        _beam_checks(logits, scores, n_beams, out_scores, out_beams, out_tokens)
+    (rows, vocab), (prompts, choices) = size, shape
+    if prompts == 0:
+        return
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, n_beams, out_scores, out_beams, out_tokens)
+    lib = build.load("branches")
+    scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
+    _check(lib.hk_beam_select(logits.data_ptr(), scores.data_ptr(), prompts, n_beams, vocab, choices, out_scores.data_ptr(), out_beams.data_ptr(),
+                              out_tokens.data_ptr(), scratch.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "beam_select", 2)
+
+
+def _beam_checks(logits, scores, n_beams, out_scores, out_beams, out_tokens) -> None:
     _need(logits, "logits", torch.float32, 2)
     _need(scores, "scores", torch.float32, 1)
     _need(out_scores, "out_scores", torch.float32, 2)
     _need(out_beams, "out_beams", torch.int32, 2)
     _need(out_tokens, "out_tokens", torch.int32, 2)
-    (rows, vocab), shape, dev = logits.shape, out_scores.shape, logits.get_device()
+    (rows, vocab), shape = logits.shape, out_scores.shape
     prompts, choices = shape
     if n_beams < 1 or rows != prompts * n_beams or scores.shape != (rows,):
         raise KernelError(f"beam_select: {rows} rows of logits and {scores.shape[0]} scores for {prompts} prompts of {n_beams} beams")
@@ -1698,15 +1731,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
         return
     if n_beams > 256 or not 1 <= choices <= min(256, n_beams * vocab) or vocab > 1 << 30 or n_beams * vocab >= 1 << 31:
         raise KernelError(f"beam_select: {choices} choices of {n_beams} beams and {vocab} tokens; up to 256 beams and 256 choices are taken, no more than there are")
-    if not (scores.get_device() == dev and out_scores.get_device() == dev and out_beams.get_device() == dev and out_tokens.get_device() == dev):
+    if not _one_device(logits, scores, out_scores, out_beams, out_tokens):
         raise KernelError("beam_select: all tensors must be on one device")
-    if dev != torch._C._cuda_getDevice():
-        with torch.cuda.device(dev):
-            return beam_select(logits, scores, n_beams, out_scores, out_beams, out_tokens)
-    lib = build.load("branches")
-    scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
-    _check(lib.hk_beam_select(logits.data_ptr(), scores.data_ptr(), prompts, n_beams, vocab, choices, out_scores.data_ptr(), out_beams.data_ptr(),
-                              out_tokens.data_ptr(), scratch.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "beam_select", 2)
 
 
 from . import attention_fast, gemm_fast  # noqa: E402  (they use this module; looked up once, not on each call)

@@ -126,7 +126,7 @@ def test_beam_selection_refuses_rows_that_its_indexes_do_not_hold(monkeypatch):
     monkeypatch.setattr(ops, "_need", lambda *a, **k: None)
 
     def fake(*shape):
-        return types.SimpleNamespace(shape=torch.Size(shape), get_device=lambda: 0)
+        return types.SimpleNamespace(shape=torch.Size(shape), dtype=None, get_device=lambda: 0)
     for vocab, beams in (((1 << 30) + 1, 1), (1 << 30, 2), (1 << 23, 256), (50, 257)):
         with pytest.raises(ops.KernelError, match="are taken"):
             ops.beam_select(fake(beams, vocab), fake(beams), beams, fake(1, 4), fake(1, 4), fake(1, 4))
