@@ -1647,19 +1647,22 @@ def compact_rows(table: torch.Tensor, paths: torch.Tensor, table_rows: int, tabl
     table_stride]) of tensors that the caller keeps; `paths` int32 [requests, 2 + width] = (slot, the tree's first row, its accepted
     rows in ascending order, -1 behind the last): accepted row i moves to the tree's row i; a slot has one path.  heads, row_bytes:
     the most of any array."""
-    _need(table, "table", torch.int64, 2)
-    _need(paths, "paths", torch.int32, 2)
-    if table.shape[1] != 4 or paths.shape[1] < 2:
-        raise KernelError("compact_rows: table must be [arrays, 4] and paths [requests, 2 + width]")
-    if min(table_rows, table_stride, page_tokens, heads, row_bytes, num_pages) < 1:
-        raise KernelError("compact_rows: the sizes must be positive")
-    if not _one_device(table, paths):
-        raise KernelError("compact_rows: table and paths must be on one device")
-    dev = table.get_device()
+    dev, arrays, path = table.get_device(), table.shape, paths.shape
+    if not (dev >= 0 and table.dtype is torch.int64 and paths.dtype is torch.int32 and paths.get_device() == dev and table.is_contiguous()
+            and paths.is_contiguous() and len(arrays) == 2 and len(path) == 2 and arrays[1] == 4 and path[1] >= 2 and table_rows >= 1
+            and table_stride >= 1 and page_tokens >= 1 and heads >= 1 and row_bytes >= 1 and num_pages >= 1):
+        _need(table, "table", torch.int64, 2)
+        _need(paths, "paths", torch.int32, 2)
+        if table.shape[1] != 4 or paths.shape[1] < 2:
+            raise KernelError("compact_rows: table must be [arrays, 4] and paths [requests, 2 + width]")
+        if min(table_rows, table_stride, page_tokens, heads, row_bytes, num_pages) < 1:
+            raise KernelError("compact_rows: the sizes must be positive")
+        if paths.get_device() != dev:
+            raise KernelError("compact_rows: table and paths must be on one device")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return compact_rows(table, paths, table_rows, table_stride, page_tokens, heads, row_bytes, num_pages)
-    _check(build.load("branches").hk_compact_rows(table.data_ptr(), table.shape[0], paths.data_ptr(), paths.shape[0], paths.shape[1] - 2, table_rows,
+    _check(build.load("branches").hk_compact_rows(table.data_ptr(), arrays[0], paths.data_ptr(), path[0], path[1] - 2, table_rows,
                                                   table_stride, page_tokens, heads, row_bytes, num_pages, torch._C._cuda_getCurrentRawStream(dev)),
            "compact_rows")
 
@@ -1669,19 +1672,21 @@ def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> No
     (address, blocks, pieces a block, bytes a piece, bytes a row) of tensors that the caller keeps; `moves` int32 [m, 3] = (from,
     to, rows): of each piece (a key head's rows of a page; a state is one piece and one row) the first `rows` rows are copied.  In one call no block
     is written twice, and none is both read and written.  most_bytes: the most that a block of any array has."""
-    _need(table, "table", torch.int64, 2)
-    _need(moves, "moves", torch.int32, 2)
-    if table.shape[1] != 5 or moves.shape[1] != 3:
-        raise KernelError("copy_blocks: table must be [arrays, 5] and moves [m, 3]")
-    if most_bytes < 1:
-        raise KernelError("copy_blocks: most_bytes must be positive")
-    if not _one_device(table, moves):
-        raise KernelError("copy_blocks: table and moves must be on one device")
-    dev = table.get_device()
+    dev, arrays, move = table.get_device(), table.shape, moves.shape
+    if not (dev >= 0 and table.dtype is torch.int64 and moves.dtype is torch.int32 and moves.get_device() == dev and table.is_contiguous()
+            and moves.is_contiguous() and len(arrays) == 2 and len(move) == 2 and arrays[1] == 5 and move[1] == 3 and most_bytes >= 1):
+        _need(table, "table", torch.int64, 2)
+        _need(moves, "moves", torch.int32, 2)
+        if table.shape[1] != 5 or moves.shape[1] != 3:
+            raise KernelError("copy_blocks: table must be [arrays, 5] and moves [m, 3]")
+        if most_bytes < 1:
+            raise KernelError("copy_blocks: most_bytes must be positive")
+        if moves.get_device() != dev:
+            raise KernelError("copy_blocks: table and moves must be on one device")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return copy_blocks(table, moves, most_bytes)
-    _check(build.load("branches").hk_copy_blocks(table.data_ptr(), table.shape[0], moves.data_ptr(), moves.shape[0], most_bytes,
+    _check(build.load("branches").hk_copy_blocks(table.data_ptr(), arrays[0], moves.data_ptr(), move[0], most_bytes,
                                                 torch._C._cuda_getCurrentRawStream(dev)), "copy_blocks")
 
 
