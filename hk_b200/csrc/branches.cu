@@ -15,7 +15,7 @@ struct BlockArray {
   long long address, blocks, pieces, piece, row;
 };
 
-constexpr int COPY_THREADS = 256, COPY_DEEP = 8;      // threads; vectors that a thread has on their way at once
+constexpr int COPY_THREADS = 128, COPY_DEEP = 8;      // threads; vectors that a thread has on their way at once
 
 template <typename V>
 __device__ __forceinline__ void copy_part(uint8_t* to, const uint8_t* from, long long pieces, long long piece, long long used) {
@@ -39,7 +39,10 @@ __device__ __forceinline__ void copy_part(uint8_t* to, const uint8_t* from, long
   }
 }
 
-__global__ void __launch_bounds__(COPY_THREADS)
+// Bound by DRAM: 7 pages of 128 KB in 72 arrays (67 MB, read and written) 13.7 us with the launch, 4.9 TB/s; 19 states of 1 MB in 36
+// arrays 167, 8.6 TB/s (part of it in L2).  Blocks of 256 threads (half as many a SM, for the registers): 15.6 and 170; four vectors a
+// thread on their way: 14.0 and 166; 2 states 22.9, 24.9 and 23.3.
+__global__ void __launch_bounds__(COPY_THREADS, 8)
 copy_blocks_kernel(const BlockArray* __restrict__ table, const int* __restrict__ moves) {
   const BlockArray a = table[blockIdx.z];
   const int from = moves[3 * blockIdx.y], to = moves[3 * blockIdx.y + 1], rows = moves[3 * blockIdx.y + 2];
