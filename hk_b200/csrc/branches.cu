@@ -44,6 +44,8 @@ __device__ __forceinline__ void copy_part(uint8_t* to, const uint8_t* from, long
 // thread on their way: 14.0 and 166; 2 states 22.9, 24.9 and 23.3.
 __global__ void __launch_bounds__(COPY_THREADS, 8)
 copy_blocks_kernel(const BlockArray* __restrict__ table, const int* __restrict__ moves) {
+  pdl_launch_dependents();
+  pdl_wait();
   const BlockArray a = table[blockIdx.z];
   const int from = moves[3 * blockIdx.y], to = moves[3 * blockIdx.y + 1], rows = moves[3 * blockIdx.y + 2];
   if (from < 0 || to < 0 || from >= a.blocks || to >= a.blocks || from == to || rows <= 0) return;
@@ -85,13 +87,16 @@ __device__ __forceinline__ void move_rows(const RowArray& a, const int2* from, c
 
 // A block takes a request and some neighbouring arrays, and finds the pages of its path once for all that share a block table: finding
 // them is a chain of three reads, and as long as moving an array's rows.  Bound by the reads' and writes' way through DRAM in pieces of
-// a row of a head (256 bytes): 64 requests of up to nine rows in 72 arrays, 42 MB, take 14.4 us, 2.9 TB/s (blocks of 256 threads 17.4, of
-// 64 14.4; four reads a thread on their way 16.5); 16 requests 6.2.
+// a row of a head (256 bytes): 64 requests of up to nine rows in 72 arrays, 42 MB, take 13.4 us one call behind the other, 3.2 TB/s, and
+// 15.5 as replays over three caches in turn (over two, which partly stay in L2: 14.4, in blocks of 256 threads 17.4, of 64 14.4, with
+// four reads a thread on their way 16.5, 16 requests 6.2).
 __global__ void __launch_bounds__(KEEP_THREADS, 8)
 compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_block, const int* __restrict__ paths, int width, int table_rows,
                     int table_stride, int page_tokens, long long num_pages) {
   __shared__ int2 from[KEEP_PATH], to[KEEP_PATH];
   __shared__ int count;
+  pdl_launch_dependents();
+  pdl_wait();
   const int* path = paths + (size_t)blockIdx.x * (width + 2);
   const int slot = path[0], first = path[1], a0 = blockIdx.y * per_block, a1 = min(arrays, a0 + per_block);
   if (slot < 0 || slot >= table_rows || first < 0) return;
@@ -159,9 +164,13 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
 // keeps a sum of exponentials a thread against a reference of its own (a tile's sixteen in float32, all beyond that in 64 bits) and the
 // largest of each thread's sixteen.  When the part is through, a bar is found that at least `choices` of those reach, and only the few
 // sixteens that reach it are read again for the tokens that can be among the part's best.  (Looking for them on the way took a barrier
-// a tile and, with some lane over the bar in most tiles, one and a half times the instructions.)  A CTA a prompt
-// then joins the parts' sums, scores the parts' tokens in 64 bits and ranks them: rounded to float32, scores of some -10 lie 1e-6 apart,
-// and neighbours among a million would be equal often enough.  What is left is the error of the exponentials, some 1e-8 of a sum.
+// a tile and, with some lane over the bar in most tiles, one and a half times the instructions: 42 us for 28.)  A CTA a prompt then joins
+// the parts' sums, scores the parts' tokens in 64 bits and ranks them: rounded to float32, scores of some -10 lie 1e-6 apart, and
+// neighbours among a million would be equal often enough.  What is left is the error of the exponentials, some 1e-8 of a sum.
+//
+// Time: some 15 us of dependent steps (start, bar, read again, sums, rank) and the stream at DRAM's rate: 4, 8 and 16 prompts of 8 beams
+// over 151,936 tokens take 18.5, 21.9 and 28.2 us (39 MB more: 6.3 us, 6.2 TB/s), a prompt of 4 beams 12.3, of 128 with 256 choices 132.
+// (Blocks of 128 threads, eight a SM: 37.9; tiles asked into L2 ahead: 28.5 to 30.8.)
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
 constexpr int BC = 2048;              // candidates that are ranked side by side; more than that only among equal logits
@@ -673,7 +682,7 @@ HK_API int hk_copy_blocks(const long long* table, int arrays, const int* moves, 
   if (arrays <= 0 || n_moves <= 0 || most_bytes <= 0) return 0;
   if (arrays > 65535 || n_moves > 65535) return HK_ERR_UNSUPPORTED;
   const long long part = 16LL * COPY_THREADS * COPY_DEEP, blocks = (most_bytes + part - 1) / part;
-  return hk_launch(copy_blocks_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)n_moves, (unsigned)arrays), dim3(COPY_THREADS), 0,
+  return hk_launch_pdl(copy_blocks_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)n_moves, (unsigned)arrays), dim3(COPY_THREADS), 0,
                    (cudaStream_t)stream, reinterpret_cast<const BlockArray*>(table), moves);
 }
 
@@ -690,7 +699,7 @@ HK_API int hk_compact_rows(const long long* table, int arrays, const int* paths,
   // one wave of blocks (eight a SM) where that is up to 8 arrays a block
   int per_block = (int)(((long long)arrays * requests + 148 * 8 - 1) / (148 * 8));
   per_block = per_block < 1 ? 1 : per_block > 8 ? 8 : per_block;
-  return hk_launch(compact_rows_kernel, dim3((unsigned)requests, (unsigned)((arrays + per_block - 1) / per_block)), dim3(KEEP_THREADS), 0,
+  return hk_launch_pdl(compact_rows_kernel, dim3((unsigned)requests, (unsigned)((arrays + per_block - 1) / per_block)), dim3(KEEP_THREADS), 0,
                    (cudaStream_t)stream, reinterpret_cast<const RowArray*>(table), arrays, per_block, paths, width, table_rows, table_stride, page_tokens,
                    num_pages);
 }
