@@ -606,6 +606,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// x0, x1 times a plus b, and x0, x1 plus y0, y1: two float32 numbers an instruction, rounded as one by one
+__device__ __forceinline__ void fma_two(float& x0, float& x1, float a, float b) {
+  asm("{\n\t.reg .b64 x, f, s;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmov.b64 s, {%3, %3};\n\tfma.rn.f32x2 x, x, f, s;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}" : "+f"(x0), "+f"(x1) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add_two(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+}
 __device__ __forceinline__ float ex2(float x) {      // 2^x, one instruction; 2^-inf = 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -1014,10 +1023,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = ex2(fmaf(__uint_as_float(su[2 * e]), sl, shift));
-            const float p1 = ex2(fmaf(__uint_as_float(su[2 * e + 1]), sl, shift));
-            l0 += p0;
-            l1 += p1;
+            float p0 = __uint_as_float(su[2 * e]), p1 = __uint_as_float(su[2 * e + 1]);
+            fma_two(p0, p1, sl, shift);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            add_two(l0, l1, p0, p1);
             const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
             pw[e] = *reinterpret_cast<const uint32_t*>(&pk);
           }
