@@ -496,7 +496,7 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 //
 // Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits).  They are taken against a reference, an
 // integer near the largest score of the first tile in which a row sees anything: bfloat16 and the sums in float32 have exponents to
-// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference two
+// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference three
 // tiles later, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
 // threads need not meet over it.  Where one tile jumps by more than 2^60 the row's sum is set to NaN, and the row is taken again (below).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 128;
@@ -646,9 +646,9 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][TC_ROWS * HD * 2];
   alignas(1024) uint8_t k[STAGES][TC_KEYS * HD * 2];
   alignas(1024) uint8_t v[STAGES][TC_KEYS * HD * 2];
-  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2][2], p_full[2][2], o_done[2], drained[2], pair[2][4];
-  float first[2][2][2][TC_ROWS], asked[4][2][2][TC_ROWS];   // [tile % 2][group][half of the keys][row]: a first tile's largest score;
-                                                            // [tile % 4]..: the reference asked for
+  alignas(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[2][2], p_full[2][2], o_done[2], drained[2], pair[2][4], turn[2];
+  float first[2][2][2][TC_ROWS], asked[8][2][2][TC_ROWS];   // [tile % 2][group][half of the keys][row]: a first tile's largest score;
+                                                            // [tile % 8]..: the reference asked for
   float2 ml[2][2][TC_ROWS];   // the reference and the sum
   Walk start;                 // the share behind its first segment
   Segment lead;               // its first segment, if it has any
@@ -754,6 +754,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       }
       mbar_init(&sm.o_done[i], 1);
       mbar_init(&sm.drained[i], 1);
+      mbar_init(&sm.turn[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&sm.pair[i][j], 2);
     }
     sm.abort_flag = 0;
@@ -837,7 +838,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const uint32_t x = __shfl_sync(0xffffffffu, (uint32_t)(warp - MMA_WARP), 0);
     if (elect_one()) {
       bool ok = true, issued = false;
-      uint32_t tiles_done = 0, steps = 0, seg = 0;
+      uint32_t tiles_done = 0, steps = 0, seg = 0, turns = x ^ 1;      // (the first turn is the first group's)
       const uint32_t sp = tmem + x * SP_COL[1], oc = tmem + O_COL[0] + x * HD;
       const uint64_t dq0 = desc_k_major(smem_u32(sm.q[0])), dk0 = desc_k_major(smem_u32(sm.k[0])), dv0 = desc_mn_major(smem_u32(sm.v[0]), TC_KEYS * 128);
       constexpr uint32_t STAGE16 = TC_KEYS * HD * 2 >> 4, HALF16 = TC_KEYS / 2 * 128 >> 4;      // descriptors count in 16 bytes
@@ -876,7 +877,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           for (int h = 0; h < 2; ++h) {
             if (!ok) break;
             if (!mbar_wait(&sm.p_full[x][h], (steps + t) & 1u, abort_flag) ||
-                (h == 0 && !mbar_wait(&sm.v_full[st], (n / STAGES) & 1u, abort_flag))) { ok = false; break; }
+                (h == 0 && !mbar_wait(&sm.v_full[st], (n / STAGES) & 1u, abort_flag)) ||
+                (two && !mbar_wait(&sm.turn[x], turns++ & 1u, abort_flag))) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < TC_KEYS / 32; ++kk)
@@ -887,6 +889,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             if (t + 1 < jobs) ok = issue_s(h, next);       // behind this stream's product with V: it overwrites the P that it reads
             else if (h == 1) umma_commit(&sm.o_done[x]);
+            if (two) mbar_arrive(&sm.turn[x ^ 1]);
           }
           n = next;
         }
@@ -940,11 +943,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       const int jobs = two ? s.n : (s.n + 1 - x) / 2;
       float m = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
       for (int n = 0; n < jobs; ++n, ++jobs_done) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x][half], jobs_done & 1u, abort_flag))) { ok = false; break; }
-        if (!busy) {
-          if (lane == 0) mbar_arrive(&sm.p_full[x][half]);
-          continue;
-        }
+        // what can be done while the scores are on their way
         const int j0 = (t0 + (two ? n : 2 * n + x)) * TC_KEYS + half * HK;
         const bool part = j0 < lo || j0 + HK > context;
         uint32_t see[2] = {0xffffffffu, 0xffffffffu}, su[32];
@@ -952,6 +951,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           const TreeRow tr = tree_row(a, s.q, token, valid);
           see[0] = visible32(tr, j0);
           see[1] = visible32(tr, j0 + 32);
+        }
+        // m is alike in a row's two threads, and so are the branches that they take
+        const bool fresh = __any_sync(0xffffffffu, valid && m == -CUDART_INF_F);
+        float asked = m;
+        // what the two asked for three tiles ago: the tensor core's thread had seen both announce it before it issued the last tile's scores
+        if (n >= 3) asked = fmaxf(sm.asked[(n - 3) & 7][x][0][r], sm.asked[(n - 3) & 7][x][1][r]);
+        const bool moves = __any_sync(0xffffffffu, asked > m);
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[x][half], jobs_done & 1u, abort_flag))) { ok = false; break; }
+        if (!busy) {
+          if (lane == 0) mbar_arrive(&sm.p_full[x][half]);
+          continue;
         }
         tc_fence_after();
         // 32 of the thread's scores, capped and in the exponent's domain but for the factor sl, -inf where they do not count
@@ -967,8 +977,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             for (int i = 0; i < 32; ++i) su[i] = ((c ? see[1] : see[0]) >> i) & 1u ? su[i] : 0xff800000u;
           }
         };
-        // m is alike in a row's two threads, and so are the branches that they take
-        if (__any_sync(0xffffffffu, valid && m == -CUDART_INF_F)) {
+        if (fresh) {
           float top = -CUDART_INF_F;
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
@@ -984,36 +993,32 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           if (!__all_sync(0xffffffffu, mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag))) { ok = false; break; }
           ++met;
           if (m == -CUDART_INF_F) m = ceilf(fmaxf(sm.first[n & 1][x][0][r], sm.first[n & 1][x][1][r]));
-        } else if (n >= 2) {
-          // what the two asked for two tiles ago: the tensor core's thread had seen both announce it before it issued these scores
-          const float asked = fmaxf(sm.asked[(n - 2) & 3][x][0][r], sm.asked[(n - 2) & 3][x][1][r]);
-          if (__any_sync(0xffffffffu, asked > m)) {
-            // O may be touched: this half's product with V of the last tile is complete, since these scores are, and the other half's is
-            // once its scores are; the next ones wait for the two warps, which meet when both have done their part of the dims
-            bool fine = mbar_wait(&sm.s_full[x][half ^ 1], jobs_done & 1u, abort_flag);
-            tc_fence_after();
-            const float corr = asked > m ? exp2f(m - asked) : 1.0f;
-            l0 *= corr;
-            l1 *= corr;
+        } else if (moves) {
+          // O may be touched: this half's product with V of the last tile is complete, since these scores are, and the other half's is
+          // once its scores are; the next ones wait for the two warps, which meet when both have done their part of the dims
+          bool fine = mbar_wait(&sm.s_full[x][half ^ 1], jobs_done & 1u, abort_flag);
+          tc_fence_after();
+          const float corr = asked > m ? exp2f(m - asked) : 1.0f;
+          l0 *= corr;
+          l1 *= corr;
 #pragma unroll 1
-            for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 16) {
-              uint32_t o[16];
-              tmem_ld16(oc + (uint32_t)c0, o);
-              tmem_ld_wait();
+          for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16(oc + (uint32_t)c0, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st16(oc + (uint32_t)c0, o);
-            }
-            m = fmaxf(m, asked);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.pair[x][quarter]);
-            fine = mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag) && fine;
-            tc_fence_after();
-            if (!__all_sync(0xffffffffu, fine)) { ok = false; break; }
-            ++met;
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(oc + (uint32_t)c0, o);
           }
+          m = fmaxf(m, asked);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.pair[x][quarter]);
+          fine = mbar_wait(&sm.pair[x][quarter], met & 1u, abort_flag) && fine;
+          tc_fence_after();
+          if (!__all_sync(0xffffffffu, fine)) { ok = false; break; }
+          ++met;
         }
         const float shift = m == -CUDART_INF_F ? 0.f : -m, l_before = l0 + l1;
         // a half's P lies in the columns of its own scores that are read already (a loop: a short call waits for its instructions)
@@ -1042,7 +1047,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             ask = m;
           }
         }
-        sm.asked[n & 3][x][half][r] = ask;
+        sm.asked[n & 7][x][half][r] = ask;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
