@@ -16,8 +16,8 @@
 //
 // Measured (32 heads over 8 key heads of 128, captured and replayed): 16 tokens behind 2,000 rows 16.5 us, all of it the start and end of
 // the two kernels (8.5 MB); 8 requests of 32 tokens, ragged up to 8,000 rows, 41 us (122 MB, 3.0 TB/s); 32 requests of 64 tokens behind up to
-// 8,192 rows 198 us (680 MB, 3.4 TB/s, 580 TFLOP/s); 64 tokens behind 131,001 rows 154 us (895 TFLOP/s); the last two at the power cap,
-// called again and again for a second, 225 and 180.  The generic kernel took 391, 4,463, 47,593 and 76,055.
+// 8,192 rows 183 us (680 MB, 3.7 TB/s, 630 TFLOP/s); 64 tokens behind 131,001 rows 144 us (955 TFLOP/s); the last two at the power cap,
+// called again and again for a second, 214 and 168.  The generic kernel took 391, 4,463, 47,593 and 76,055.
 //
 // What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays or the bounds is
 // skipped, and a page outside the pool is not read.
@@ -489,16 +489,16 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 // behind its product with V; products of one thread run in order, so they overwrite P only once it was read.  (One lane for both groups was
 // what the kernel waited for: a product takes it some 40 clocks to issue, and a tile of 256 rows is 48 of them.)
 //
-// Bound by the hand-overs: a stream takes some 3,700 clocks a tile of 256 rows, of which the tensor core and the exponentials need 2,048
-// each.  Behind one long context the tensor pipe is active 37 % of the time, the unit of the exponentials as much, issue slots 42 %.
-// (64 tokens behind 131,001 rows: 157 us; scores read 16 at a time with two reads on their way 162, an eighth to a quarter of the
-// exponentials by a polynomial 165 to 170.)
+// With two row tiles the two lanes issue a stream's product with V and its next scores in turns.  Side by side, both groups' products end
+// at the same time, then their exponentials run at the same time, and each unit waits for the other (151 us for 143 below); in turns the
+// four streams keep a quarter apart.  With one row tile (every lane's next keys come when they come) that waits for more than it saves.
 //
-// Probabilities are rounded to bfloat16 for the tensor core (the sum of a row keeps 32 bits).  They are taken against a reference, an
-// integer near the largest score of the first tile in which a row sees anything: bfloat16 and the sums in float32 have exponents to
-// spare, so a score may run ahead of it and nothing is lost.  A tile whose probabilities sum to more than 2^24 moves the reference three
-// tiles later, by a power of two, which rounds nothing.  So no tile but the first is looked through for its maximum, and a row's two
-// threads need not meet over it.  Where one tile jumps by more than 2^60 the row's sum is set to NaN, and the row is taken again (below).
+// Bound by a stream's own way around, some 3,500 clocks a tile: 170 until the first scores are in registers, 1,200 of exponentials (512
+// alone), 300 until the tensor core's lane has seen them and has its turn, 900 for the products and their announcement, of which shared
+// memory's bandwidth takes 640 (a product of 64 keys reads 128 rows of Q: 6 KB in 32 clocks' work).  The exponentials' unit is active 58 %
+// of that, shared memory 73 %.  (64 tokens behind 131,001 rows, 144 us: scores of 128 keys at once, two streams, 153; an eighth, a
+// quarter and a third of the exponentials by a polynomial 145, 146 and 147; the turn passed on behind the product with V 145; tiles asked
+// into L2 ahead 148.)
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 128;
 typedef Cut<2 * TC_ROWS, TC_KEYS, 4> TcCut;
 constexpr float MUCH = 16777216.0f, TOO_MUCH = 1152921504606846976.0f;      // 2^24, 2^60
