@@ -704,17 +704,10 @@ HK_API int hk_compact_rows(const long long* table, int arrays, const int* paths,
                    num_pages);
 }
 
-// Bytes of scratch (16-byte aligned) that hk_beam_select wants.
-HK_API long long hk_beam_select_scratch(int rows, int V, int choices) {
-  if (rows <= 0 || V <= 0 || choices <= 0) return 0;
-  int parts, length;
-  beam_cut(rows, V, &parts, &length);
-  return (long long)rows * parts * ((long long)sizeof(RowPart) + 8LL * choices);
-}
-
-// logits float32 [prompts * beams, V], scores float32 [prompts * beams]; out_* [prompts, choices].
+// logits float32 [prompts * beams, V], scores float32 [prompts * beams]; out_* [prompts, choices]; scratch (16-byte aligned) of
+// max(592, prompts * beams) * (16 + 8 * choices) bytes: rows have no more parts together than that.
 HK_API int hk_beam_select(const float* logits, const float* scores, int prompts, int beams, int V, int choices, float* out_scores,
-                          int* out_beams, int* out_tokens, void* scratch, void* stream) {
+                          int* out_beams, int* out_tokens, void* scratch, long long scratch_bytes, void* stream) {
   if (prompts <= 0) return 0;
   if (beams < 1 || beams > BEAM_MOST || V < 1 || V > (1 << 30) || choices < 1 || choices > BEAM_MOST || (long long)beams * V > 0x7fffffffLL ||
       choices > (long long)beams * V || (long long)prompts * beams > 0x7fffffffLL || (((uintptr_t)scratch) & 15) != 0)
@@ -723,6 +716,7 @@ HK_API int hk_beam_select(const float* logits, const float* scores, int prompts,
   int parts, length;
   beam_cut(rows, V, &parts, &length);
   if ((long long)rows * parts > 0x7fffffffLL || (long long)beams * parts * choices > 0x7fffffffLL) return HK_ERR_UNSUPPORTED;
+  if (scratch_bytes < (long long)rows * parts * ((long long)sizeof(RowPart) + 8LL * choices)) return HK_ERR_UNSUPPORTED;
   RowPart* part = static_cast<RowPart*>(scratch);
   float* part_x = reinterpret_cast<float*>(part + (size_t)rows * parts);
   int* part_i = reinterpret_cast<int*>(part_x + (size_t)rows * parts * choices);

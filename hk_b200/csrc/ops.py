@@ -1690,6 +1690,9 @@ def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> No
                                                 torch._C._cuda_getCurrentRawStream(dev)), "copy_blocks")
 
 
+_BEAM_PARTS = 592      # CTAs of a wave, among which rows are cut (`hk_beam_select` in csrc/branches.cu refuses less scratch than it uses)
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_scores: torch.Tensor, out_beams: torch.Tensor,
                 out_tokens: torch.Tensor) -> None:
     """The best continuations of beams: of all beams k of a prompt and tokens v the out_scores.shape[1] with the largest scores[b, k] +
@@ -1714,10 +1717,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return beam_select(logits, scores, n_beams, out_scores, out_beams, out_tokens)
-    lib = build.load("branches")
-    scratch = torch.empty(lib.hk_beam_select_scratch(rows, vocab, choices), dtype=torch.uint8, device=logits.device)
-    _check(lib.hk_beam_select(logits.data_ptr(), scores.data_ptr(), prompts, n_beams, vocab, choices, out_scores.data_ptr(), out_beams.data_ptr(),
-                              out_tokens.data_ptr(), scratch.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)), "beam_select", 2)
+    size = max(_BEAM_PARTS, rows) * (16 + 8 * choices)
+    scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    _check(build.load("branches").hk_beam_select(logits.data_ptr(), scores.data_ptr(), prompts, n_beams, vocab, choices, out_scores.data_ptr(),
+                                                 out_beams.data_ptr(), out_tokens.data_ptr(), scratch.data_ptr(), size,
+                                                 torch._C._cuda_getCurrentRawStream(dev)), "beam_select", 2)
 
 
 def _beam_checks(logits, scores, n_beams, out_scores, out_beams, out_tokens) -> None:
