@@ -1574,15 +1574,17 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
                       table_rows, stride, m, most_tokens, most_keys, words, n, page_tokens, H, G, hd, window, 1 if sink else 0, scale, softcap)
     if (hd == 128 or hd == 64) and choice != "generic":
         rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
-        # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor
-        # cores of two: one for either group of warps
+        # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor cores of
+        # two, one for either group of warps, but of no more units than one: two short ones take a CTA twice as long (16 tokens
+        # behind 100 rows: 18.5 us for 12.3).  A unit of a few tiles is cut all the same: whole ones of 4 tiles and more take longer.
         held = all_keys if all_keys > 0 else m * most_keys
         if window > 0:
             held = min(held, m * (window + most_tokens))
         tall = most_tokens * (H // G)
-        tiles = -(-tall // rows) * G * (held // keys + m)
+        units = -(-tall // rows) * G
+        tiles = units * (held // keys + m)
         sms = gemm_fast._sms(q.device)
-        ctas = max(1, min(sms * 2, tiles) if wide else min(sms, (tiles + 1) // 2))
+        ctas = max(1, min(sms * 2, tiles) if wide else min(sms, max(units * m, (tiles + 1) // 2)))
         cap = min(rows, tall)
         part = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
         at = part.data_ptr()
