@@ -16,8 +16,8 @@
 //
 // Measured (32 heads over 8 key heads of 128, captured and replayed): 16 tokens behind 2,000 rows 16.5 us, all of it the start and end of
 // the two kernels (8.5 MB); 8 requests of 32 tokens, ragged up to 8,000 rows, 41 us (122 MB, 3.0 TB/s); 32 requests of 64 tokens behind up to
-// 8,192 rows 183 us (680 MB, 3.7 TB/s, 630 TFLOP/s); 64 tokens behind 131,001 rows 144 us (955 TFLOP/s); the last two at the power cap,
-// called again and again for a second, 214 and 168.  The generic kernel took 391, 4,463, 47,593 and 76,055.
+// 8,192 rows 182 us (680 MB, 3.7 TB/s, 632 TFLOP/s); 64 tokens behind 131,001 rows 142 us (968 TFLOP/s); the last two at the power cap,
+// called again and again for a second, 210 and 165.  The generic kernel took 391, 4,463, 47,593 and 76,055.
 //
 // What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays or the bounds is
 // skipped, and a page outside the pool is not read.
@@ -319,7 +319,9 @@ __global__ void __launch_bounds__(CW * 32) tree_combine_kernel(const TreeArgs a,
   const int token = token_of(a, row0 + row), head = g * a.group + row0 + row - token * a.group;
   pdl_wait();
   if (row >= rows) return;
-  constexpr int DEEP = 8;                // parts on their way at once
+  // parts on their way at once: in float32 there are more (1,500 rows: 24.5 us with 12, 26.7 with 8); in bfloat16 there are more rows, and
+  // blocks of more registers leave some waiting (8 ragged requests: 40.9 us with 8, 43.4 with 12)
+  constexpr int DEEP = sizeof(T) == 4 ? 12 : 8;
   float m = -CUDART_INF_F, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -1215,12 +1217,13 @@ int launch_tc(const TreeArgs& a, int ctas, cudaStream_t s) {
 }
 
 // ---- float32 ------------------------------------------------------------------------------------------------------------------
-// A tile has 32 rows, keys come 64 at a time through shared memory, and scores and sums are register tiles of multiply-adds over
-// 16-byte loads (4 x 4 scores a thread along the head's dims, 4 rows x HD / 16 dims of sums).  The next tile's keys arrive while this
-// one's probabilities are made, the next values while the next scores are.  Bound by the shared-memory reads beside the multiply-adds and
-// by its start and end: 2 requests of 15 tokens behind 1,500 rows (16 heads over 8 of 128) 30 us (the generic kernel 334), 19 MB and 0.27
-// GFLOP, 3.7 us at the multiply-adds' peak.
-constexpr int F32_ROWS = 32, F32_KEYS = 64, F32_THREADS = 128, F32_LDP = F32_KEYS + 4;
+// A tile has 32 rows, keys come 32 at a time through shared memory, and scores and sums are register tiles of multiply-adds over
+// 16-byte loads (4 x 2 scores a thread along the head's dims, 4 rows x HD / 16 dims of sums).  The next tile's keys arrive while this
+// one's probabilities are made, the next values while the next scores are.  Bound by the shared-memory reads beside the multiply-adds, by
+// start and end and by shares of whole tiles: 2 requests of 15 tokens behind 1,500 rows (16 heads over 8 of 128) 24.5 us (the generic
+// kernel 334), 19 MB and 0.27 GFLOP, 3.7 us at the multiply-adds' peak.  In tiles of 64 keys, two CTAs a SM, that takes 30.8 us, behind
+// 3,000 rows 41.0 for 31.1, 8 requests of 64 tokens behind up to 4,000 197 for 191, but 2 behind 20 rows 14.4 for 16.4.
+constexpr int F32_ROWS = 32, F32_KEYS = 32, F32_THREADS = 128, F32_LDP = F32_KEYS + 4;
 typedef Cut<F32_ROWS, F32_KEYS, 1> F32Cut;
 
 template <int HD>
@@ -1229,14 +1232,14 @@ struct F32Smem {
   float q[F32_ROWS * LD], k[F32_KEYS * LD], v[F32_KEYS * LD], p[F32_ROWS * F32_LDP];
   float corr[F32_ROWS], inv[F32_ROWS];
   float2 ml[F32_ROWS];
-  uint32_t see[F32_ROWS][2];
+  uint32_t see[F32_ROWS][F32_KEYS / 32];
   long long at[2][F32_KEYS];      // [parity of the tile]: where a key's row lies in the pages, -1 where there is none
   Walk start;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs a) {
-  constexpr int LD = F32Smem<HD>::LD, C4 = HD / 4, B = HD / 64, RI = F32_ROWS / 8;
+__global__ void __launch_bounds__(F32_THREADS, 4) tree_f32_kernel(const TreeArgs a) {
+  constexpr int LD = F32Smem<HD>::LD, C4 = HD / 4, B = HD / 64, RI = F32_ROWS / 8, WORDS = F32_KEYS / 32, KJ = F32_KEYS / 16;
   extern __shared__ __align__(16) uint8_t f32_raw[];
   F32Smem<HD>& sm = *reinterpret_cast<F32Smem<HD>*>(f32_raw);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.group;
@@ -1280,9 +1283,9 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
       *reinterpret_cast<float4*>(sm.q + r * LD + d) = make_float4(x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale);
     }
     const float cap = a.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
-    const TreeRow tr = tree_row(a, s.q, token_of(a, s.row0 + (tid >> 1)), tid < 2 * F32_ROWS && (tid >> 1) < s.rows);     // of row tid / 2
+    const TreeRow tr = tree_row(a, s.q, token_of(a, s.row0 + tid / WORDS), tid < WORDS * F32_ROWS && tid / WORDS < s.rows);     // of row tid / WORDS
     // the softmax's state of row tid / 4, alike in its four threads
-    const int sr = tid >> 2, sc = (tid & 3) * 16;
+    const int sr = tid >> 2, sc = (tid & 3) * 4 * KJ;
     float m = -CUDART_INF_F, l = 0.f;
     float4 acc[RI][B];
 #pragma unroll
@@ -1292,37 +1295,37 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
     for (int t = 0; t < s.n; ++t) {
       const int j0 = (s.t0 + t) * F32_KEYS;
       bool part = false;
-      if (tid < 2 * F32_ROWS) {
-        const uint32_t see = visible32(tr, j0 + 32 * (tid & 1));
-        sm.see[tid >> 1][tid & 1] = see;
-        part = (tid >> 1) < s.rows && see != 0xffffffffu;
-      } else if (t + 1 < s.n) {
-        find(t + 1, tid - 2 * F32_ROWS);
+      if (tid < WORDS * F32_ROWS) {
+        const uint32_t see = visible32(tr, j0 + 32 * (tid % WORDS));
+        sm.see[tid / WORDS][tid % WORDS] = see;
+        part = tid / WORDS < s.rows && see != 0xffffffffu;
+      } else if (t + 1 < s.n && tid - WORDS * F32_ROWS < F32_KEYS) {
+        find(t + 1, tid - WORDS * F32_ROWS);
       }
       cp_async_wait<1>();          // the keys
       part = __syncthreads_or(part);
-      float x[RI][4];
+      float x[RI][KJ];
 #pragma unroll
       for (int i = 0; i < RI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+        for (int j = 0; j < KJ; ++j) x[i][j] = 0.f;
 #pragma unroll 2
       for (int d = 0; d < HD; d += 4) {
-        float4 u[RI], v[4];
+        float4 u[RI], v[KJ];
 #pragma unroll
         for (int i = 0; i < RI; ++i) u[i] = *reinterpret_cast<const float4*>(sm.q + (ty + 8 * i) * LD + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * j) * LD + d);
+        for (int j = 0; j < KJ; ++j) v[j] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * j) * LD + d);
 #pragma unroll
         for (int i = 0; i < RI; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[i][j] = fmaf(u[i].w, v[j].w, fmaf(u[i].z, v[j].z, fmaf(u[i].y, v[j].y, fmaf(u[i].x, v[j].x, x[i][j]))));
+          for (int j = 0; j < KJ; ++j) x[i][j] = fmaf(u[i].w, v[j].w, fmaf(u[i].z, v[j].z, fmaf(u[i].y, v[j].y, fmaf(u[i].x, v[j].x, x[i][j]))));
       }
 #pragma unroll
       for (int i = 0; i < RI; ++i) {
         const int r = ty + 8 * i;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < KJ; ++j) {
           const int key = tx + 16 * j;
           float y = x[i][j];
           if (cap > 0.f) y = cap * tanhf(y * inv_cap);
@@ -1334,10 +1337,10 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
       else cp_async_commit();
       {
         float* row = sm.p + sr * F32_LDP + sc;
-        float4 y[4];
+        float4 y[KJ];
         float top = -CUDART_INF_F;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < KJ; ++e) {
           y[e] = *reinterpret_cast<const float4*>(row + 4 * e);
           top = fmaxf(top, fmaxf(fmaxf(y[e].x, y[e].y), fmaxf(y[e].z, y[e].w)));
         }
@@ -1347,7 +1350,7 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
         const float corr = expf(m - safe);                          // m = -inf: 0
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < KJ; ++e) {
           y[e] = make_float4(expf(y[e].x - safe), expf(y[e].y - safe), expf(y[e].z - safe), expf(y[e].w - safe));
           sum += (y[e].x + y[e].y) + (y[e].z + y[e].w);
           *reinterpret_cast<float4*>(row + 4 * e) = y[e];
@@ -1399,7 +1402,7 @@ __global__ void __launch_bounds__(F32_THREADS, 2) tree_f32_kernel(const TreeArgs
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
           const int r = ty + 8 * i;
-          for (int word = 0; word < 2; ++word)
+          for (int word = 0; word < WORDS; ++word)
             for (uint32_t left = sm.see[r][word]; left; left &= left - 1) {
               const int c = 32 * word + __ffs(left) - 1;
               const float f = sm.p[r * F32_LDP + c];

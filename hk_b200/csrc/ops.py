@@ -1573,10 +1573,11 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
                       ancestors.data_ptr(), positions.data_ptr(), 0 if sinks is None else sinks.data_ptr(), pages, F32 if wide else BF16,
                       table_rows, stride, m, most_tokens, most_keys, words, n, page_tokens, H, G, hd, window, 1 if sink else 0, scale, softcap)
     if (hd == 128 or hd == 64) and choice != "generic":
-        rows, keys = (_TREE_ROWS_F32, 64) if wide else (_TREE_ROWS_TC, 128)
-        # equal shares of all tiles of keys for one wave of CTAs (two a SM in float32), of a tile at least, on the tensor cores of
-        # two, one for either group of warps, but of no more units than one: two short ones take a CTA twice as long (16 tokens
-        # behind 100 rows: 18.5 us for 12.3).  A unit of a few tiles is cut all the same: whole ones of 4 tiles and more take longer.
+        rows, keys = (_TREE_ROWS_F32, 32) if wide else (_TREE_ROWS_TC, 128)
+        # Equal shares of all tiles of keys for one wave of CTAs.  On the tensor cores a CTA takes two tiles, one for either group of
+        # warps, but no two units: two short ones take it twice as long (16 tokens behind 100 rows: 18.5 us for 12.3).  In float32 two CTAs a
+        # SM, a tile each, and four of four tiles and more (2 requests behind 1,500 rows: 24.5 us with two, 29.6 with four, whose parts
+        # take longer to merge; 8 of 64 tokens behind 4,000: 223 and 187); units of two tiles are not cut.
         held = all_keys if all_keys > 0 else m * most_keys
         if window > 0:
             held = min(held, m * (window + most_tokens))
@@ -1584,7 +1585,10 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
         units = -(-tall // rows) * G
         tiles = units * (held // keys + m)
         sms = gemm_fast._sms(q.device)
-        ctas = max(1, min(sms * 2, tiles) if wide else min(sms, max(units * m, (tiles + 1) // 2)))
+        if wide:
+            ctas = min(sms * (4 if tiles >= 16 * sms else 2), units * m if tiles <= 2 * units * m else tiles)
+        else:
+            ctas = min(sms, max(units * m, (tiles + 1) // 2))
         cap = min(rows, tall)
         part = torch.empty(2 * ctas * cap * (hd + 2), dtype=torch.float32, device=q.device)
         at = part.data_ptr()
