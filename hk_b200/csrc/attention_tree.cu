@@ -526,12 +526,20 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 // Waits for the phase of this parity, a bounded time; false (and the flag set) if it did not come or another gave up.  (Without sleeps
-// between the tries: the tensor core's answers come in less than one.)
+// between the tries: the tensor core's answers come in less than one.)  Behind the flag lies the pulse of the warps that take lost rows
+// again, which takes as long as it takes: while it beats, time does not run.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
-  const long long start = clock64();
-  while (!*abort_flag && clock64() - start < WAIT_CLOCKS)
+  long long start = clock64();
+  int beat = abort_flag[1];
+  while (!*abort_flag && clock64() - start < WAIT_CLOCKS) {
     if (mbar_try_wait(bar, parity)) return true;
+    const int now = abort_flag[1];
+    if (now != beat) {
+      beat = now;
+      start = clock64();
+    }
+  }
   *abort_flag = 1;
   return false;
 }
@@ -658,7 +666,7 @@ struct TcSmem {
   Segment segment[3];         // the softmax warps' segments: the last one (until its results are out), the one in hand, the next one
   int any[3];
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, pulse;      // (side by side: mbar_wait)
 };
 
 // One row once more, by one warp in 32 bits over the keys of a segment that it sees.  For a row whose sums came out NaN or Inf: the
@@ -668,12 +676,14 @@ struct RowKeys {
   const bf16* q;
   const int* bt;
   TreeRow w;
+  volatile int* pulse;
   float scale_log2;
   int j, end;
 };
-__device__ __forceinline__ RowKeys row_keys(const TreeArgs& a, const Segment& s, int row) {
+__device__ __forceinline__ RowKeys row_keys(const TreeArgs& a, const Segment& s, int row, volatile int* pulse) {
   const int token = token_of(a, s.row0 + row), head = s.g * a.group + s.row0 + row - token * a.group;
   RowKeys k;
+  k.pulse = pulse;
   k.w = tree_row(a, s.q, token, true);
   k.q = reinterpret_cast<const bf16*>(a.q) + ((size_t)(s.q.first + token) * a.H + head) * a.hd;
   k.bt = a.block_table + (size_t)s.q.slot * a.table_stride;
@@ -687,33 +697,42 @@ __device__ __forceinline__ long long next_key(const TreeArgs& a, const Segment& 
   const uint32_t see = visible32(k.w, k.j);
   const int j = k.j + (int)(threadIdx.x & 31);
   k.j += 32;
+  if ((threadIdx.x & 31) == 0) *k.pulse = (int)clock64();
   if (!((see >> (threadIdx.x & 31)) & 1u)) return -1;
   const int page = k.bt[j / a.page_tokens];
   if (page < 0 || page >= a.num_pages) return -1;
   const long long at = (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * a.hd;
-  const bf16* key = reinterpret_cast<const bf16*>(a.k) + at;
+  const uint4 *key = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.k) + at), *query = reinterpret_cast<const uint4*>(k.q);
   float x = 0.f;
-  for (int d = 0; d < a.hd; ++d) x = fmaf(__bfloat162float(k.q[d]), __bfloat162float(key[d]), x);
+  for (int d = 0; d < a.hd / 8; ++d) {
+    const uint4 u = query[d], v = key[d];
+    const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x = fmaf(__uint_as_float(us[e] << 16), __uint_as_float(vs[e] << 16), x);
+      x = fmaf(__uint_as_float(us[e] & 0xffff0000u), __uint_as_float(vs[e] & 0xffff0000u), x);
+    }
+  }
   score = log2_score(x, k.scale_log2, cap_log2, cap_in2);
   return at;
 }
 // The row's largest score m and the sum l of exp2(score - m).
-__device__ __noinline__ void tree_row_top(const TreeArgs& a, const Segment& s, int row, float cap_log2, float cap_in2, float& m, float& l) {
+__device__ __noinline__ void tree_row_top(const TreeArgs& a, const Segment& s, int row, float cap_log2, float cap_in2, float& m, float& l, volatile int* pulse) {
   float score, top = -CUDART_INF_F, sum = 0.f;
-  for (RowKeys k = row_keys(a, s, row); k.j < k.end;)
+  for (RowKeys k = row_keys(a, s, row, pulse); k.j < k.end;)
     if (next_key(a, s, k, cap_log2, cap_in2, score) >= 0) top = fmaxf(top, score);
   top = warp_max(top);
   const float safe = top == -CUDART_INF_F ? 0.f : top;
-  for (RowKeys k = row_keys(a, s, row); k.j < k.end;)
+  for (RowKeys k = row_keys(a, s, row, pulse); k.j < k.end;)
     if (next_key(a, s, k, cap_log2, cap_in2, score) >= 0) sum += exp2f(score - safe);
   m = top;
   l = warp_sum(sum);
 }
 // A dim a lane of the row's sums against the reference m.
-__device__ __noinline__ float tree_row_again(const TreeArgs& a, const Segment& s, int row, int dim, float m, float cap_log2, float cap_in2) {
+__device__ __noinline__ float tree_row_again(const TreeArgs& a, const Segment& s, int row, int dim, float m, float cap_log2, float cap_in2, volatile int* pulse) {
   const float safe = m == -CUDART_INF_F ? 0.f : m;
   float acc = 0.f, score = 0.f;
-  for (RowKeys k = row_keys(a, s, row); k.j < k.end;) {
+  for (RowKeys k = row_keys(a, s, row, pulse); k.j < k.end;) {
     const long long at = next_key(a, s, k, cap_log2, cap_in2, score);
     const float p = exp2f(score - safe);
     for (uint32_t left = __ballot_sync(0xffffffffu, at >= 0); left; left &= left - 1) {
@@ -759,7 +778,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       mbar_init(&sm.turn[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&sm.pair[i][j], 2);
     }
-    sm.abort_flag = 0;
+    sm.abort_flag = sm.pulse = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -1137,13 +1156,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           bf16* op_row = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)op, from));
           const int head_row = __shfl_sync(0xffffffffu, head, from);
           if (!(l_row <= CUDART_MAX_NORMAL_F)) {        // the reference and the sum as well
-            tree_row_top(a, unit, odd_row, cap_log2, cap_in2, m_row, l_row);
+            tree_row_top(a, unit, odd_row, cap_log2, cap_in2, m_row, l_row, &sm.pulse);
             if (s.whole) inv_row = finish(m_row, l_row, head_row);
             else if (lane == 0 && half == 0 && (two || x == 0)) *(reinterpret_cast<float2*>(a.part_ml) + slot * a.rows_cap + odd_row) = make_float2(m_row, l_row);
           }
           for (int c0 = c_from; c0 < c_to; c0 += 32) {
             const int dim = c0 + lane;
-            const float y = tree_row_again(a, unit, odd_row, min(dim, HD - 1), m_row, cap_log2, cap_in2);
+            const float y = tree_row_again(a, unit, odd_row, min(dim, HD - 1), m_row, cap_log2, cap_in2, &sm.pulse);
             if (dim < c_to) {
               if (s.whole) op_row[dim] = __float2bfloat16_rn(y * inv_row);
               else part_place(a, slot, odd_row, dim, HD)[dim & 3] = y;

@@ -239,3 +239,53 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             call(**change)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lost", ["scores", "values"])
+def test_all_rows_taken_again_behind_long_contexts(lost):
+    """Every row of every request is lost to the tensor core: its scores jump by 2^100 in a late tile, or a value of NaN lies in a drafted
+    row that none sees.  Taking them again lasts far longer than a wait may, and nothing gives up (the fixture looks)."""
+    from hk_b200.csrc import ops
+    m, count, context, G, hd, page = 20, 100, 4000, 8, 128, 16
+    H, g = 2 * G, torch.Generator(device="cuda").manual_seed(3)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda") * 0.3
+    pages = (context + count + page - 1) // page
+    q, k, v = normal(m * count, H * hd), normal(m * pages, G, page, hd), normal(m * pages, G, page, hd)
+    if lost == "scores":
+        q.view(-1, H, hd)[:, :, 0] = 10.0
+        k[:, :, :, 0] = 0.0
+        k.view(m, pages, G, page, hd)[:, 150, :, :, 0] = 80.0
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    plain_v = v.clone()
+    at = context + count - 1                                                     # the last drafted token, which no row sees, nor its own
+    v.view(m, pages, G, page, hd)[:, at // page, :, at % page] = float("nan")
+    if lost == "scores":
+        v.copy_(plain_v)
+    table = torch.arange(m * pages, dtype=torch.int32, device="cuda").view(m, pages)
+    requests = torch.tensor([[i, i * count, count, context] for i in range(m)], dtype=torch.int32, device="cuda")
+    bits = np.zeros((m * count, -(-count // 32)), dtype=np.uint32)
+    for i in range(count - 1):
+        bits[i::count, i // 32] = 1 << (i % 32)
+    ancestors = torch.from_numpy(bits.view(np.int32)).cuda()
+    positions = torch.arange(context, context + count, dtype=torch.int32, device="cuda").repeat(m)
+    out = torch.empty_like(q)
+    ops.tree_attention(q, k, v, table, requests, ancestors, positions, out, H, G, hd, page, 0, hd ** -0.5, count, context + count)
+    torch.cuda.synchronize()
+    for i in (0, 7, m - 1):
+        rows = slice(i * count, (i + 1) * count)
+        x = q[rows].double().view(count, G, 2, hd)
+        kk, vv = (t.view(m, pages, G, page, hd)[i].transpose(0, 1).reshape(G, pages * page, hd)[:, :context + count].double() for t in (k, plain_v))
+        scores = torch.einsum("tghd,gjd->tghj", x, kk) * hd ** -0.5
+        see = torch.zeros(count, context + count, dtype=torch.bool, device="cuda")
+        see[:, :context] = True
+        own = torch.arange(count - 1, device="cuda")
+        see[own, context + own] = True
+        p = torch.softmax(scores.masked_fill(~see[:, None, None], float("-inf")), dim=-1)
+        want = torch.einsum("tghj,gjd->tghd", p, vv).reshape(count, H * hd)
+        weight = torch.einsum("tghj,gjd->tghd", p, vv.abs()).reshape(count, H * hd)
+        # one rounding of the result (2^-8 of it); probabilities rounded where the tensor core did a part of the keys (2^-8 of each); scores
+        # of up to 800 before the scale, summed 128 times in 32 bits (128 * 800 * 2^-24 / sqrt(128) = 5.4e-4, above and below: 2^-9)
+        error = (out[rows].double() - want).abs()
+        assert (error <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -9) * weight).all()
