@@ -7,6 +7,9 @@
 
 #include "common.cuh"
 
+// Every kernel here lets the next one start only behind its own wait: so no more than two calls' kernels are under way at once, and none
+// runs beside one that is to be through before the kernel before it.
+
 namespace {
 
 // ---- blocks of a cache --------------------------------------------------------------------------------------------------
@@ -44,8 +47,8 @@ __device__ __forceinline__ void copy_part(uint8_t* to, const uint8_t* from, long
 // thread on their way: 14.0 and 166; 2 states 22.9, 24.9 and 23.3.
 __global__ void __launch_bounds__(COPY_THREADS, 8)
 copy_blocks_kernel(const BlockArray* __restrict__ table, const int* __restrict__ moves) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const BlockArray a = table[blockIdx.z];
   const int from = moves[3 * blockIdx.y], to = moves[3 * blockIdx.y + 1], rows = moves[3 * blockIdx.y + 2];
   if (from < 0 || to < 0 || from >= a.blocks || to >= a.blocks || from == to || rows <= 0) return;
@@ -95,8 +98,8 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
                     int table_stride, int page_tokens, long long num_pages) {
   __shared__ int2 from[KEEP_PATH], to[KEEP_PATH];
   __shared__ int count;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int* path = paths + (size_t)blockIdx.x * (width + 2);
   const int slot = path[0], first = path[1], a0 = blockIdx.y * per_block, a1 = min(arrays, a0 + per_block);
   if (slot < 0 || slot >= table_rows || first < 0) return;
@@ -180,6 +183,12 @@ struct RowPart {
   double sum;                         // of exp(x - top)
   float top, pad;                     // (top: the part's reference, -inf if it holds nothing finite)
 };
+
+// A part that the kernel before has left: past L1, which may hold what an earlier call left there.
+__device__ __forceinline__ RowPart part_of(const RowPart* at) {
+  const float4 x = __ldcg(reinterpret_cast<const float4*>(at));
+  return {__hiloint2double(__float_as_int(x.y), __float_as_int(x.x)), x.z, x.w};
+}
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
@@ -332,8 +341,8 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   __shared__ int s_i[BC], s_n, s_found[BAR_STEPS + 1];
   __shared__ uint16_t s_pair[BC];
   __shared__ double s_sum[BT / 32];
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x, row = blockIdx.x / parts, p = blockIdx.x % parts;
   const size_t at = (size_t)row * parts + p;
   if (!finite(scores[row])) {
@@ -502,13 +511,13 @@ constexpr int CT = 512, CDEEP = 8, CHOICE_STEPS = 24;    // threads of the choic
 
 __global__ void __launch_bounds__(CT)
 beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, int groups, int parts, int ranks, uint32_t ranks_inverse,
-                   uint32_t beam_inverse, const RowPart* __restrict__ part,
-                   const float* __restrict__ part_x, const int* __restrict__ part_i, float* __restrict__ out_scores,
+                   uint32_t beam_inverse, const RowPart* part,
+                   const float* part_x, const int* part_i, float* __restrict__ out_scores,
                    int* __restrict__ out_beams, int* __restrict__ out_tokens) {
   __shared__ double s_group[CT], s_x[BC], s_lift[BEAM_MOST];      // s_lift: a beam's score less the logarithm of its sum
   __shared__ int s_i[BC], s_n, s_taken[BEAM_MOST], s_found[CHOICE_STEPS + 1];
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row0 = (size_t)b * K;
   // candidate c: the token of rank c % choices of part c / choices of the prompt's rows (-inf where a part has fewer); its flat index
@@ -523,21 +532,21 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
 #pragma unroll
   for (int j = 0; j < CDEEP; ++j) {
     const int m = threadIdx.x + j * CT, p = ranks == 1 ? m : (int)__umulhi((uint32_t)m, ranks_inverse), c = p * choices + m - p * ranks;
-    keep_x[j] = m < held ? xs[c] : -CUDART_INF_F;
-    keep_i[j] = m < held ? is[c] : 0;
+    keep_x[j] = m < held ? __ldcg(xs + c) : -CUDART_INF_F;
+    keep_i[j] = m < held ? __ldcg(is + c) : 0;
   }
   for (int k = warp; k < K; k += CT / 32) {
     const RowPart* of = part + (row0 + k) * parts;
     RowPart first = {0.0, -CUDART_INF_F, 0.f};
-    if (lane < parts) first = of[lane];
+    if (lane < parts) first = part_of(of + lane);
     float top = first.top;
 #pragma unroll 4
-    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, of[p].top);
+    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, part_of(of + p).top);
     top = warp_max(top);
     double sum = first.sum > 0.0 ? first.sum * exp((double)first.top - (double)top) : 0.0;
 #pragma unroll 4
     for (int p = lane + 32; p < parts; p += 32) {
-      const RowPart r = of[p];
+      const RowPart r = part_of(of + p);
       if (r.sum > 0.0) sum += r.sum * exp((double)r.top - (double)top);
     }
 #pragma unroll
@@ -566,12 +575,12 @@ beam_choice_kernel(const float* __restrict__ scores, int K, int V, int choices, 
     for (int c0 = threadIdx.x; c0 < all; c0 += CT * CDEEP) {
       float x[CDEEP];
 #pragma unroll
-      for (int j = 0; j < CDEEP; ++j) x[j] = c0 + j * CT < all ? xs[c0 + j * CT] : -CUDART_INF_F;
+      for (int j = 0; j < CDEEP; ++j) x[j] = c0 + j * CT < all ? __ldcg(xs + c0 + j * CT) : -CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < CDEEP; ++j)
         if (x[j] > -CUDART_INF_F) {
           const int c = c0 + j * CT, k = c / of_beam;
-          take((double)x[j] + s_lift[k], k * V + is[c]);
+          take((double)x[j] + s_lift[k], k * V + __ldcg(is + c));
         }
     }
   };

@@ -234,6 +234,29 @@ def test_beams_replayed_and_on_two_streams():
         assert np.array_equal(out[1].cpu().numpy(), want[1]) and np.array_equal(out[2].cpu().numpy(), want[2])
 
 
+def test_beams_of_many_calls_in_flight():
+    """Calls that wait one behind the other for the GPU, on other inputs by turns: each starts beside the one before, on the same scratch."""
+    from hk_b200.csrc import ops
+    rng = np.random.default_rng(9)
+    work = torch.randn(4096, 4096, device="cuda", dtype=torch.bfloat16)
+    for beams, choices, V, rows in ((3, 6, 5936, 51), (8, 16, 30001, 64)):
+        inputs = [((rng.standard_normal((rows, V)) * 3).astype(np.float32), -(rng.random(rows) * 3).astype(np.float32)) for _ in range(3)]
+        wants = [beam_reference(x, s, beams, choices) for x, s in inputs]
+        inputs = [(torch.from_numpy(x).cuda(), torch.from_numpy(s).cuda()) for x, s in inputs]
+        outs = [(torch.empty((rows // beams, choices), device="cuda"), *(torch.empty((rows // beams, choices), dtype=torch.int32, device="cuda") for _ in range(2)))
+                for _ in range(60)]
+        for _ in range(20):
+            work @ work
+        for i, out in enumerate(outs):
+            ops.beam_select(*inputs[i % 3], beams, *out)
+        torch.cuda.synchronize()
+        for i, (score, beam, token) in enumerate(outs):
+            want = wants[i % 3]
+            assert np.array_equal(beam.cpu().numpy(), want[1]) and np.array_equal(token.cpu().numpy(), want[2])
+            # (as in check_beams)
+            assert (np.abs(score.cpu().numpy() - want[0]) <= 2.0 ** -24 * np.abs(want[0]) + 2.0 ** -22).all()
+
+
 def test_beam_refusals():
     from hk_b200.csrc import ops
     logits, scores = torch.randn(6, 50, device="cuda"), torch.zeros(6, device="cuda")
