@@ -184,7 +184,8 @@ struct RowPart {
   float top, pad;                     // (top: the part's reference, -inf if it holds nothing finite)
 };
 
-// A part that the kernel before has left: past L1, which may hold what an earlier call left there.
+// A part that the kernel before has left.  Past L1: this kernel starts beside that one, on SMs whose L1 may hold a sector as it was before
+// a neighbouring part's CTA wrote its half.
 __device__ __forceinline__ RowPart part_of(const RowPart* at) {
   const float4 x = __ldcg(reinterpret_cast<const float4*>(at));
   return {__hiloint2double(__float_as_int(x.y), __float_as_int(x.x)), x.z, x.w};
