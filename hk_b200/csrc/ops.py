@@ -1696,6 +1696,7 @@ def copy_blocks(table: torch.Tensor, moves: torch.Tensor, most_bytes: int) -> No
                                                 torch._C._cuda_getCurrentRawStream(dev)), "copy_blocks")
 
 
+BEAM_CHOICES = 256      # choices of a prompt
 _BEAM_PARTS = 592      # CTAs of a wave, among which rows are cut (`hk_beam_select` in csrc/branches.cu refuses less scratch than it uses)
 
 

@@ -1,8 +1,9 @@
 """Beam search above the step function: the most probable continuations of a prompt, several at a time.
 
 The beams of a prompt are requests of the engine.  A step runs all beams of all prompts as one decode batch, `ops.beam_select` chooses
-the best continuations over beams and vocabulary on the device (two per beam, so that enough are left when some of them end), and
-`Engine.reorder` makes the requests go on with the beams chosen: pages are shared until a beam writes them, states are copied.
+the best continuations over beams and vocabulary on the device (one more per beam and end token than there are beams, so that enough are
+left when some of them end), and `Engine.reorder` makes the requests go on with the beams chosen: pages are shared until a beam writes
+them, states are copied.
 
 A continuation that ends (an end token among the first `beams` choices of its step, or the most tokens) is a finished one; finished
 ones are ordered by the sum of their tokens' log probabilities over length^length_penalty, the end token's probability included.  A
@@ -17,6 +18,7 @@ import numpy as np
 import torch
 
 from ..csrc import ops
+from ..csrc.ops import BEAM_CHOICES
 from .engine import Engine, EngineError, StepEntry
 
 
@@ -48,7 +50,7 @@ class BeamSearch:
         if beams > engine.cache.books.max_requests:
             raise ValueError(f"{beams} beams need as many request slots; the engine has {engine.cache.books.max_requests}")
         self.engine, self.beams, self.most, self.penalty = engine, int(beams), int(max_new_tokens), float(length_penalty)
-        self.eos = set(int(t) for t in eos_token_ids)
+        self.eos = set(int(t) for t in eos_token_ids if 0 <= int(t) < engine.vocab)
         self.chunk = max(1, min(int(prefill_chunk), engine.max_batch_tokens))
 
     def run(self, prompts: Sequence[Sequence[int]]) -> List[List[Continuation]]:
@@ -114,7 +116,6 @@ class BeamSearch:
     def _choose(self, prompts: List[_Prompt], logits: torch.Tensor, opened: List[tuple]) -> None:
         """The next beams of prompts with equally many running beams each (a prompt with fewer has places that are not there)."""
         width = max(len(g.names) for g in prompts)
-        choices = min(2 * self.beams, width * self.engine.vocab)
         scores = np.full((len(prompts), width), -np.inf, dtype=np.float32)
         for i, g in enumerate(prompts):
             scores[i, :len(g.scores)] = g.scores
@@ -124,25 +125,47 @@ class BeamSearch:
                 rows += [at + min(k, len(g.names) - 1) for k in range(width)]
                 at += len(g.names)
             logits = logits[torch.tensor(rows, device=logits.device)]
-        dev = logits.device
-        best = torch.empty((len(prompts), choices), dtype=torch.float32, device=dev)
-        beam, token = (torch.empty((len(prompts), choices), dtype=torch.int32, device=dev) for _ in range(2))
-        ops.beam_select(logits, torch.from_numpy(scores.reshape(-1)).to(dev), width, best, beam, token)
-        best, beam, token = best.tolist(), beam.tolist(), token.tolist()
+        scores = torch.from_numpy(scores.reshape(-1)).to(logits.device)
+        # `beams` choices that go on are among the best beams + (end tokens) * width
+        most = self.beams + len(self.eos) * width
+        ahead = chosen = self._best(logits, scores, width, min(most, width * self.engine.vocab)) if most <= BEAM_CHOICES else None
+        if chosen is None:                                     # all end tokens as one, with their probabilities together
+            ahead = self._best(logits, scores, width, min(self.beams, width * self.engine.vocab))
+            chosen = self._best(self._ends_as_one(logits), scores, width, min(self.beams + width, width * (self.engine.vocab + 1)))
         for i, g in enumerate(prompts):
             parents, outputs, totals = [], [], []
-            for rank, (s, k, t) in enumerate(zip(best[i], beam[i], token[i])):
+            for s, k, t in ahead[i][:self.beams]:
+                if s != -np.inf and t in self.eos:
+                    g.finished.append(Continuation(list(g.outputs[k]), self._final(s, len(g.outputs[k]) + 1), True))
+            for s, k, t in chosen[i]:
                 if s == -np.inf or len(parents) == self.beams:
                     break
-                if t in self.eos:
-                    if rank < self.beams:
-                        g.finished.append(Continuation(list(g.outputs[k]), self._final(s, len(g.outputs[k]) + 1), True))
+                if t in self.eos or t == self.engine.vocab:
                     continue
                 parents.append(k)
                 outputs.append(g.outputs[k] + [t])
                 totals.append(s)
             self._follow(g, parents, opened)
             g.outputs, g.scores = outputs, totals
+
+    @staticmethod
+    def _best(logits: torch.Tensor, scores: torch.Tensor, width: int, choices: int) -> List[List[tuple]]:
+        """For each prompt (score, beam, token) of its best choices, best first."""
+        prompts, dev = logits.shape[0] // width, logits.device
+        best = torch.empty((prompts, choices), dtype=torch.float32, device=dev)
+        beam, token = (torch.empty((prompts, choices), dtype=torch.int32, device=dev) for _ in range(2))
+        ops.beam_select(logits, scores, width, best, beam, token)
+        return [list(zip(*lists)) for lists in zip(best.tolist(), beam.tolist(), token.tolist())]
+
+    def _ends_as_one(self, logits: torch.Tensor) -> torch.Tensor:
+        """The logits with the end tokens masked and a token more, as probable as all of them together (its logit is rounded to float32,
+        2^-24 of it: what the sum of a row's exponentials can be off by)."""
+        ends = torch.tensor(sorted(self.eos), device=logits.device)
+        x = logits[:, ends].double()
+        x = torch.where(torch.isfinite(x), x, -torch.inf)
+        out = torch.cat([logits, torch.logsumexp(x, dim=1, keepdim=True).float()], dim=1)
+        out[:, ends] = -torch.inf
+        return out
 
     def _follow(self, g: _Prompt, parents: List[int], opened: List[tuple]) -> None:
         """Makes the prompt's requests the chosen beams, as many as there are parents."""
