@@ -169,11 +169,13 @@ compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_bloc
 // sixteens that reach it are read again for the tokens that can be among the part's best.  (Looking for them on the way took a barrier
 // a tile and, with some lane over the bar in most tiles, one and a half times the instructions: 42 us for 28.)  A CTA a prompt then joins
 // the parts' sums, scores the parts' tokens in 64 bits and ranks them: rounded to float32, scores of some -10 lie 1e-6 apart, and
-// neighbours among a million would be equal often enough.  What is left is the error of the exponentials, some 1e-8 of a sum.
+// neighbours among a million would be equal often enough.  What is left is the error of the exponentials and of their sums by sixteens:
+// at most 2^-21 + 2^-24 of a row's sum (5e-7), mostly some 1e-8.
 //
-// Time: some 15 us of dependent steps (start, bar, read again, sums, rank) and the stream at DRAM's rate: 4, 8 and 16 prompts of 8 beams
-// over 151,936 tokens take 18.5, 21.9 and 28.2 us (39 MB more: 6.3 us, 6.2 TB/s), a prompt of 4 beams 12.3, of 128 with 256 choices 132.
-// (Blocks of 128 threads, eight a SM: 37.9; tiles asked into L2 ahead: 28.5 to 30.8.)
+// Time: some 15 us of dependent steps (start, bar, read again, sums, rank) and the stream: 4, 8 and 16 prompts of 8 beams over 151,936
+// tokens take 20.5, 23.4 and 30.9 us (39 MB more: 7.5 us, 5.2 TB/s), a prompt of 4 beams 12.4, of 128 with 256 choices 159.  (Exponentials
+// of differences taken in 32 bits, up to 1.8e-6 off: 28.3 for 16 prompts.  Blocks of 128 threads, eight a SM, or tiles asked into L2 ahead
+// were slower.)
 constexpr int BT = 256;               // threads
 constexpr int BEAM_MOST = 256;        // choices
 constexpr int BC = 2048;              // candidates that are ranked side by side; more than that only among equal logits
@@ -302,32 +304,51 @@ __device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 
-// The sum of e^(v - safe), differences up to 20 and so: 2^(x log2 e) with the product in two parts, so that the constant's rounding adds
-// no error that all terms share; the product's own rounding is 2^-24 of it, the power's 2 units in the last place.
-__device__ __forceinline__ float tile_sum(const float* v, float safe) {
-  const uint64_t less = two(-safe, -safe), high = two(1.4426950216293335f, 1.4426950216293335f), low = two(1.9259629e-8f, 1.9259629e-8f);
-  uint64_t sum = two(0.f, 0.f);
+// A thread's reference: what the exponentials of its sum are held against.  The difference of a logit and the reference is not taken in 32
+// bits, since a difference of d is off by up to d 2^-25, which all terms of a sum may share.  Both are split into a whole number and at
+// most a half, x log2(e) = n + f, by a product that is not rounded before n comes off; the exponential is 2^(f - the reference's f) with
+// the whole numbers' difference added to the bits of its exponent.  So a term is off by the approximation (2 units in the last place) and
+// 2^-23, whatever x is, and the reference's own term is 1.  `base` is 0 but for logits of 2^20 and more, which lie so far apart that their
+// differences up to 107 are exact.
+struct Reference {
+  float base, magic, rest, low;         // magic: 1.5 2^23 - n; rest: f; low: what smaller logits (and NaN) count as, e^-80 of the reference
+};
+constexpr float LOG2E_HIGH = 1.4426950216293335f, LOG2E_LOW = 1.9259629e-8f, WHOLE = 12582912.0f;      // WHOLE: 1.5 2^23
+__device__ __forceinline__ Reference reference_of(float ref) {
+  const float base = fabsf(ref) < 1048576.0f ? 0.f : ref, x = ref - base, n = fmaf(x, LOG2E_HIGH, WHOLE) - WHOLE;
+  return {base, WHOLE - n, fmaf(x, LOG2E_LOW, fmaf(x, LOG2E_HIGH, -n)), x - 80.0f};
+}
+
+// The sum of e^(v - reference) over sixteen logits up to 20 above it, added in four steps.  (In two chains of eight, equal terms share the
+// chains' roundings.)
+__device__ __forceinline__ float tile_sum(float* v, const Reference& of) {
+  if (of.base != 0.f)
+#pragma unroll
+    for (int e = 0; e < BE; ++e) v[e] -= of.base;
+  const uint64_t high = two(LOG2E_HIGH, LOG2E_HIGH), less_high = two(-LOG2E_HIGH, -LOG2E_HIGH), less_low = two(-LOG2E_LOW, -LOG2E_LOW),
+                 magic = two(of.magic, of.magic), back = two(-of.magic, -of.magic), rest = two(of.rest, of.rest);
+  uint64_t sum[BE / 2];
 #pragma unroll
   for (int e = 0; e < BE; e += 2) {
-    const uint64_t x = add_two(two(v[e], v[e + 1]), less), z = fma_two(x, low, mul_two(x, high));
+    const uint64_t x = two(fmaxf(v[e], of.low), fmaxf(v[e + 1], of.low)), n = fma_two(x, high, magic);      // n: 1.5 2^23 + x's - the reference's
+    const uint64_t less_f = add_two(fma_two(x, less_low, fma_two(x, less_high, add_two(n, back))), rest);
     float y0, y1;
-    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %2;\n\tex2.approx.ftz.f32 %0, a;\n\tex2.approx.ftz.f32 %1, b;\n\t}"
-        : "=f"(y0), "=f"(y1) : "l"(z));
-    sum = add_two(sum, two(y0, y1));
+    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %2;\n\tneg.f32 a, a;\n\tneg.f32 b, b;\n\tex2.approx.ftz.f32 %0, a;\n\tex2.approx.ftz.f32 %1, b;\n\t}"
+        : "=f"(y0), "=f"(y1) : "l"(less_f));
+    sum[e / 2] = two(__uint_as_float(__float_as_uint(y0) + ((uint32_t)n << 23)), __uint_as_float(__float_as_uint(y1) + ((uint32_t)(n >> 32) << 23)));
   }
+#pragma unroll
+  for (int step = 1; step < BE / 2; step *= 2)
+#pragma unroll
+    for (int e = 0; e < BE / 2; e += 2 * step) sum[e] = add_two(sum[e], sum[e + step]);
   float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum[0]));
   return a + b;
 }
 
@@ -372,6 +393,7 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
   };
   const int tiles = (end - begin + BT * BE - 1) / (BT * BE), per = (tiles + SLOTS - 1) / SLOTS;
   float slot_high = -CUDART_INF_F, mine = -CUDART_INF_F, ref = -CUDART_INF_F;
+  Reference reference = {0.f, 0.f, 0.f, 0.f};
   double sum = 0.0;
   int slot = 0, in_slot = 0;
   auto tile = [&](int t, float* v, float* next) {
@@ -397,15 +419,9 @@ beam_rows_kernel(const float* __restrict__ logits, const float* __restrict__ sco
     if (high > ref + 20.0f) {          // also true for the first finite value
       sum *= ref == -CUDART_INF_F ? 0.0 : exp((double)ref - (double)high);
       ref = high;
+      reference = reference_of(ref);
     }
-    const float safe = ref == -CUDART_INF_F ? 0.f : ref;
-    float s = tile_sum(v, safe);
-    if (s != s) {                      // NaN where a value is
-#pragma unroll
-      for (int e = 0; e < BE; ++e) v[e] = finite(v[e]) ? v[e] : -CUDART_INF_F;
-      s = tile_sum(v, safe);
-    }
-    sum += (double)s;
+    if (ref > -CUDART_INF_F) sum += (double)tile_sum(v, reference);
   };
   float one[BE], other[BE];
   load(0, one);

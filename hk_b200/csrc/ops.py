@@ -1706,8 +1706,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, out_sc
     log softmax(logits[b, k])[v], best first, of equal ones the lowest k * vocab + v first.  logits float32 [prompts * n_beams,
     vocab], scores float32 [prompts * n_beams]; out_scores float32, out_beams (k) and out_tokens (v) int32 [prompts, choices].  A logit
     that is not finite counts as -inf, and so do all continuations of a beam whose score is not finite (one that is not there yet, or no
-    longer).  Scores are compared in 64 bits; the exponentials in a beam's sum have 32, so continuations of two beams that lie within some
-    1e-7 of each other may come in either order (always the same one).  Up to 256 beams and 256 choices."""
+    longer).  Scores are compared in 64 bits; the exponentials in a beam's sum have 32 and put all its scores off by up to 5e-7 (mostly some
+    1e-8), so continuations of two beams that lie no further apart may come in either order (always the same one).  Up to 256 beams and 256 choices."""
     # (the usual call in one condition, as in `tree_attention`)
     f32, i32, dev = torch.float32, torch.int32, logits.get_device()
     shape, size, row = out_scores.shape, logits.shape, scores.shape
