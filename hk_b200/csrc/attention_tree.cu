@@ -20,7 +20,7 @@
 // called again and again for a second, 210 and 165.  The generic kernel took 391, 4,463, 47,593 and 76,055.
 //
 // What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays or the bounds is
-// skipped, and a page outside the pool is not read.
+// skipped, and the keys of a page that is not in the pool are not seen.
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -667,11 +667,12 @@ struct TcSmem {
   int any[3];
   uint32_t tmem_base;
   int abort_flag, pulse;      // (side by side: mbar_wait)
+  int gone;                   // a page of the share is not in the pool
 };
 
 // One row once more, by one warp in 32 bits over the keys of a segment that it sees.  For a row whose sums came out NaN or Inf: the
 // tensor core's product takes whole tiles of values, and a probability of zero does not keep out a NaN or Inf among those that the row
-// does not see; or one tile's scores ran too far ahead of the reference.
+// does not see; or one tile's scores ran too far ahead of the reference; or a page of the share is not in the pool.
 struct RowKeys {
   const bf16* q;
   const int* bt;
@@ -778,7 +779,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       mbar_init(&sm.turn[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&sm.pair[i][j], 2);
     }
-    sm.abort_flag = sm.pulse = 0;
+    sm.abort_flag = sm.pulse = sm.gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -829,13 +830,22 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       };
       // 32 boxes at a time, a lane each; the next 32 are on their way meanwhile
       int at = s.t0 * boxes + lane;
-      int row = row_of(at, page_of(at));
-      int page = page_of(at + 32);
+      // Keys of a page that is not there are found too late for the scores' masks: rows of the pool lie in their place, and the softmax
+      // threads take every row once more without them, from here on for all of the share (this is no usual call).  The arrival for the
+      // tile's keys publishes the flag.
+      auto tell = [&](int page) {
+        if (__any_sync(0xffffffffu, page < 0 || page >= a.num_pages) && lane == 0) *static_cast<volatile int*>(&sm.gone) = 1;
+      };
+      int page = page_of(at);
+      int row = row_of(at, page);
+      tell(page);
+      page = page_of(at + 32);
       int sent = 0;
       for (int i = 0; i < s.n && alive; ++i, ++n) {
         if (sent == 32) {
           at += 32;
           row = row_of(at, page);
+          tell(page);
           page = page_of(at + 32);
           sent = 0;
         }
@@ -1081,7 +1091,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_done[y], o_done[y] & 1u, abort_flag))) ok = false;
         else ++o_done[y];
       }
-      sm.ml[x][half][r] = make_float2(m, l0 + l1);
+      // (a thread has seen what was told before its own tiles came; a row's sums meet, and one that is lost makes all of them)
+      sm.ml[x][half][r] = make_float2(m, *static_cast<volatile int*>(&sm.gone) ? CUDART_NAN_F : l0 + l1);
       tc_fence_before();
       ok = !softmax_any(!ok);
       if (!ok) break;
@@ -1253,6 +1264,7 @@ struct F32Smem {
   float2 ml[F32_ROWS];
   uint32_t see[F32_ROWS][F32_KEYS / 32];
   long long at[2][F32_KEYS];      // [parity of the tile]: where a key's row lies in the pages, -1 where there is none
+  uint32_t there[2];              // and the keys that have one
   Walk start;
 };
 
@@ -1275,10 +1287,13 @@ __global__ void __launch_bounds__(F32_THREADS, 4) tree_f32_kernel(const TreeArgs
   while (next_segment<F32Cut>(a, w, s)) {
     const int* bt = a.block_table + (size_t)s.q.slot * a.table_stride;
     const int end = s.q.context + s.q.count;
-    // where the keys of a tile lie: found once for keys and values, by threads that nothing else waits for
+    // where the keys of a tile lie: found once for keys and values, by a warp that nothing else waits for
+    static_assert(F32_KEYS == 32 && WORDS * F32_ROWS == 32, "a lane a key; the rows' masks by the first warp");
     auto find = [&](int tile, int r) {
       const int j = (s.t0 + tile) * F32_KEYS + r, page = j < end ? bt[j / a.page_tokens] : -1;
       sm.at[tile & 1][r] = page >= 0 && page < a.num_pages ? (((long long)page * a.G + s.g) * a.page_tokens + j % a.page_tokens) * HD : -1;
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);
+      if (r == 0) sm.there[tile & 1] = there;
     };
     // a tile's keys or values, what does not exist as zeros
     auto fetch = [&](const void* pages, float* dst, int tile) {
@@ -1315,7 +1330,7 @@ __global__ void __launch_bounds__(F32_THREADS, 4) tree_f32_kernel(const TreeArgs
       const int j0 = (s.t0 + t) * F32_KEYS;
       bool part = false;
       if (tid < WORDS * F32_ROWS) {
-        const uint32_t see = visible32(tr, j0 + 32 * (tid % WORDS));
+        const uint32_t see = visible32(tr, j0 + 32 * (tid % WORDS)) & sm.there[t & 1];
         sm.see[tid / WORDS][tid % WORDS] = see;
         part = tid / WORDS < s.rows && see != 0xffffffffu;
       } else if (t + 1 < s.n && tid - WORDS * F32_ROWS < F32_KEYS) {

@@ -1532,8 +1532,8 @@ def tree_attention(q, k_pages, v_pages, block_table, requests, ancestors, positi
     order.  A token sees all cached rows and the drafted ones whose bits are set in its row of `ancestors` int32 [n, words] (bit j %
     32 of word j / 32: drafted token j of its request; for a tree its ancestors and itself); with `window` w only those at positions
     above its own less w, where a cached row's position is its place and a drafted token's is in `positions` int32 [n] (not below the
-    request's cached rows).  A token that sees nothing gives zeros; rows of no request keep what they hold.  sink, sinks, softcap
-    as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them: one beyond them is left out;
+    request's cached rows).  A token that sees nothing gives zeros; rows of no request keep what they hold; keys of a page that is
+    not in the pool (-1) are not seen.  sink, sinks, softcap as in `paged_attention`.  most_tokens and most_keys bound a request's drafted tokens (at most 256) and its rows with them: one beyond them is left out;
     all_keys: the rows of all requests together, where the caller knows it (0: as if all had the most)."""
     H, G, hd = n_heads, n_kv_heads, head_dim
     # The usual call in one condition (a call of one user's tree costs the host as much as the GPU); what it does not let through goes
