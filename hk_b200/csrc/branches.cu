@@ -8,7 +8,9 @@
 #include "common.cuh"
 
 // Every kernel here lets the next one start only behind its own wait: so no more than two calls' kernels are under way at once, and none
-// runs beside one that is to be through before the kernel before it.
+// runs beside one that is to be through before the kernel before it.  What a kernel before may have written in part of a 32-byte sector
+// (blocks and rows of odd sizes, parts of a choice) is read past L1: it is read once, so L1 gives nothing, and whatever an SM's L1 took in
+// for that kernel, while this one had started, does not count.
 
 namespace {
 
@@ -33,7 +35,7 @@ __device__ __forceinline__ void copy_part(uint8_t* to, const uint8_t* from, long
       if (i < all) {
         const long long p = pieces == 1 ? 0 : (long long)((unsigned long long)i / (unsigned long long)per);
         at[k] = p * piece + (i - p * per) * (long long)sizeof(V);
-        v[k] = *reinterpret_cast<const V*>(from + at[k]);
+        v[k] = __ldcg(reinterpret_cast<const V*>(from + at[k]));
       }
     }
 #pragma unroll
@@ -81,7 +83,7 @@ __device__ __forceinline__ void move_rows(const RowArray& a, const int2* from, c
     V v[KEEP_DEEP];
 #pragma unroll
     for (int k = 0; k < KEEP_DEEP; ++k)
-      if (i0 + k < n) v[k] = *reinterpret_cast<const V*>(base + from[i0 + k].x * page_bytes + from[i0 + k].y * a.row);
+      if (i0 + k < n) v[k] = __ldcg(reinterpret_cast<const V*>(base + from[i0 + k].x * page_bytes + from[i0 + k].y * a.row));
 #pragma unroll
     for (int k = 0; k < KEEP_DEEP; ++k)
       if (i0 + k < n) *reinterpret_cast<V*>(base + to[i0 + k].x * page_bytes + to[i0 + k].y * a.row) = v[k];
@@ -186,8 +188,7 @@ struct RowPart {
   float top, pad;                     // (top: the part's reference, -inf if it holds nothing finite)
 };
 
-// A part that the kernel before has left.  Past L1: this kernel starts beside that one, on SMs whose L1 may hold a sector as it was before
-// a neighbouring part's CTA wrote its half.
+// A part that the kernel before has left (past L1, see above).
 __device__ __forceinline__ RowPart part_of(const RowPart* at) {
   const float4 x = __ldcg(reinterpret_cast<const float4*>(at));
   return {__hiloint2double(__float_as_int(x.y), __float_as_int(x.x)), x.z, x.w};
