@@ -69,6 +69,7 @@ def _runtime() -> ctypes.CDLL:
             ("hk_books_first_page", ctypes.POINTER(ctypes.c_int32), [vp, ci]), ("hk_books_n_pages", ctypes.POINTER(ctypes.c_int32), [vp, ci]),
             ("hk_books_open", ci, [vp]), ("hk_books_close", ci, [vp, ci]), ("hk_books_release_passed", ci, [vp, ci]),
             ("hk_books_pages_to_take", ci, [vp, ci, ci, ctypes.POINTER(ci)]), ("hk_books_pages_passed", ci, [vp, ci, ctypes.POINTER(ci)]), ("hk_books_free_pages", None, [vp, ctypes.POINTER(ci)]),
+            ("hk_books_step_pages", ci, [vp, ctypes.POINTER(ci), ctypes.POINTER(ci), ci, ctypes.POINTER(ci)]),
             ("hk_books_shared_page", ci, [vp, ci, ctypes.POINTER(ci), ctypes.POINTER(ci)]), ("hk_books_fork", ci, [vp, ci]),
             ("hk_books_copies", ci, [vp, ctypes.POINTER(ci), ci]), ("hk_books_extend", ci, [vp, ci, ci]), ("hk_books_truncate", ci, [vp, ci, ci]), ("hk_books_audit", ci, [vp]),
         ]:
@@ -207,6 +208,13 @@ class CacheBooks:
     def pages_to_take(self, slot: int, n_new: int) -> List[int]:
         """For each group: the pages `extend(slot, n_new)` would take from the pool."""
         self._check(self._rt.hk_books_pages_to_take(self._h, int(slot), int(n_new), self._take))
+        return list(self._take[:len(self.groups)])
+
+    def step_pages(self, slots: Sequence[int], n_new: Sequence[int]) -> List[int]:
+        """For each group: the pages that a step takes from the pool, less those that its windows give back, where slots[i] gets
+        n_new[i] tokens: first all of them give back what they have passed (`release_passed`), then each is extended."""
+        m = len(slots)
+        self._check(self._rt.hk_books_step_pages(self._h, (ctypes.c_int * m)(*slots), (ctypes.c_int * m)(*n_new), m, self._take))
         return list(self._take[:len(self.groups)])
 
     def free_pages(self) -> List[int]:

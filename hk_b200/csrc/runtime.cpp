@@ -229,6 +229,34 @@ HK_API int hk_books_pages_to_take(void* h, int slot, int n_new, int* out) {
   return 0;
 }
 
+// For each group: the pages that a step of n_new[i] tokens for each of the slots takes from the pool, less those that its windows give
+// back, in the order of a step: all slots give back what they have passed, then each takes its own.  A shared page comes back with the last
+// of its holders to pass it, and the last one that holds it still writes it where it is.
+HK_API int hk_books_step_pages(void* h, const int* slots, const int* n_new, int m, int* out) {
+  Books& b = *static_cast<Books*>(h);
+  for (int i = 0; i < m; ++i)
+    if (!b.is_live(slots[i])) return b.fail(ERR_CACHE, "slot " + std::to_string(slots[i]) + " is not live");
+  for (size_t gi = 0; gi < b.groups.size(); ++gi) {
+    Group& g = b.groups[gi];
+    std::map<int, int> left;                             // the holders of shared pages that the step has given up in part
+    auto holders = [&](int p) -> int& { return left.emplace(p, g.pool.holders[(size_t)p]).first->second; };
+    out[gi] = 0;
+    for (int i = 0; i < m; ++i)
+      for (int k = g.first_page[(size_t)slots[i]], end = b.passed_end(g, slots[i], b.length[(size_t)slots[i]]); k < end; ++k) {
+        const int p = b.entry(g, slots[i], k);
+        if (g.pool.holders[(size_t)p] == 1 || --holders(p) == 0) --out[gi];
+      }
+    for (int i = 0; i < m; ++i) {
+      out[gi] += std::max(0, b.pages_for(b.length[(size_t)slots[i]] + n_new[i]) - g.n_pages[(size_t)slots[i]]);
+      if (n_new[i] > 0 && b.writes_shared(g, slots[i]) && holders(b.entry(g, slots[i], (int)(b.length[(size_t)slots[i]] / b.page_tokens))) > 1) {
+        --holders(b.entry(g, slots[i], (int)(b.length[(size_t)slots[i]] / b.page_tokens)));
+        ++out[gi];
+      }
+    }
+  }
+  return 0;
+}
+
 HK_API void hk_books_free_pages(void* h, int* out) {
   Books& b = *static_cast<Books*>(h);
   for (size_t g = 0; g < b.groups.size(); ++g) out[g] = (int)b.groups[g].pool.free_list.size();

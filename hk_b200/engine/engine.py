@@ -313,8 +313,7 @@ class Engine:
         books = self.cache.books
         total = 0
         seen = set()
-        take = [0] * len(books.groups)
-        shared: Dict[tuple, list] = {}         # (group, page) that several hold -> [writers in this step, holders]
+        slots = []
         trees = any(e.parents is not None for e in entries)
         if trees and not self.takes_trees:
             raise EngineError("this model does not take trees of drafted tokens (a mixer keeps a state, or an attention that knows no trees)")
@@ -343,19 +342,11 @@ class Engine:
                 raise ContextFull(
                     f"request {e.request!r} would reach {int(books.length[slot]) + n} tokens; the context holds {books.max_context}")
             total += n
-            # pages the window has passed come back before any are taken
-            passed = books.pages_passed(slot)
-            for gi, k in enumerate(books.pages_to_take(slot, n)):
-                take[gi] += k - passed[gi]
-            for gi, (page, holders) in enumerate(books.shared_pages(slot)):
-                if page >= 0:
-                    shared.setdefault((gi, page), [0, holders])[0] += 1
-        for (gi, _), (writers, holders) in shared.items():
-            if writers == holders:             # the last of a page's holders writes it where it is
-                take[gi] -= 1
+            slots.append(slot)
         if total > self.max_batch_tokens:
             raise BatchTooLarge(f"{total} tokens in one step; the engine takes {self.max_batch_tokens}")
-        for gi, k in enumerate(take):
+        # pages the windows have passed come back before any are taken
+        for gi, k in enumerate(books.step_pages(slots, [len(e.tokens) for e in entries])):
             if k > books.groups[gi].pool.free_count:
                 raise OutOfPages(f"the step needs {k} more pages in group {gi}; {books.groups[gi].pool.free_count} are free")
 
