@@ -195,7 +195,8 @@ class PagedCache:
         """Makes the copies that the books owe and uploads the block-table rows that changed since the last call.  The copies read
         pageable host memory, so they are complete (staged) when the call returns and the
         books may change again at once."""
-        self._copy_pages()
+        if self.books.owes_copies():         # (8 us a step otherwise, for nothing in all steps without forks)
+            self._copy_pages()
         if not self.books.dirty:
             return
         if len(self.books.dirty) > 4:            # many rows (a batch of beams): one upload, not one a row

@@ -227,6 +227,10 @@ class CacheBooks:
         self._check(self._rt.hk_books_shared_page(self._h, int(slot), self._take, self._holders))
         return list(zip(self._take[:len(self.groups)], self._holders[:len(self.groups)]))
 
+    def owes_copies(self) -> bool:
+        """Whether `take_copies` has any to give."""
+        return self._rt.hk_books_copies(self._h, None, 0) > 0
+
     def take_copies(self) -> np.ndarray:
         """The copies owed since the last call, in order: int32 [n, 4] = (group, from page, to page, rows)."""
         n = int(self._rt.hk_books_copies(self._h, None, 0))

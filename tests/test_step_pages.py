@@ -97,3 +97,26 @@ def test_what_is_refused_would_not_have_fitted(seed):
             books.audit()
             tight += min(books.free_pages()) == 0 < min(before)
     assert refused > 0 and tight > 0
+
+
+def test_steps_without_forks_ask_for_no_copies(monkeypatch):
+    import torch
+
+    from hk_b200.cache.device import PagedCache
+    from hk_b200.parts.base import KVCacheSpec, Precision
+    cache = PagedCache([KVCacheSpec(2, 4)], Precision(torch.float32, torch.device("cpu")), 4, 8, 3, 32)
+    taken = []
+    take = cache.books.take_copies
+    monkeypatch.setattr(cache.books, "take_copies", lambda: taken.append(1) or take())
+    a = cache.open()
+    for n in (6, 1, 1):
+        cache.books.extend(a, n)
+        cache.sync_tables()
+    assert not taken
+    cache.books.extend(cache.fork([a])[0], 1)          # at a full page: no copy either
+    cache.sync_tables()
+    assert not taken
+    cache.books.extend(a, 1)
+    cache.books.extend(cache.fork([a])[0], 1)
+    cache.sync_tables()
+    assert taken == [1] and not cache.books.owes_copies()
