@@ -17,6 +17,7 @@ from typing import List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from ..cache.pages import OutOfPages, TooManyRequests
 from ..csrc import ops
 from ..csrc.ops import BEAM_CHOICES
 from .engine import Engine, EngineError, StepEntry
@@ -49,6 +50,8 @@ class BeamSearch:
             raise ValueError("max_new_tokens must be at least 1")
         if beams > engine.cache.books.max_requests:
             raise ValueError(f"{beams} beams need as many request slots; the engine has {engine.cache.books.max_requests}")
+        if beams > engine.max_batch_tokens:
+            raise ValueError(f"{beams} beams are as many tokens a step; the engine takes {engine.max_batch_tokens}")
         self.engine, self.beams, self.most, self.penalty = engine, int(beams), int(max_new_tokens), float(length_penalty)
         self.eos = set(int(t) for t in eos_token_ids if 0 <= int(t) < engine.vocab)
         self.chunk = max(1, min(int(prefill_chunk), engine.max_batch_tokens))
@@ -62,8 +65,14 @@ class BeamSearch:
                 raise EngineError(f"a prompt of {len(p)} tokens and {self.most} new ones pass the context of {self.engine.max_context}")
         at_once = max(1, min(self.engine.cache.books.max_requests, self.engine.max_batch_tokens) // self.beams)
         out: List[List[Continuation]] = []
-        for i in range(0, len(plist), at_once):
-            out += self._group(plist[i:i + at_once])
+        while len(out) < len(plist):
+            group = plist[len(out):len(out) + at_once]
+            try:
+                out += self._group(group)
+            except (OutOfPages, TooManyRequests):
+                if len(group) == 1:
+                    raise
+                at_once = len(group) // 2        # pages, or slots that other requests leave, for fewer
         self.engine.check_kernel_status()
         return out
 

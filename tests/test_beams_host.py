@@ -21,9 +21,15 @@ class FakeEngine:
         self.texts = {}
         self.steps = []
 
-    def open_request(self, name):
+    def take_slot(self, name, tokens):
+        from hk_b200.cache.pages import TooManyRequests
         assert name not in self.texts
-        self.texts[name] = []
+        if len(self.texts) == self.cache.books.max_requests:
+            raise TooManyRequests("no slot")
+        self.texts[name] = tokens
+
+    def open_request(self, name):
+        self.take_slot(name, [])
 
     def close_request(self, name):
         del self.texts[name]
@@ -32,8 +38,7 @@ class FakeEngine:
         return name in self.texts
 
     def fork_request(self, name, new):
-        assert new not in self.texts
-        self.texts[new] = list(self.texts[name])
+        self.take_slot(new, list(self.texts[name]))
 
     def reorder(self, names, parents):
         old = [list(self.texts[n]) for n in names]
@@ -41,7 +46,6 @@ class FakeEngine:
             self.texts[n] = list(old[p])
 
     def step(self, entries):
-        assert len(self.texts) <= self.cache.books.max_requests
         self.steps.append(sum(len(e.tokens) for e in entries))
         rows = []
         for e in entries:
@@ -151,3 +155,52 @@ def test_every_token_ends(choice):
     got = BeamSearch(FakeEngine(logits_of, vocab), 3, 5, 1.0, range(vocab)).run([[1]])[0]
     agree(got, all_continuations(logits_of, vocab, [1], 3, 5, 1.0, set(range(vocab))), 5)
     assert [c.tokens for c in got] == [[]] * 3 and all(c.ended for c in got)
+
+
+class SmallPool(FakeEngine):
+    """The same with room for `most` tokens in all requests together."""
+
+    def __init__(self, logits_of, vocab, most, **options):
+        super().__init__(logits_of, vocab, **options)
+        self.most = most
+
+    def step(self, entries):
+        from hk_b200.cache.pages import OutOfPages
+        if sum(map(len, self.texts.values())) + sum(len(e.tokens) for e in entries) > self.most:
+            raise OutOfPages("no room")
+        return super().step(entries)
+
+
+@pytest.mark.parametrize("most", [30, 45, 60, 1000])
+def test_prompts_that_do_not_fit_together(most, choice):
+    """Fewer prompts at once where the pool has no room for as many as there are slots; an error only where one alone has none."""
+    from hk_b200.cache.pages import OutOfPages
+    logits_of = random_model(2, 11, {3}, 2.0)
+    prompts = [[1, 2], [3], [4, 5, 6], [7], [8, 9]]
+    eng = SmallPool(logits_of, 11, most)
+    got = BeamSearch(eng, 3, 6, 1.0, (3,)).run(prompts)
+    for p, mine in zip(prompts, got):
+        agree(mine, all_continuations(logits_of, 11, p, 3, 6, 1.0, {3}), 6)
+    assert not eng.texts
+    with pytest.raises(OutOfPages):
+        BeamSearch(SmallPool(logits_of, 11, 10), 3, 6, 1.0, (3,)).run(prompts)
+
+
+def test_slots_that_other_requests_hold(choice):
+    logits_of = random_model(2, 11, {3}, 2.0)
+    eng = FakeEngine(logits_of, 11, max_requests=12)
+    for i in range(5):
+        eng.open_request(i)
+    prompts = [[1, 2], [3], [4, 5, 6], [7], [8, 9]]
+    got = BeamSearch(eng, 3, 6, 1.0, (3,)).run(prompts)
+    for p, mine in zip(prompts, got):
+        agree(mine, all_continuations(logits_of, 11, p, 3, 6, 1.0, {3}), 6)
+    assert sorted(eng.texts) == list(range(5))
+
+
+def test_more_beams_than_a_step_takes():
+    """Known before any prompt is read."""
+    eng = FakeEngine(random_model(1, 11, set(), 0.0), 11, max_batch_tokens=7)
+    BeamSearch(eng, 7, 4)
+    with pytest.raises(ValueError):
+        BeamSearch(eng, 8, 4)
