@@ -689,11 +689,13 @@ int beam_groups(int choices) {
   return g;
 }
 
-// How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part,
-// of rows with 32 tiles and more a tile (more parts than a warp has lanes take the choice longer than they save: 4 rows of 151,936
-// 14.6 us in half tiles, 12.6 in whole ones).
+// How many parts a row is cut into, a length of 4 values and more: one wave of CTAs (four a SM), and no less than half a tile a part, of
+// rows of 16 tiles and more a tile: the stream is shorter with more parts and the choice behind it longer.  In half and in whole tiles, 4
+// rows take 12.8 and 15.5 us at 32,000 logits, 12.4 and 15.4 at 50,304, 12.6 and 12.5 at 65,536, 14.1 and 12.7 at 100,352, 15.3 and 13.8 at
+// 151,936; 8 rows 12.8 and 15.7, 13.4 and 15.3, 13.5 and 12.6, 15.1 and 13.9, 16.9 and 14.8.  (The other way round of what was measured: 1
+// row of 32,000 14.5 and 12.0, 2 of 128,256 and of 151,936 12.9 and 15.0, 13.7 and 15.4.)
 void beam_cut(int rows, int V, int* parts, int* length) {
-  const int wave = 148 * 4, tile = BT * BE, least = V >= 32 * tile ? tile : tile / 2, most = (V - 1) / least + 1;
+  const int wave = 148 * 4, tile = BT * BE, least = V >= 16 * tile ? tile : tile / 2, most = (V - 1) / least + 1;
   int n = wave / rows;
   n = n < 1 ? 1 : n > most ? most : n;
   *length = ((V + n - 1) / n + 3) & ~3;
