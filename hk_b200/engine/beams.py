@@ -20,7 +20,7 @@ import torch
 from ..cache.pages import OutOfPages, TooManyRequests
 from ..csrc import ops
 from ..csrc.ops import BEAM_CHOICES
-from .engine import Engine, EngineError, StepEntry
+from .engine import Engine, EngineError, StepEntry, check_prompt
 
 
 @dataclass
@@ -59,8 +59,7 @@ class BeamSearch:
     def run(self, prompts: Sequence[Sequence[int]]) -> List[List[Continuation]]:
         plist = [[int(t) for t in p] for p in prompts]
         for p in plist:
-            if not p:
-                raise ValueError("the prompt has no tokens")
+            check_prompt(self.engine, p)
             if len(p) + self.most - 1 > self.engine.max_context:
                 raise EngineError(f"a prompt of {len(p)} tokens and {self.most} new ones pass the context of {self.engine.max_context}")
         at_once = max(1, min(self.engine.cache.books.max_requests, self.engine.max_batch_tokens) // self.beams)

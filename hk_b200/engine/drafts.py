@@ -16,7 +16,8 @@ from typing import Dict, List, Optional, Sequence, Tuple
 from ..cache.pages import OutOfPages
 from ..csrc.ops import TREE_TOKENS
 from ..sampling import Sampler, SamplingParams, SamplingState
-from .engine import Engine, EngineError, StepEntry
+from .engine import Engine, EngineError, StepEntry, check_prompt
+from .scheduler import fits_alone
 
 
 class LookupDrafts:
@@ -99,13 +100,16 @@ class DraftDecoder:
 
     def run(self, prompts: Sequence[Sequence[int]], params: Sequence[SamplingParams]) -> List[List[int]]:
         plist = [[int(t) for t in p] for p in prompts]
-        if any(not p for p in plist):
-            raise ValueError("the prompt has no tokens")
+        if len(params) != len(plist):
+            raise ValueError(f"{len(plist)} prompts and {len(params)} of sampling parameters")
         if any(p.adjusts_logits for p in params):
             raise ValueError("penalties and biases follow the tokens drawn so far: they cannot be had with drafted tokens")
         for p in plist:
+            check_prompt(self.engine, p)
             if len(p) > self.engine.max_context:
                 raise EngineError(f"the prompt has {len(p)} tokens; the context holds {self.engine.max_context}")
+            if not fits_alone(self.engine.cache.books, min(len(p) + self.most - 1, self.engine.max_context), self.engine.max_batch_tokens):
+                raise OutOfPages(f"a prompt of {len(p)} tokens and its continuation need more pages than there are")
         out: List[List[int]] = [[] for _ in plist]
         waiting = deque(_Request(i, LookupDrafts(p), SamplingState.start(s, p)) for i, (p, s) in enumerate(zip(plist, params)))
         running: List[_Request] = []

@@ -43,6 +43,15 @@ class UnknownRequest(EngineError):
     pass
 
 
+def check_prompt(engine, prompt: Sequence[int]) -> None:
+    """Raises what makes a prompt of token ids none for this model."""
+    if not prompt:
+        raise ValueError("the prompt has no tokens")
+    for t in prompt:
+        if not 0 <= t < engine.vocab:
+            raise TokenOutOfRange(f"token id {t} is outside the vocabulary of {engine.vocab}")
+
+
 class KernelTimeout(EngineError):
     pass
 

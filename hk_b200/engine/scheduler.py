@@ -74,6 +74,14 @@ class _SampledTokens:
     event: object
 
 
+def fits_alone(books, tokens: int, batch_tokens: int) -> bool:
+    """Whether the pools could hold a request of `tokens` tokens, read up to `batch_tokens` a step, if it were the only one."""
+    pages = -(-tokens // books.page_tokens)
+    return not (any(pages > g.pool.num_pages for g in books.groups if g.window is None) or
+                any(min(pages, -(-(g.window + batch_tokens) // books.page_tokens) + 1) > g.pool.num_pages
+                    for g in books.groups if g.window is not None))
+
+
 class Scheduler:
     def __init__(self, engine, sampler=None, max_batch_tokens: Optional[int] = None, prefill_chunk: int = 512,
                  eos_token_ids: Sequence[int] = (), run_ahead: bool = True):
@@ -108,11 +116,8 @@ class Scheduler:
             raise RequestRefused(f"the prompt has {len(prompt)} tokens; the context holds {self.engine.max_context}")
         # the most the request can ever hold: its prompt and all but the last generated token
         most = min(len(prompt) + max_new_tokens - 1, self.engine.max_context)
-        pages = -(-most // self.books.page_tokens)
-        if any(pages > g.pool.num_pages for g in self.books.groups if g.window is None) or \
-                any(min(pages, -(-(g.window + self.max_batch_tokens) // self.books.page_tokens) + 1) > g.pool.num_pages
-                    for g in self.books.groups if g.window is not None):
-            raise RequestRefused(f"the request needs {pages} pages alone; the pool has fewer")
+        if not fits_alone(self.books, most, self.max_batch_tokens):
+            raise RequestRefused(f"the request needs {-(-most // self.books.page_tokens)} pages alone; the pool has fewer")
         req = Request(self._next_id, prompt, int(max_new_tokens),
                       SamplingState.start(params or SamplingParams(), prompt))
         self._next_id += 1

@@ -204,3 +204,27 @@ def test_more_beams_than_a_step_takes():
     BeamSearch(eng, 7, 4)
     with pytest.raises(ValueError):
         BeamSearch(eng, 8, 4)
+
+
+@pytest.mark.parametrize("bad", [[], [11], [-1], [3, 4, 99]])
+def test_prompts_are_looked_at_before_any_is_read(bad, choice):
+    from hk_b200.engine import EngineError
+    eng = FakeEngine(random_model(1, 11, set(), 0.0), 11)
+    with pytest.raises((EngineError, ValueError)):
+        BeamSearch(eng, 2, 4).run([[1], [2], bad])
+    assert not eng.steps
+
+
+def test_drafted_requests_are_looked_at_before_any_is_read():
+    """As the scheduler does: tokens outside the vocabulary, more than the pool holds, and sampling parameters for each prompt."""
+    from hk_b200.cache import CacheBooks, OutOfPages
+    from hk_b200.engine import DraftDecoder, EngineError
+    from hk_b200.sampling import SamplingParams
+    eng = FakeEngine(random_model(1, 11, set(), 0.0), 11, max_context=64)
+    eng.takes_trees, eng.cache.books = True, CacheBooks([None], page_tokens=4, num_pages=5, max_requests=3, max_context=64)
+    greedy = SamplingParams(temperature=0.0)
+    for prompts, n, kind in (([[1], []], 2, ValueError), ([[1], [11]], 2, EngineError), ([[1], [2, -1]], 2, EngineError), ([[1], [2]], 1, ValueError),
+                             ([[1], [2]], 3, ValueError), ([[1], [2] * 65], 2, EngineError), ([[1], [2] * 17], 2, OutOfPages)):
+        with pytest.raises(kind):
+            DraftDecoder(eng, 3, 5, sampler=object()).run(prompts, [greedy] * n)
+    assert not eng.steps
