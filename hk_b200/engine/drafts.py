@@ -4,8 +4,9 @@ The guesses come from the request's own tokens (`LookupDrafts`): where its last 
 a guess at what comes now; several such places make a tree.  A step runs the request's last token and the tree behind it
 (`StepEntry.parents`), a token is drawn at every node from the logits there, and the path along which the tree guessed right is kept
 (`Engine.accept`).  What is drawn at a node is what a step by step decoding would have drawn in its place (the same logits, the same
-place of the request's random stream), so the output is the same: only the number of steps is smaller.  (In bfloat16 a node's logits
-can differ from a single step's in the last bits, as they do between batch sizes.)
+place of the request's random stream), so the output is the same: only the number of steps is smaller.  (In bfloat16 the logits of a
+step with guesses can differ from a single step's in the last bits, as they do between batch sizes, and so can what is drawn where two
+tokens are that close.  A step in which no request has a guess is a single step.)
 """
 from __future__ import annotations
 
@@ -180,6 +181,8 @@ class DraftDecoder:
             tokens, parents = r.drafts.tree(room) if room > 0 else ([], [])
             trees.append(([r.pending] + tokens, [-1] + [p + 1 for p in parents]))
             entries.append(StepEntry(name, trees[-1][0], list(range(len(trees[-1][0]))), trees[-1][1]))
+        if all(len(tokens) == 1 for tokens, _ in trees):       # nobody has a guess: a step by step decoding's step, captured as that one is
+            entries = [StepEntry(e.request, e.tokens, [0]) for e in entries]
         return trees, entries
 
     def _step(self, running: List[_Request], waiting, names, out) -> None:
@@ -226,7 +229,8 @@ class DraftDecoder:
             self.stats.tokens += len(r.output) - before
             r.sampling.drawn += len(new)
             if goes_on:
-                accepted[name] = path
+                if entries[0].parents is not None:
+                    accepted[name] = path
                 going.append(r)
             else:
                 self._close(name, names)
