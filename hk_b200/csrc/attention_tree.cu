@@ -136,7 +136,7 @@ __device__ __forceinline__ uint32_t visible32(const TreeRow& w, int j0) {
   return see;
 }
 
-// cap c and scale as the tensor-core and float32 kernels use them, in the base-2 domain: c log2(e) tanh(s / c)
+// cap c and scale as the tensor-core kernel uses them, in the base-2 domain: c log2(e) tanh(s / c)
 __device__ __forceinline__ float log2_score(float raw, float scale_log2, float cap_log2, float cap_in2) {
   if (cap_log2 > 0.f) {
     // C - 2 C / (e^(2z) + 1), z = score / c: saturates the right way at both ends, absolute error of the tanh about 2e-7
@@ -498,9 +498,14 @@ int launch_generic(const TreeArgs& a, cudaStream_t s) {
 // Bound by a stream's own way around, some 3,500 clocks a tile: 170 until the first scores are in registers, 1,200 of exponentials (512
 // alone), 300 until the tensor core's lane has seen them and has its turn, 900 for the products and their announcement, of which shared
 // memory's bandwidth takes 640 (a product of 64 keys reads 128 rows of Q: 6 KB in 32 clocks' work).  The exponentials' unit is active 58 %
-// of that, shared memory 73 %.  (64 tokens behind 131,001 rows, 144 us: scores of 128 keys at once, two streams, 153; an eighth, a
-// quarter and a third of the exponentials by a polynomial 145, 146 and 147; the turn passed on behind the product with V 145; tiles asked
-// into L2 ahead 148.)
+// of that, shared memory 73 %.
+// Probabilities are rounded to bfloat16 for the product with V, as the tensor core takes both operands in one type; their sum is of the
+// unrounded ones.  That is an error of up to 2^-8 of each term beside the 2^-8 of the result's own rounding: 0.0024 of the result's norm
+// against 0.0017 of a result that is rounded once (rows of independent values: each rounding is 0.0017).  Two products, with the rounding's
+// remainder in the second, would take it away for half as many products again.
+//
+// Dropped (64 tokens behind 131,001 rows, 144 us): scores of 128 keys at once, two streams, 153; an eighth, a quarter and a third of the
+// exponentials by a polynomial 145, 146 and 147; the turn passed on behind the product with V 145; tiles asked into L2 ahead 148.
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_SOFTMAX = 512, TC_THREADS = TC_SOFTMAX + 128;
 typedef Cut<2 * TC_ROWS, TC_KEYS, 4> TcCut;
 constexpr float MUCH = 16777216.0f, TOO_MUCH = 1152921504606846976.0f;      // 2^24, 2^60
@@ -787,7 +792,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
-  pdl_launch_dependents();
+  pdl_launch_dependents();             // not before the wait: tree_combine_kernel reads the requests ahead of its own
   if (warp == 0) {
     Walk w = share_start<TcCut>(a, blockIdx.x, gridDim.x).w;
     Segment s;
@@ -1276,7 +1281,7 @@ __global__ void __launch_bounds__(F32_THREADS, 4) tree_f32_kernel(const TreeArgs
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, group = a.group;
   const float* qp = reinterpret_cast<const float*>(a.q);
   pdl_wait();
-  pdl_launch_dependents();
+  pdl_launch_dependents();             // not before the wait: tree_combine_kernel reads the requests ahead of its own
   if (tid < 32) {
     const Walk w = share_start<F32Cut>(a, blockIdx.x, gridDim.x).w;
     if (tid == 0) sm.start = w;
