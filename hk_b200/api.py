@@ -62,7 +62,8 @@ def generate_with_engine(engine: Engine, prompts, max_new_tokens: int = 20, temp
     temperature 0 picks the most likely token.  With seed != 0, request i draws from the
     stream of seed + i, so results do not depend on batching.  `run_ahead`: launch a decode step before
     the host has read the previous step's tokens (same tokens, less idle GPU time).  `draft_tokens` N > 0: a step verifies up to N
-    tokens guessed from the request's own text (`engine/drafts.py`); the output is the same, penalties are not taken."""
+    tokens guessed from the request's own text (`engine/drafts.py`); the output is the same (in bfloat16 but for tokens whose logits lie within its last bits), penalties are
+    not taken."""
     plist, _ = _as_prompts(prompts)
     if eos_token_ids is None:
         eos_token_ids = getattr(engine.config, "eos_token_ids", ())

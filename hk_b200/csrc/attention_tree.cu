@@ -14,10 +14,10 @@
 // CTA), which `tree_combine_kernel` merges in order.
 // Nothing depends on the host but bounds on the sizes: a launch can be captured and replayed over other contexts.
 //
-// Measured (32 heads over 8 key heads of 128, captured and replayed): 16 tokens behind 2,000 rows 16.5 us, all of it the start and end of
+// Measured (32 heads over 8 key heads of 128, captured and replayed): 16 tokens behind 2,000 rows 16.6 us, all of it the start and end of
 // the two kernels (8.5 MB); 8 requests of 32 tokens, ragged up to 8,000 rows, 41 us (122 MB, 3.0 TB/s); 32 requests of 64 tokens behind up to
-// 8,192 rows 182 us (680 MB, 3.7 TB/s, 632 TFLOP/s); 64 tokens behind 131,001 rows 142 us (968 TFLOP/s); the last two at the power cap,
-// called again and again for a second, 210 and 165.  The generic kernel took 391, 4,463, 47,593 and 76,055.
+// 8,192 rows 184 us (680 MB, 3.7 TB/s, 625 TFLOP/s); 64 tokens behind 131,001 rows 144 us (954 TFLOP/s); the last two at the power cap,
+// called again and again for a second, 209 to 217 and 164 to 172.  The generic kernel took 391, 4,463, 47,593 and 76,055.
 //
 // What the device arrays say is checked where it is read: a request whose slot, rows or lengths lie outside the arrays or the bounds is
 // skipped, and the keys of a page that is not in the pool are not seen.

@@ -93,7 +93,7 @@ __device__ __forceinline__ void move_rows(const RowArray& a, const int2* from, c
 // A block takes a request and some neighbouring arrays, and finds the pages of its path once for all that share a block table: finding
 // them is a chain of three reads, and as long as moving an array's rows.  Bound by the reads' and writes' way through DRAM in pieces of
 // a row of a head (256 bytes): 64 requests of up to nine rows in 72 arrays, 42 MB, take 13.4 us one call behind the other, 3.2 TB/s, and
-// 15.5 as replays over three caches in turn (over two, which partly stay in L2: 14.4, in blocks of 256 threads 17.4, of 64 14.4, with
+// 15.2 as replays over three caches in turn (over two, which partly stay in L2: 13.5, through L1 14.1; through it in blocks of 256 threads 17.4, of 64 14.4, with
 // four reads a thread on their way 16.5, 16 requests 6.2).
 __global__ void __launch_bounds__(KEEP_THREADS, 8)
 compact_rows_kernel(const RowArray* __restrict__ table, int arrays, int per_block, const int* __restrict__ paths, int width, int table_rows,
